@@ -1,0 +1,383 @@
+// Matrix product with bias, activation and residual in its epilogue, and its gradients:
+// dd_linear_fwd, dd_linear_bwd_data, dd_linear_bwd_weight, dd_linear_act_bwd.
+//
+//   y = act(z) + res,  z[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]
+//   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz
+//
+// bf16 (16 x 16-bit products per matrix instruction step) or e4m3 (twice the rate, half the bytes);
+// sums in fp32.  All three products are P Q^T with different storage orders: an operand is
+// contraction-contiguous (KC) or row-contiguous (RC).
+#include "block_core.h"
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// What happens to a finished sum on its way out.
+struct Epi {
+  void* y; long ldy; int ytype;
+  const float* bias;
+  int act;
+  const void* res; long ldr;
+  __bf16* z; long ldz;
+  const float* xs; const float* wsc;
+  int accumulate;
+  int vec;         // 16-byte accesses are aligned for every operand above
+};
+
+__device__ __forceinline__ float act_any(int act, float z) {
+  switch (act) {
+    case DD_ACT_ELU: return act_f<DD_ACT_ELU>(z);
+    case DD_ACT_SILU: return act_f<DD_ACT_SILU>(z);
+    case DD_ACT_GELU: return act_f<DD_ACT_GELU>(z);
+    default: return z;
+  }
+}
+
+// V consecutive outputs of row m from column n; V == 8 needs e.vec and n + 8 <= N.
+template <int V>
+__device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V]) {
+  if (e.xs) {
+    const float s = e.xs[m];
+    float w[V];
+    load_f32<V>(e.wsc + n, w);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = v[j] * s * w[j];
+  }
+  if (e.bias) {
+    float b[V];
+    load_f32<V>(e.bias + n, b);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += b[j];
+  }
+  // the pre-activation is kept in bf16 for the backward pass (the derivative is read from it: an
+  // error of 2^-9 relative, the size of the rounding of the gradients themselves)
+  if (e.z) store_bf16<V>(e.z + m * e.ldz + n, v);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = act_any(e.act, v[j]);
+  if (e.res) {
+    float r[V];
+    if (e.ytype == DD_F32) load_f32<V>((const float*)e.res + m * e.ldr + n, r);
+    else load_bf16<V>((const __bf16*)e.res + m * e.ldr + n, r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += r[j];
+  }
+  if (e.ytype == DD_F32) {
+    float* p = (float*)e.y + m * e.ldy + n;
+    if (e.accumulate) {
+      float o[V];
+      load_f32<V>(p, o);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += o[j];
+    }
+    store_f32<V>(p, v);
+  } else {
+    __bf16* p = (__bf16*)e.y + m * e.ldy + n;
+    if (e.accumulate) {
+      float o[V];
+      load_bf16<V>(p, o);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += o[j];
+    }
+    store_bf16<V>(p, v);
+  }
+}
+
+// An operand: R rows (of the output's rows or columns), contraction length K.
+struct Mat { const void* p; long ld; int R; int vec; };
+
+constexpr int ROWB = 128;         // bytes of the contraction per tile row
+constexpr int LROW = ROWB + 16;   // LDS row: 16 bytes more, so that 16-byte reads of 8 rows fall on different banks
+
+// General kernel: 64 x 64 tile, four waves of 32 x 32, operands staged through registers with bounds
+// checks on every element that needs them: any size, order and alignment.
+template <int ES, bool RC>
+__device__ __forceinline__ void stage(const Mat& a, long r0, long k0, int K, char* sh) {
+  constexpr int PER = 16 / ES, BK = ROWB / ES;
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int ch = threadIdx.x + it * 256;
+    if constexpr (!RC) {
+      const int r = ch >> 3, kc = (ch & 7) * PER;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r0 + r < a.R) {
+        const char* p = (const char*)a.p + ((r0 + r) * a.ld + k0 + kc) * ES;
+        if (a.vec && k0 + kc + PER <= K) {
+          v = *reinterpret_cast<const uint4*>(p);
+        } else {
+          unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (k0 + kc + j < K) {
+              if constexpr (ES == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
+              else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
+            }
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      *reinterpret_cast<uint4*>(sh + r * LROW + kc * ES) = v;
+    } else {
+      // 8 consecutive rows of one k, written one by one into their K-contiguous rows
+      const int k = ch >> 3, rr = (ch & 7) * 8;
+      unsigned short e[8] = {};
+      if (k0 + k < K) {
+        const unsigned short* p = (const unsigned short*)a.p + (k0 + k) * a.ld + r0 + rr;
+        if (a.vec && r0 + rr + 8 <= a.R) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          *reinterpret_cast<uint4*>(e) = v;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (r0 + rr + j < a.R) e[j] = p[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) *reinterpret_cast<unsigned short*>(sh + (rr + j) * LROW + k * 2) = e[j];
+      (void)BK;
+    }
+  }
+}
+
+template <int ES, bool P_RC, bool Q_RC>
+__global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int kspan, float* slabs, Epi e) {
+  __shared__ __attribute__((aligned(16))) char sh[2 * 64 * LROW];
+  char* shp = sh;
+  char* shq = sh + 64 * LROW;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long m0 = (long)blockIdx.x * 64, n0 = (long)blockIdx.y * 64;
+  const long kb = (long)blockIdx.z * kspan;
+  const int kend = (int)min((long)K, kb + kspan);
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32, r = lane & 31, half = lane >> 5;
+  f32x16 acc = {};
+  for (long k0 = kb; k0 < kend; k0 += ROWB / ES) {
+    stage<ES, P_RC>(P, m0, k0, kend, shp);
+    stage<ES, Q_RC>(Q, n0, k0, kend, shq);
+    __syncthreads();
+    // Q is the instruction's first operand: a lane then holds four consecutive columns of one row
+    if constexpr (ES == 2) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const bf16x8 q = *reinterpret_cast<const bf16x8*>(shq + (wn + r) * LROW + s * 32 + half * 16);
+        const bf16x8 p = *reinterpret_cast<const bf16x8*>(shp + (wm + r) * LROW + s * 32 + half * 16);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, p, acc, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        i32x8 q, p;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int o = s * 64 + half * 32 + h * 16;
+          const uint4 a = *reinterpret_cast<const uint4*>(shq + (wn + r) * LROW + o);
+          const uint4 b = *reinterpret_cast<const uint4*>(shp + (wm + r) * LROW + o);
+          q[4 * h] = a.x; q[4 * h + 1] = a.y; q[4 * h + 2] = a.z; q[4 * h + 3] = a.w;
+          p[4 * h] = b.x; p[4 * h + 1] = b.y; p[4 * h + 2] = b.z; p[4 * h + 3] = b.w;
+        }
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(q, p, acc, 0, 0, 0, 127, 0, 127);
+      }
+    }
+    __syncthreads();
+  }
+  // the 64 x 64 sums through LDS, so that a lane finishes eight consecutive columns
+  float* out = reinterpret_cast<float*>(sh);
+#pragma unroll
+  for (int t = 0; t < 16; ++t) out[(wm + r) * 68 + wn + 8 * (t / 4) + 4 * half + t % 4] = acc[t];
+  __syncthreads();
+  for (int it = 0; it < 2; ++it) {
+    const int ch = threadIdx.x + it * 256, mr = ch >> 3, nc = (ch & 7) * 8;
+    const long m = m0 + mr, n = n0 + nc;
+    if (m >= P.R) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = out[mr * 68 + nc + j];
+    if (slabs) {
+      float* p = slabs + ((long)blockIdx.z * P.R + m) * Q.R + n;
+      for (int j = 0; j < 8; ++j)
+        if (n + j < Q.R) p[j] = v[j];
+    } else if (e.vec && n + 8 <= Q.R) {
+      finish<8>(e, m, n, v);
+    } else {
+      for (int j = 0; j < 8; ++j)
+        if (n + j < Q.R) { float t[1] = {v[j]}; finish<1>(e, m, n + j, t); }
+    }
+  }
+}
+
+// Sum of the partial results of a split contraction, slabs ascending, and the epilogue.
+__global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, Epi e) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long MN = M * N;
+  if (e.vec && N % 8 == 0) {
+    if (i * 8 >= MN) return;
+    float v[8], t[8];
+    load_f32<8>(slabs + i * 8, v);
+    for (int s = 1; s < S; ++s) {
+      load_f32<8>(slabs + s * MN + i * 8, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    finish<8>(e, i * 8 / N, i * 8 % N, v);
+  } else {
+    for (long q = i; q < MN; q += (long)gridDim.x * 256) {
+      float v[1] = {slabs[q]};
+      for (int s = 1; s < S; ++s) v[0] += slabs[s * MN + q];
+      finish<1>(e, q / N, q % N, v);
+    }
+  }
+}
+
+// Splits of a contraction: none where the tiles alone fill the chip.
+inline int pick_splits(long tiles, int ktiles, size_t slab_bytes, size_t ws_bytes) {
+  if (tiles >= 256 || ktiles < 8) return 1;
+  long s = min(512 / tiles, (long)ktiles / 4);
+  while (s > 1 && slab_bytes * (size_t)s > ws_bytes) --s;
+  return (int)max(s, 1l);
+}
+
+template <int ES, bool P_RC, bool Q_RC>
+int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+  const int bk = ROWB / ES;
+  const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));
+  DD_REQUIRE(tiles.y <= 65535, "dd_linear: more than 4194240 output columns");
+  const int ktiles = dd_ceil_div(K, bk);
+  const int S = pick_splits((long)tiles.x * tiles.y, ktiles, sizeof(float) * (size_t)P.R * Q.R, ws ? ws_bytes : 0);
+  const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
+  k_linear_any<ES, P_RC, Q_RC><<<dim3(tiles.x, tiles.y, parts), 256, 0, st>>>(P, Q, K, kspan, parts > 1 ? ws : nullptr, e);
+  DD_CHECK_LAUNCH(who);
+  if (parts > 1) {
+    const long work = (long)P.R * Q.R / (e.vec && Q.R % 8 == 0 ? 8 : 1);
+    k_linear_finish<<<dd_ceil_div(work, 256), 256, 0, st>>>(ws, parts, P.R, Q.R, e);
+    DD_CHECK_LAUNCH(who);
+  }
+  return 0;
+}
+
+// dz = dy act'(z), and the workgroup's share of dbias.  act 0: dz == dy, only the column sums.
+template <int V>
+__global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz,
+                                                 int act, float* parts, int M, int N, int rows_per) {
+  const long c = ((long)blockIdx.x * 256 + threadIdx.x) * V;
+  if (c >= N) return;
+  float sum[V] = {};
+  const long m0 = (long)blockIdx.y * rows_per, m1 = min((long)M, m0 + rows_per);
+  for (long m = m0; m < m1; ++m) {
+    float d[V], t[V];
+    load_bf16<V>(dy + m * ldy + c, d);
+    if (act != DD_ACT_NONE) {
+      load_bf16<V>(z + m * ldz + c, t);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        switch (act) {
+          case DD_ACT_ELU: d[j] *= act_slope<DD_ACT_ELU>(t[j]); break;
+          case DD_ACT_SILU: d[j] *= act_slope<DD_ACT_SILU>(t[j]); break;
+          default: d[j] *= act_slope<DD_ACT_GELU>(t[j]);
+        }
+      }
+      // bf16: the two products that read dz take bf16 operands
+      store_bf16<V>(dz + m * lddz + c, d);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] += d[j];
+  }
+  if (parts) store_f32<V>(parts + (long)blockIdx.y * N + c, sum);
+}
+
+__global__ void __launch_bounds__(1024) k_bias_sum(const float* parts, int n, int N, void* out, int type, int accumulate) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  float t = 0.f;
+  if (c < N)
+    for (int i = w; i < n; i += 16) t += parts[(long)i * N + c];
+  sh[w][lane] = t;
+  __syncthreads();
+  if (w || c >= N) return;
+  t = sh[0][lane];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) t += sh[i][lane];
+  if (type == DD_F32) { float* p = (float*)out + c; *p = accumulate ? *p + t : t; }
+  else { __bf16* p = (__bf16*)out + c; *p = (__bf16)(accumulate ? (float)*p + t : t); }
+}
+
+inline int mat_vec(const void* p, long ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
+inline bool out_vec(const void* p, long ld, int type) { return p == nullptr || rows_aligned(p, ld, type, 16); }
+
+}  // namespace
+
+extern "C" int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
+                             const float* w_scale, const float* bias, int act, const void* res, long ldr, void* y, long ldy,
+                             int y_type, void* z, long ldz, int M, int N, int K, float* ws, size_t ws_bytes, void* stream) {
+  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_fwd: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(type == DD_BF16 || type == DD_E4M3, "dd_linear_fwd: x and w are bf16 or e4m3 (fp32: dd_gemm_f32)");
+  DD_REQUIRE(y_type == DD_BF16 || y_type == DD_F32, "dd_linear_fwd: y is bf16 or fp32");
+  DD_REQUIRE(act >= DD_ACT_NONE && act <= DD_ACT_GELU, "dd_linear_fwd: unknown activation");
+  DD_REQUIRE((type == DD_E4M3) == (x_scale != nullptr) && (type == DD_E4M3) == (w_scale != nullptr),
+             "dd_linear_fwd: x_scale and w_scale go with e4m3 operands, and only with them");
+  if (M == 0) return 0;
+  DD_REQUIRE(x && w && y, "dd_linear_fwd: null x, w or y");
+  DD_REQUIRE(ldx >= K && ldw >= K && ldy >= N && (!res || ldr >= N) && (!z || ldz >= N), "dd_linear_fwd: a leading dimension is too small");
+  const int es = dtype_size(type);
+  const Mat P{x, ldx, M, mat_vec(x, ldx, es)}, Q{w, ldw, N, mat_vec(w, ldw, es)};
+  Epi e{y, ldy, y_type, bias, act, res, ldr, (__bf16*)z, ldz, x_scale, w_scale, 0, 0};
+  e.vec = out_vec(y, ldy, y_type) && out_vec(res, ldr, y_type) && out_vec(z, ldz, DD_BF16) && out_vec(bias, 0, DD_F32) &&
+          out_vec(w_scale, 0, DD_F32);
+  if (type == DD_BF16) return product<2, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
+  return product<1, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int dd_linear_bwd_data(const void* dz, long lddz, const void* w, long ldw, void* dx, long lddx, int x_type, int M,
+                                  int N, int K, float* ws, size_t ws_bytes, void* stream) {
+  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_bwd_data: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(x_type == DD_BF16 || x_type == DD_F32, "dd_linear_bwd_data: dx is bf16 or fp32");
+  if (M == 0) return 0;
+  DD_REQUIRE(dz && w && dx, "dd_linear_bwd_data: null pointer");
+  DD_REQUIRE(lddz >= N && ldw >= K && lddx >= K, "dd_linear_bwd_data: a leading dimension is too small");
+  const Mat P{dz, lddz, M, mat_vec(dz, lddz, 2)}, Q{w, ldw, K, mat_vec(w, ldw, 2)};
+  Epi e{dx, lddx, x_type};
+  e.vec = out_vec(dx, lddx, x_type);
+  return product<2, false, true>("dd_linear_bwd_data", P, Q, N, e, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int dd_linear_bwd_weight(const void* dz, long lddz, const void* x, long ldx, void* dw, long lddw, int w_type,
+                                    int accumulate, int M, int N, int K, float* ws, size_t ws_bytes, void* stream) {
+  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_bwd_weight: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(w_type == DD_BF16 || w_type == DD_F32, "dd_linear_bwd_weight: dw is bf16 or fp32");
+  if (M == 0 && accumulate) return 0;
+  DD_REQUIRE(dw && (M == 0 || (dz && x)), "dd_linear_bwd_weight: null pointer");
+  DD_REQUIRE(lddw >= K && (M == 0 || (lddz >= N && ldx >= K)), "dd_linear_bwd_weight: a leading dimension is too small");
+  const Mat P{dz, lddz, N, mat_vec(dz, lddz, 2)}, Q{x, ldx, K, mat_vec(x, ldx, 2)};
+  Epi e{dw, lddw, w_type};
+  e.accumulate = accumulate;
+  e.vec = out_vec(dw, lddw, w_type);
+  return product<2, true, true>("dd_linear_bwd_weight", P, Q, M, e, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long ldz, int act, void* dz, long lddz, void* dbias,
+                                 int bias_type, int accumulate, int M, int N, float* ws, size_t ws_bytes, void* stream) {
+  DD_REQUIRE(M >= 0 && N > 0, "dd_linear_act_bwd: M >= 0 and N > 0 are needed");
+  DD_REQUIRE(act >= DD_ACT_NONE && act <= DD_ACT_GELU, "dd_linear_act_bwd: unknown activation");
+  DD_REQUIRE(!dbias || bias_type == DD_F32 || bias_type == DD_BF16, "dd_linear_act_bwd: dbias is fp32 or bf16");
+  const bool act_on = act != DD_ACT_NONE;
+  if (!act_on && !dbias) return 0;
+  if (M == 0 && (!dbias || accumulate)) return 0;
+  DD_REQUIRE(M == 0 || (dy && ldy >= N), "dd_linear_act_bwd: dy is null or its leading dimension is below N");
+  DD_REQUIRE(M == 0 || !act_on || (z && dz && ldz >= N && lddz >= N), "dd_linear_act_bwd: an activation needs z and dz");
+  const hipStream_t st = (hipStream_t)stream;
+  const int al = 16;
+  const bool vec = N % 8 == 0 && rows_aligned(dy, ldy, DD_BF16, al) && rows_aligned(ws, 0, DD_F32, al) &&
+                   (!act_on || (rows_aligned(z, ldz, DD_BF16, al) && rows_aligned(dz, lddz, DD_BF16, al)));
+  const int cols = dd_ceil_div(dd_ceil_div(N, vec ? 8 : 1), 256);
+  const int parts = max(1, min(min(M, 512), dd_ceil_div(1024, cols)));
+  const int rows_per = dd_ceil_div(M, parts), n = rows_per ? dd_ceil_div(M, rows_per) : 0;
+  DD_REQUIRE(!dbias || ws_bytes / sizeof(float) >= (size_t)n * N, "dd_linear_act_bwd: the workspace is too small");
+  if (M > 0) {
+    const dim3 grid(cols, n);
+    if (vec) k_act_bwd<8><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz, act, dbias ? ws : nullptr, M, N, rows_per);
+    else k_act_bwd<1><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz, act, dbias ? ws : nullptr, M, N, rows_per);
+    DD_CHECK_LAUNCH("dd_linear_act_bwd");
+  }
+  if (dbias) {
+    k_bias_sum<<<dd_ceil_div(N, 64), 1024, 0, st>>>(ws, n, N, dbias, bias_type, accumulate);
+    DD_CHECK_LAUNCH("dd_linear_act_bwd(dbias)");
+  }
+  return 0;
+}

@@ -35,8 +35,10 @@ extern "C" {
  * 9: dd_imagine_rollout_oh_fwd added; dd_imagine_rollout_supported answers discrete = 1 shapes.
  * 10: dd_ln_act_fwd_head / dd_ln_act_bwd_head added.
  * 11 (round 6): dd_gemm_f32_x, dd_imag_set_rows, dd_conv2d_s2_wgrad_ln,
- * dd_conv2d_s2_down_ln, dd_conv2d_s2_down_lnbwd, dd_stamp added. */
-#define DD_ABI_VERSION 11
+ * dd_conv2d_s2_down_ln, dd_conv2d_s2_down_lnbwd, dd_stamp added.
+ * 12: the residual recurrent block added: dd_rms_norm_fwd / _bwd, dd_quant_rows, dd_linear_fwd,
+ * dd_linear_act_bwd / _bwd_data / _bwd_weight, dd_gated_scan_fwd / _bwd. */
+#define DD_ABI_VERSION 12
 int dd_version(void);
 const char* dd_last_error(void);
 
@@ -240,6 +242,79 @@ int dd_gru_cell_bwd(const float* dhn, long lddn, const float* z3, long ldz,
                     const float* h, long ldh, float* dz3, long lddz,
                     float* dh, long lddh, float* dy3, long lddy,
                     float* zx, long ldzx, int U, int rows, int D, void* stream);
+
+/* ---- residual recurrent block --------------------------------------------------- */
+
+/* Operators of a block whose recurrence is linear in its state (so that the T steps of a replayed
+ * sequence are one scan instead of T dependent contractions): a root-mean-square norm that adds the
+ * residual stream, a product with its epilogue, the gated scan.  The counterparts on the RSSM path
+ * are dd_ln_act_fwd (nets.py:585-602), dd_gemm_f32 (nets.py:573) and dd_gru_cell_fwd
+ * (nets.py:149-160).  Storage types are given per operand; arithmetic, sums and states are fp32.
+ * `void*` operands are row-major views [rows, cols] with a leading dimension in ELEMENTS. */
+#define DD_F32 0
+#define DD_BF16 1
+#define DD_E4M3 2   /* OCP float8 e4m3 (no infinities, largest value 448) */
+#define DD_ACT_NONE 0
+#define DD_ACT_ELU 1
+#define DD_ACT_SILU 2
+#define DD_ACT_GELU 3 /* z * (1 + erf(z / sqrt(2))) / 2 */
+
+/* s = round(x + res) in res_type;  y = s / sqrt(mean(s^2) + eps) * gamma, from s as it is stored.
+ * res may be NULL (s = x, stored only if s is given); s may be res or x itself (same view).  With
+ * y_type DD_E4M3 a row of y is divided by scale[row] = max|y| / 448 and rounded (nearest even); a row
+ * whose largest magnitude is below 1e-30 becomes zeros with scale 1.  rstd [rows] may be NULL.
+ * C <= 32768; x, res fp32 or bf16. */
+int dd_rms_norm_fwd(const void* x, long ldx, int x_type, const void* res, long ldr, int res_type,
+                    void* s, long lds, const float* gamma, void* y, long ldy, int y_type,
+                    float* rstd, float* scale, int rows, int C, float eps, void* stream);
+/* ds = dres + d y / d s applied to dy: the gradient of x AND of res (dres, ds in res_type; dres may be
+ * NULL, ds may be dres itself).  dgamma (NULL ok) = or += (accumulate) sum over rows; partial sums of
+ * up to 1024 workgroups in ws (rows * C or 1024 * C floats, whichever is less), added in a fixed order. */
+int dd_rms_norm_bwd(const void* dy, long ldy, int y_type, const void* s, long lds, int res_type,
+                    const float* rstd, const float* gamma, const void* dres, long ldr, void* ds, long ldd,
+                    float* dgamma, int accumulate, int rows, int C, float* ws, size_t ws_bytes, void* stream);
+/* The 8-bit output of dd_rms_norm_fwd for rows that come from elsewhere (weights [out, in] once,
+ * activations that no norm precedes): q = e4m3(x / scale[row]), scale[row] = max|x| / 448. */
+int dd_quant_rows(const void* x, long ldx, int x_type, void* q, long ldq, float* scale, int rows, int C,
+                  void* stream);
+
+/* y[m][n] = act(z[m][n]) + res[m][n],  z = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n].
+ * x [M,K] and w [N,K] both bf16, or both e4m3 with their scales; bias, scales fp32; y bf16 or fp32, res
+ * in y's type; z (bf16, NULL ok) is stored for the backward pass.  bias, res NULL ok; res may be y
+ * itself (same view).  ws: partial sums of a split contraction. */
+int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
+                  const float* w_scale, const float* bias, int act, const void* res, long ldr, void* y, long ldy,
+                  int y_type, void* z, long ldz, int M, int N, int K, float* ws, size_t ws_bytes, void* stream);
+/* Gradients of the bf16 product (the gradient of res is dy).  dd_linear_act_bwd: dz = dy act'(z) (bf16;
+ * dz may be dy or z itself; with DD_ACT_NONE z and dz are unused, dz IS dy) and dbias [N] (NULL ok);
+ * dd_linear_bwd_data: dx [M,K] = dz w; dd_linear_bwd_weight: dw [N,K] = or += (accumulate) dz^T x.
+ * Sums are split and added in a fixed order: equal calls give equal bits. */
+int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long ldz, int act, void* dz, long lddz,
+                      void* dbias, int bias_type, int accumulate, int M, int N, float* ws, size_t ws_bytes,
+                      void* stream);
+int dd_linear_bwd_data(const void* dz, long lddz, const void* w, long ldw, void* dx, long lddx, int x_type,
+                       int M, int N, int K, float* ws, size_t ws_bytes, void* stream);
+int dd_linear_bwd_weight(const void* dz, long lddz, const void* x, long ldx, void* dw, long lddw, int w_type,
+                         int accumulate, int M, int N, int K, float* ws, size_t ws_bytes, void* stream);
+
+/* h[t] = a[t] h[t-1] + gate[t] phi(c[t]) over T steps of B sequences (rows b * T + t, D channels):
+ * v = u + shift, a = sigmoid(-v), gate = sigmoid(v) - the blend of dd_gru_cell_fwd, whose gates do not
+ * see h here - or sigmoid(i) if i is given; phi = tanh (cand_tanh) or the identity.  first (fp32, one
+ * per row with stride fstride, NULL ok): non-zero restarts the sequence at that step from a zero state,
+ * whatever the state held.  h0, hT [B,D] fp32 contiguous: the state before the first and after the last
+ * step (NULL: zeros / not wanted; hT may be h0).  u, c, i, h all fp32 or all bf16.  T = 1 is the single
+ * step of serving.  ws (8-byte aligned): the time axis is split over workgroups where B * D alone does
+ * not fill the chip. */
+int dd_gated_scan_fwd(const void* u, long ldu, const void* c, long ldc, const void* i, long ldi, int type,
+                      const float* first, long fstride, const float* h0, void* h, long ldh, float* hT,
+                      int B, int T, int D, float shift, int cand_tanh, float* ws, size_t ws_bytes, void* stream);
+/* Gradients from dh (of every h) and dhT (of the state after the last step, NULL ok), with the stored h:
+ * du, dc, di (with i) in the operands' type, dh0 [B,D] (NULL ok; may be dhT). */
+int dd_gated_scan_bwd(const void* dh, long lddh, const void* u, long ldu, const void* c, long ldc, const void* i,
+                      long ldi, const void* h, long ldh, int type, const float* first, long fstride,
+                      const float* h0, const float* dhT, void* du, long lddu, void* dc, long lddc, void* di,
+                      long lddi, float* dh0, int B, int T, int D, float shift, int cand_tanh, float* ws,
+                      size_t ws_bytes, void* stream);
 
 /* ---- fused observe scan ------------------------------------------------------- */
 

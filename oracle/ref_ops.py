@@ -300,6 +300,125 @@ class RefOps:
     stats[:, 0] = mean[:, 0]
     stats[:, 1] = rstd[:, 0]
 
+  # ---- residual recurrent block (float64 whatever the storage types) ----------------
+
+  @staticmethod
+  def _e4m3(v):
+    """Nearest e4m3 value of |v| <= 448, ties to even, in float64: 3 bits behind the leading one,
+    steps of 2^-9 below 2^-6."""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    return (torch.round(v / step) * step).clamp(-448.0, 448.0)
+
+  def quant_rows(self, x, q, scale):
+    x = x.double()
+    most = x.abs().amax(1, keepdim=True)
+    some = most >= 1e-30
+    q.copy_(self._e4m3(torch.where(some, x * (448.0 / torch.where(some, most, torch.ones_like(most))), x)))
+    scale.copy_(torch.where(some, most / 448.0, torch.ones_like(most))[:, 0])
+
+  def rms_norm_fwd(self, x, gamma, y, rstd=None, res=None, s=None, scale=None, eps=1e-6):
+    total = x.double() if res is None else x.double() + res.double()
+    if s is not None:
+      s.copy_(total.float() if s.dtype != torch.float64 else total)
+      total = s.double()
+    inv = torch.rsqrt((total * total).mean(1, keepdim=True) + eps)
+    if rstd is not None:
+      rstd.copy_(inv[:, 0])
+    out = total * inv * gamma.double()
+    if scale is not None:
+      self.quant_rows(out, y, scale)
+    else:
+      y.copy_(out)
+
+  def rms_norm_bwd(self, dy, s, rstd, gamma, ds, dgamma=None, dres=None, accumulate=False):
+    inv = rstd.double()[:, None]
+    n, d = s.double() * inv, dy.double()
+    g = d * gamma.double()
+    out = inv * (g - n * (g * n).mean(1, keepdim=True))
+    if dgamma is not None:
+      t = (d * n).sum(0)
+      dgamma.copy_(dgamma.double() + t if accumulate else t)
+    ds.copy_(out if dres is None else out + dres.double())
+
+  @staticmethod
+  def _act(z, act):
+    """Activation and derivative."""
+    if act in (None, 'none'):
+      return z, torch.ones_like(z)
+    if act == 'elu':
+      return torch.where(z > 0, z, torch.expm1(z)), torch.where(z > 0, torch.ones_like(z), torch.exp(z))
+    if act == 'silu':
+      p = torch.sigmoid(z)
+      return z * p, p * (1 + z * (1 - p))
+    p = 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+    return z * p, p + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+
+  def linear_fwd(self, x, w, y, bias=None, act=None, res=None, z=None, x_scale=None, w_scale=None):
+    t = x.double() @ w.double().t()
+    if x_scale is not None:
+      t = t * x_scale.double()[:, None] * w_scale.double()
+    if bias is not None:
+      t = t + bias.double()
+    if z is not None:
+      z.copy_(t)
+    t = self._act(t, act)[0]
+    y.copy_(t if res is None else t + res.double())
+
+  def linear_bwd(self, dy, x, w, dx=None, dw=None, dbias=None, act=None, z=None, dz=None, accumulate=False):
+    g = dy.double()
+    if act not in (None, 'none'):
+      g = g * self._act(z.double(), act)[1]
+    for out, t in ((dbias, g.sum(0)), (dx, g @ w.double()), (dw, g.t() @ x.double())):
+      if out is not None:
+        out.copy_(out.double() + t if accumulate and out is not dx else t)
+    if act not in (None, 'none'):
+      dz.copy_(g)
+
+  @staticmethod
+  def _scan_gates(u, c, i, T, first, shift, cand):
+    B, D = u.shape[0] // T, u.shape[1]
+    v = u.double().reshape(B, T, D) + shift
+    restart = torch.zeros(B, T, 1, dtype=torch.bool) if first is None else (first != 0).reshape(B, T, 1)
+    gate = torch.sigmoid(v if i is None else i.double().reshape(B, T, D))
+    x = c.double().reshape(B, T, D)
+    return B, D, torch.sigmoid(-v), restart, gate, (torch.tanh(x) if cand else x)
+
+  def gated_scan_fwd(self, u, c, h, T, i=None, first=None, h0=None, hT=None, shift=-1.0, cand='tanh'):
+    B, D, a, restart, gate, phi = self._scan_gates(u, c, i, T, first, shift, cand)
+    x = torch.zeros(B, D, dtype=torch.float64) if h0 is None else h0.double()
+    out = []
+    for t in range(T):
+      x = gate[:, t] * phi[:, t] + torch.where(restart[:, t], torch.zeros_like(x), a[:, t] * x)
+      out.append(x)
+    h.copy_(torch.stack(out, 1).reshape(B * T, D))
+    if hT is not None:
+      hT.copy_(x)
+
+  def gated_step(self, u, c, h, h0, hT, i=None, first=None, shift=-1.0, cand='tanh'):
+    self.gated_scan_fwd(u, c, h, 1, i, first, h0, hT, shift, cand)
+
+  def gated_scan_bwd(self, dh, u, c, h, du, dc, T, i=None, di=None, first=None, h0=None, dhT=None, dh0=None,
+                     shift=-1.0, cand='tanh'):
+    B, D, a, restart, gate, phi = self._scan_gates(u, c, i, T, first, shift, cand)
+    zero = torch.zeros(B, D, dtype=torch.float64)
+    states = h.double().reshape(B, T, D)
+    g = zero if dhT is None else dhT.double()
+    rows = []
+    for t in reversed(range(T)):
+      g = g + dh.double().reshape(B, T, D)[:, t]
+      before = states[:, t - 1] if t else zero if h0 is None else h0.double()
+      before = torch.where(restart[:, t], zero, before)
+      slope = a[:, t] * (1 - a[:, t])
+      rows.append((g * ((phi[:, t] if i is None else 0.0) - before) * slope,
+                   g * gate[:, t] * (1 - phi[:, t] ** 2 if cand else 1.0),
+                   g * phi[:, t] * gate[:, t] * (1 - gate[:, t])))
+      g = torch.where(restart[:, t], zero, a[:, t] * g)
+    for out, k in ((du, 0), (dc, 1), (di, 2)):
+      if out is not None:
+        out.copy_(torch.stack([r[k] for r in rows[::-1]], 1).reshape(B * T, D))
+    if dh0 is not None:
+      dh0.copy_(g)
+
   def gru_bwd(self, dhn, z3, stats, gamma, beta, h, dz3, dh, dy3, zero=None):
     D = h.shape[1]
     mean, rstd = stats[:, :1], stats[:, 1:2]
