@@ -8,6 +8,7 @@
 // sums in fp32.  All three products are P Q^T with different storage orders: an operand is
 // contraction-contiguous (KC) or row-contiguous (RC).
 #include "block_core.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -203,6 +204,236 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
   }
 }
 
+// ---- tiled kernel --------------------------------------------------------------------------------
+//
+// BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
+// contraction per step.  A step's tiles come from global memory straight into LDS (16 bytes per lane,
+// no registers in between), two stages: while the instructions of one run, the next is in flight.
+// Reads past an operand's end give zeros (buffer descriptor) - no bounds checks in the loop.
+//
+// LDS holds 16-byte chunks; which chunk of its row a slot holds is permuted by the row, on the GLOBAL
+// address of the copy (the LDS side of a copy is fixed: base + lane * 16), so that the lanes of a read
+// fall on different banks:
+//   KC operand: tile [R][128 B], slot c of row r holds chunk c ^ ((r >> 1) & 7); a lane reads 16 bytes
+//     (8 bf16 or 16 e4m3 of its row)
+//   RC operand: tile [64 k][R], slot c of row k holds chunk c ^ ((k & 3) << 2); read by the transposing
+//     LDS load: 4 k of one row per lane, two loads for the 8 k an instruction wants
+#define DD_LDS __attribute__((address_space(3)))
+
+template <int ES, bool RC, int R_, int NW>
+struct TileCopy {
+  static constexpr int N = R_ / 8 / NW, BK = ROWB / ES;   // copies per wave and step
+  const char* base;      // tile's first byte of the next step
+  long step;             // bytes per step
+  unsigned size;         // bytes from base to the end of the tile's last row (KC) or of a whole step (RC)
+  unsigned ldb, cols;    // RC: bytes of a row, of the tile's part of it and what is behind
+  int voff[N];
+  int col;               // KC: contraction elements in front of the lane's chunk, for the parities of the row
+  __device__ __forceinline__ void init(const Mat& a, long r0, long k0, int K, int wave, int lane) {
+    base = (const char*)a.p + (RC ? k0 * a.ld + r0 : r0 * a.ld + k0) * ES;
+    step = RC ? BK * a.ld * ES : ROWB;
+    ldb = (unsigned)(a.ld * ES);
+    cols = (unsigned)((a.R - r0) * ES);
+    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = (i * NW + wave) * 64 + lane;
+      if constexpr (RC) {
+        const int k = id / (R_ / 8), c = (id % (R_ / 8)) ^ ((k & 3) << 2);
+        voff[i] = (int)(k * ldb) + c * 16;
+      } else {
+        const int r = id >> 3, c = (id & 7) ^ ((r >> 1) & 7);
+        voff[i] = (int)(r * ldb) + c * 16;
+      }
+    }
+    // NW is even: (r >> 1) & 7 = 4 (wave & 1) + (lane >> 4) for every copy
+    col = ((lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7)) * (16 / ES);
+  }
+  // The copies of the next step into LDS offset `lds`; rest: contraction elements left (none: zeros).
+  // Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that
+  // it cannot tell apart from the copy's target; the one wait that is needed is sync_copies.
+  __device__ __forceinline__ void issue(unsigned lds, int wave, int rest) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    unsigned bytes = rest > 0 ? size : 0u;
+    if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
+    const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, bytes, 0x00020000u};
+    if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks past the end are
+#pragma unroll                            // moved out of the descriptor's range
+      for (int i = 0; i < N; ++i) voff[i] = col >= rest ? 0x7fffffff : voff[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(lds + (i * NW + wave) * 1024), "v"(voff[i]), "s"(rs) : "memory");
+    base += step;
+    if (!RC) size -= ROWB;
+  }
+};
+// Every copy of this wave has landed, and then every wave's; reads issued before are complete.
+__device__ __forceinline__ void sync_copies() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt 0, lgkmcnt 0
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The instruction operand of rows r .. r + 31 and contraction step s (16 bf16: ES 2, 64 e4m3: ES 1).
+template <int ES, bool RC, int R_>
+struct Frag;
+template <int R_>
+struct Frag<2, false, R_> {
+  typedef bf16x8 T;
+  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
+    const int row = r + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((row >> 1) & 7);
+    return *reinterpret_cast<const bf16x8*>(sh + row * ROWB + c * 16);
+  }
+};
+template <int R_>
+struct Frag<2, true, R_> {
+  typedef bf16x8 T;
+  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const int k = s * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);   // & 3 is the lane's alone
+    const int row = r + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const int at = k * (R_ * 2) + (((row >> 3) ^ ((k & 3) << 2)) << 4) + (row & 4) * 2;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DD_LDS s16x4*)(sh + at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DD_LDS s16x4*)(sh + at + 4 * R_ * 2));
+    const s16x8 t = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return __builtin_bit_cast(bf16x8, t);
+  }
+};
+template <int R_>
+struct Frag<1, false, R_> {
+  typedef i32x8 T;
+  // (which 32 of the 64 elements a lane holds, and in which order, is free: both operands agree)
+  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
+    const int row = r + (lane & 31), x = (row >> 1) & 7, c = 4 * s + 2 * (lane >> 5);
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 a = *reinterpret_cast<const i32x4*>(sh + row * ROWB + ((c ^ x) << 4));
+    const i32x4 b = *reinterpret_cast<const i32x4*>(sh + row * ROWB + (((c + 1) ^ x) << 4));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+__device__ __forceinline__ f32x16 mma(bf16x8 q, bf16x8 p, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, p, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(i32x8 q, i32x8 p, f32x16 c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(q, p, c, 0, 0, 0, 127, 0, 127);
+}
+
+template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
+  constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, STAGE = (BM + BN) * ROWB;
+  constexpr int STEPS = ES == 2 ? 4 : 2, BK = ROWB / ES;
+  __shared__ __attribute__((aligned(1024))) char sh[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles, four
+  // columns wide, so that its L2 serves the rows and weights that its 32 running tiles share
+  // (4 x 8 tiles read 12 operand tiles per step, 2 x 16 would read 18).
+  const int total = gridDim.x, q8 = total / 8, r8 = total % 8, xcd = blockIdx.x % 8;
+  int id = xcd * q8 + min(xcd, r8) + blockIdx.x / 8;
+  const int split = id / (tm * tn);
+  id -= split * (tm * tn);
+  const int band = id / (4 * tm), width = min(4, tn - 4 * band);
+  id -= band * 4 * tm;
+  const int nt = 4 * band + id % width, mt = id / width;
+  const long m0 = (long)mt * BM, n0 = (long)nt * BN, kb = (long)split * kspan;
+  const int kend = (int)min((long)K, kb + kspan), steps = (kend - (int)kb + BK - 1) / BK;
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+
+  TileCopy<ES, P_RC, BM, NW> cp;
+  TileCopy<ES, Q_RC, BN, NW> cq;
+  cp.init(P, m0, kb, K, wave, lane);
+  cq.init(Q, n0, kb, K, wave, lane);
+  const unsigned lds = (unsigned)(uintptr_t)(DD_LDS char*)sh;
+  f32x16 acc[MT][NT] = {};
+  int rest = kend - (int)kb;   // of the step that is copied next
+  // A group: one contraction step of the instruction, all of the wave's rows (e4m3: half of them, its
+  // operands are twice as large).  Two register sets.
+  constexpr int H = ES == 2 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
+  typename Frag<ES, P_RC, BM>::T p[2][MH];
+  typename Frag<ES, Q_RC, BN>::T q[2][NT];
+  auto read = [&](int stage, int g) {
+    const char* a = sh + stage;
+    if (g % H == 0)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) q[(g / H) & 1][j] = Frag<ES, Q_RC, BN>::read(a + BM * ROWB, wn + 32 * j, g / H, lane);
+#pragma unroll
+    for (int i = 0; i < MH; ++i) p[g & 1][i] = Frag<ES, P_RC, BM>::read(a, wm + 32 * (i + (g % H) * MH), g / H, lane);
+  };
+  // Step t + 2's copies are issued as soon as step t's stage is free, behind the instructions of two
+  // groups (in one go they would hold the waves up while the address unit works through them), and are
+  // waited for at the end of step t + 1.  Operands of a group are read one group ahead, across the barrier
+  // too, so that the matrix unit has work while the waves meet.
+  cp.issue(lds, wave, rest);
+  cq.issue(lds + BM * ROWB, wave, rest);
+  rest -= BK;
+  sync_copies();
+  cp.issue(lds + STAGE, wave, rest);
+  read(0, 0);
+  for (int t = 0; t < steps; ++t) {
+    const int here = (t & 1) * STAGE, next = STAGE - here;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      if (g + 1 < GROUPS) {
+        read(here, g + 1);
+      } else {
+        sync_copies();
+        read(next, 0);   // (after the last step: the other stage's old contents, not used)
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < MH; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          acc[i + (g % H) * MH][j] = mma(q[(g / H) & 1][j], p[g & 1][i], acc[i + (g % H) * MH][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (g == GROUPS - 1) cp.issue(lds + here, wave, rest);
+      if (g == 0) {
+        cq.issue(lds + next + BM * ROWB, wave, rest);
+        rest -= BK;
+      }
+    }
+  }
+  sync_copies();
+
+  // 32 rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds
+  // four consecutive columns of one row), then eight lanes finish a row's 64 columns, 8 each
+  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR;
+  static_assert(NW * 32 * LD * 4 <= 2 * STAGE, "the epilogue's LDS");
+  float* out = reinterpret_cast<float*>(sh) + wave * 32 * LD;
+  float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(out + (lane & 31) * LD + 32 * j + 8 * g + 4 * (lane >> 5)) = v;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPI) {
+      const long m = m0 + wm + 32 * i + r, n = n0 + wn + (lane % LPR) * 8;
+      float v[8];
+      load_f32<8>(out + r * LD + (lane % LPR) * 8, v);
+      if (m < P.R) {
+        if (slab) {
+          if (Q.R % 8 == 0) { if (n < Q.R) store_f32<8>(slab + m * Q.R + n, v); }
+          else
+            for (int k = 0; k < 8; ++k)
+              if (n + k < Q.R) slab[m * Q.R + n + k] = v[k];
+        } else if (e.vec && n + 8 <= Q.R) {
+          finish<8>(e, m, n, v);
+        } else {
+          for (int k = 0; k < 8; ++k)
+            if (n + k < Q.R) { float u[1] = {v[k]}; finish<1>(e, m, n + k, u); }
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // Sum of the partial results of a split contraction, slabs ascending, and the epilogue.
 __global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, Epi e) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -234,8 +465,41 @@ inline int pick_splits(long tiles, int ktiles, size_t slab_bytes, size_t ws_byte
   return (int)max(s, 1l);
 }
 
+// Can the tiled kernel's copies read this operand?  16-byte chunks: aligned rows of whole chunks along
+// the contiguous axis; offsets within a tile below 2^31.
+inline bool tileable(const Mat& a, bool rc, int K, int es) {
+  return a.vec && (rc ? a.R : K) % (16 / es) == 0 && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
+}
+
+template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
+int tiled(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+  const int bk = ROWB / ES, tm = dd_ceil_div(P.R, BM), tn = dd_ceil_div(Q.R, BN), ktiles = dd_ceil_div(K, bk);
+  const long tiles = (long)tm * tn;
+  int S = 1;
+  if (tiles < 192 && ktiles >= 16) {
+    S = (int)max(1l, min(256 / tiles, (long)ktiles / 8));
+    while (S > 1 && sizeof(float) * (size_t)P.R * Q.R * S > (ws ? ws_bytes : 0)) --S;
+  }
+  const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
+  DD_REQUIRE(tiles * parts < (1l << 31), "dd_linear: too many tiles");
+  k_linear_tile<ES, P_RC, Q_RC, BM, BN, WM, WN><<<(unsigned)(tiles * parts), 64 * WM * WN, 0, st>>>(
+      P, Q, K, kspan, tm, tn, parts > 1 ? ws : nullptr, e);
+  DD_CHECK_LAUNCH(who);
+  if (parts > 1) {
+    const long work = (long)P.R * Q.R / (e.vec && Q.R % 8 == 0 ? 8 : 1);
+    k_linear_finish<<<dd_ceil_div(work, 256), 256, 0, st>>>(ws, parts, P.R, Q.R, e);
+    DD_CHECK_LAUNCH(who);
+  }
+  return 0;
+}
+
 template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+  static const int force = getenv("DD_LIN_TILE") ? atoi(getenv("DD_LIN_TILE")) : -1;
+  if (K > 0 && tileable(P, P_RC, K, ES) && tileable(Q, Q_RC, K, ES) && force != 0) {
+    if (force == 1 || (force < 0 && (long)P.R * Q.R >= 256l * 256 * 128)) return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, P, Q, K, e, ws, ws_bytes, st);
+    if (force == 2 || force < 0) return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, P, Q, K, e, ws, ws_bytes, st);
+  }
   const int bk = ROWB / ES;
   const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));
   DD_REQUIRE(tiles.y <= 65535, "dd_linear: more than 4194240 output columns");
