@@ -124,20 +124,36 @@ __device__ __forceinline__ float tanh_f(float x) {
   return a < 0.3f ? s : l;
 }
 
+// e^x - 1 for x <= 0: Taylor polynomial where the difference would cancel (next term 5e-9 relative).
+__device__ __forceinline__ float expm1_neg(float x) {
+  const float s = x * (1.f + x * (1.f / 2 + x * (1.f / 6 + x * (1.f / 24 + x * (1.f / 120 + x * (1.f / 720 + x * (1.f / 5040)))))));
+  return x > -0.3f ? s : fast_exp(x) - 1.0f;
+}
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), with Abramowitz and Stegun's 7.1.26 for erf
+// (absolute error 1.5e-7, so 0.75e-7 here) on the same exponential.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float t = fast_rcp(1.0f + 0.3275911f * 0.70710678118654752f * fabsf(z));
+  e = fast_exp(-0.5f * z * z);
+  const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z >= 0.f ? 1.0f - q : q;
+}
+
 // y = act(z); codes of include/daydreamer_hip.h
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) {
-  if constexpr (ACT == DD_ACT_ELU) return z > 0.f ? z : expm1f(z);
-  if constexpr (ACT == DD_ACT_SILU) { float p, q; sigmoid2(z, p, q); return z * p; }
-  if constexpr (ACT == DD_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  float p, q;
+  if constexpr (ACT == DD_ACT_ELU) return z > 0.f ? z : expm1_neg(z);
+  if constexpr (ACT == DD_ACT_SILU) { sigmoid2(z, p, q); return z * p; }
+  if constexpr (ACT == DD_ACT_GELU) return z * normal_cdf(z, q);
   return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
+  float p, q;
   if constexpr (ACT == DD_ACT_ELU) return z > 0.f ? 1.0f : fast_exp(z);
-  if constexpr (ACT == DD_ACT_SILU) { float p, q; sigmoid2(z, p, q); return p * (1.0f + z * q); }
-  if constexpr (ACT == DD_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * fast_exp(-0.5f * z * z) * 0.39894228040143268f;
+  if constexpr (ACT == DD_ACT_SILU) { sigmoid2(z, p, q); return p * (1.0f + z * q); }
+  if constexpr (ACT == DD_ACT_GELU) { p = normal_cdf(z, q); return p + z * q * 0.39894228040143268f; }
   return 1.0f;
 }
 

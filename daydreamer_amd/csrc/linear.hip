@@ -23,7 +23,7 @@ struct Epi {
   __bf16* z; long ldz;
   const float* xs; const float* wsc;
   int accumulate;
-  int vec;         // 16-byte accesses are aligned for every operand above
+  int vec;         // 8, 2 or 1 consecutive columns are aligned for every operand above
 };
 
 __device__ __forceinline__ float act_any(int act, float z) {
@@ -35,7 +35,7 @@ __device__ __forceinline__ float act_any(int act, float z) {
   }
 }
 
-// V consecutive outputs of row m from column n; V == 8 needs e.vec and n + 8 <= N.
+// V <= e.vec consecutive outputs of row m from column n.
 template <int V>
 __device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V]) {
   if (e.xs) {
@@ -82,6 +82,17 @@ __device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V])
     }
     store_bf16<V>(p, v);
   }
+}
+
+// Eight columns (fewer at the end of a row) of which not all are there or aligned; v in LDS.
+__device__ __forceinline__ void finish_ragged(const Epi& e, long m, long n, long N, const float* v) {
+  if (e.vec >= 2 && n + 8 <= N) {
+#pragma unroll 1
+    for (int j = 0; j < 8; j += 2) { float t[2] = {v[j], v[j + 1]}; finish<2>(e, m, n + j, t); }
+    return;
+  }
+#pragma unroll 1
+  for (int j = 0; j < 8 && n + j < N; ++j) { float t[1] = {v[j]}; finish<1>(e, m, n + j, t); }
 }
 
 // An operand: R rows (of the output's rows or columns), contraction length K.
@@ -195,11 +206,10 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
       float* p = slabs + ((long)blockIdx.z * P.R + m) * Q.R + n;
       for (int j = 0; j < 8; ++j)
         if (n + j < Q.R) p[j] = v[j];
-    } else if (e.vec && n + 8 <= Q.R) {
+    } else if (e.vec == 8 && n + 8 <= Q.R) {
       finish<8>(e, m, n, v);
     } else {
-      for (int j = 0; j < 8; ++j)
-        if (n + j < Q.R) { float t[1] = {v[j]}; finish<1>(e, m, n + j, t); }
+      finish_ragged(e, m, n, Q.R, out + mr * 68 + nc);
     }
   }
 }
@@ -252,20 +262,26 @@ struct TileCopy {
   // The copies of the next step into LDS offset `lds`; rest: contraction elements left (none: zeros).
   // Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that
   // it cannot tell apart from the copy's target; the one wait that is needed is sync_copies.
-  __device__ __forceinline__ void issue(unsigned lds, int wave, int rest) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  __device__ __forceinline__ u32x4 begin(int rest) {
     unsigned bytes = rest > 0 ? size : 0u;
     if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
     const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, bytes, 0x00020000u};
     if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks past the end are
 #pragma unroll                            // moved out of the descriptor's range
       for (int i = 0; i < N; ++i) voff[i] = col >= rest ? 0x7fffffff : voff[i];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(lds + (i * NW + wave) * 1024), "v"(voff[i]), "s"(rs) : "memory");
     base += step;
     if (!RC) size -= ROWB;
+    return rs;
+  }
+  __device__ __forceinline__ void one(const u32x4& rs, unsigned lds, int wave, int i) const {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(lds + (i * NW + wave) * 1024), "v"(voff[i]), "s"(rs) : "memory");
+  }
+  __device__ __forceinline__ void issue(unsigned lds, int wave, int rest) {
+    const u32x4 rs = begin(rest);
+#pragma unroll
+    for (int i = 0; i < N; ++i) one(rs, lds, wave, i);
   }
 };
 // Every copy of this wave has landed, and then every wave's; reads issued before are complete.
@@ -351,13 +367,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   constexpr int H = ES == 2 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
   typename Frag<ES, P_RC, BM>::T p[2][MH];
   typename Frag<ES, Q_RC, BN>::T q[2][NT];
-  auto read = [&](int stage, int g) {
+  // one of a group's NT + MH operands
+  auto read1 = [&](int stage, int g, int k) {
     const char* a = sh + stage;
-    if (g % H == 0)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) q[(g / H) & 1][j] = Frag<ES, Q_RC, BN>::read(a + BM * ROWB, wn + 32 * j, g / H, lane);
-#pragma unroll
-    for (int i = 0; i < MH; ++i) p[g & 1][i] = Frag<ES, P_RC, BM>::read(a, wm + 32 * (i + (g % H) * MH), g / H, lane);
+    if (k < NT) {
+      if (g % H == 0) q[(g / H) & 1][k] = Frag<ES, Q_RC, BN>::read(a + BM * ROWB, wn + 32 * k, g / H, lane);
+    } else {
+      p[g & 1][k - NT] = Frag<ES, P_RC, BM>::read(a, wm + 32 * (k - NT + (g % H) * MH), g / H, lane);
+    }
   };
   // Step t + 2's copies are issued as soon as step t's stage is free, behind the instructions of two
   // groups (in one go they would hold the waves up while the address unit works through them), and are
@@ -368,93 +385,188 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   rest -= BK;
   sync_copies();
   cp.issue(lds + STAGE, wave, rest);
-  read(0, 0);
+#pragma unroll
+  for (int k = 0; k < NT + MH; ++k) read1(0, 0, k);
   for (int t = 0; t < steps; ++t) {
     const int here = (t & 1) * STAGE, next = STAGE - here;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      if (g + 1 < GROUPS) {
-        read(here, g + 1);
-      } else {
-        sync_copies();
-        read(next, 0);   // (after the last step: the other stage's old contents, not used)
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      if (g + 1 == GROUPS) sync_copies();
+      typename decltype(cp)::u32x4 rs;
+      if (g == GROUPS - 1) rs = cp.begin(rest);
+      if (g == 0) { rs = cq.begin(rest); rest -= BK; }
 #pragma unroll
-      for (int i = 0; i < MH; ++i)
+      for (int i = 0; i < MH; ++i) {
+#pragma unroll
+        for (int k = i * (NT + MH) / MH; k < (i + 1) * (NT + MH) / MH; ++k)
+          read1(g + 1 < GROUPS ? here : next, g + 1 < GROUPS ? g + 1 : 0, k);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
           acc[i + (g % H) * MH][j] = mma(q[(g / H) & 1][j], p[g & 1][i], acc[i + (g % H) * MH][j]);
-      __builtin_amdgcn_sched_barrier(0);
-      if (g == GROUPS - 1) cp.issue(lds + here, wave, rest);
-      if (g == 0) {
-        cq.issue(lds + next + BM * ROWB, wave, rest);
-        rest -= BK;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < cp.N; ++k)
+          if (g == GROUPS - 1 && k >= i * cp.N / MH && k < (i + 1) * cp.N / MH) cp.one(rs, lds + here, wave, k);
+#pragma unroll
+        for (int k = 0; k < cq.N; ++k)
+          if (g == 0 && k >= i * cq.N / MH && k < (i + 1) * cq.N / MH) cq.one(rs, lds + next + BM * ROWB, wave, k);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
   sync_copies();
 
   // 32 rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds
-  // four consecutive columns of one row), then eight lanes finish a row's 64 columns, 8 each
-  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR;
+  // four consecutive columns of one row); LPR lanes finish a row, 8 columns each, in two halves of RI rows
+  // per lane.  What they need from memory is requested before
+  // the exchange through LDS.  The loop stays rolled - the next
+  // accumulators move down - because copies of three activations would not fit the instruction cache.
+  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI;
+  static_assert(RI * RPI == 16, "a half is whole rows of every lane");
   static_assert(NW * 32 * LD * 4 <= 2 * STAGE, "the epilogue's LDS");
   float* out = reinterpret_cast<float*>(sh) + wave * 32 * LD;
   float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
+  const int nc = (lane % LPR) * 8;
+  const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
+  const bool full = e.vec == 8 && n + 8 <= Q.R;
+  uint4 res[RI][2];
+  float xs[RI];
+  auto fetch = [&](int i) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        *reinterpret_cast<f32x4*>(out + (lane & 31) * LD + 32 * j + 8 * g + 4 * (lane >> 5)) = v;
-      }
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += RPI) {
-      const long m = m0 + wm + 32 * i + r, n = n0 + wn + (lane % LPR) * 8;
-      float v[8];
-      load_f32<8>(out + r * LD + (lane % LPR) * 8, v);
-      if (m < P.R) {
-        if (slab) {
-          if (Q.R % 8 == 0) { if (n < Q.R) store_f32<8>(slab + m * Q.R + n, v); }
-          else
-            for (int k = 0; k < 8; ++k)
-              if (n + k < Q.R) slab[m * Q.R + n + k] = v[k];
-        } else if (e.vec && n + 8 <= Q.R) {
-          finish<8>(e, m, n, v);
+    for (int k = 0; k < RI; ++k) {
+      const long m = mrow + 16 * i + RPI * k;
+      if (!full || slab || m >= P.R) continue;
+      if (e.xs) xs[k] = e.xs[m];
+      if (e.res) {
+        if (e.ytype == DD_F32) {
+          res[k][0] = reinterpret_cast<const uint4*>((const float*)e.res + m * e.ldr + n)[0];
+          res[k][1] = reinterpret_cast<const uint4*>((const float*)e.res + m * e.ldr + n)[1];
         } else {
-          for (int k = 0; k < 8; ++k)
-            if (n + k < Q.R) { float u[1] = {v[k]}; finish<1>(e, m, n + k, u); }
+          res[k][0] = *reinterpret_cast<const uint4*>((const __bf16*)e.res + m * e.ldr + n);
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+  };
+  fetch(0);
+#pragma unroll 1
+  for (int i = 0; i < 2 * MT; ++i) {
+    if (i % 2 == 0) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 v = {acc[0][j][4 * g], acc[0][j][4 * g + 1], acc[0][j][4 * g + 2], acc[0][j][4 * g + 3]};
+          *reinterpret_cast<f32x4*>(out + (lane & 31) * LD + 32 * j + 8 * g + 4 * (lane >> 5)) = v;
+        }
+#pragma unroll
+        for (int k = 0; k + 1 < MT; ++k) acc[k][j] = acc[k + 1][j];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    const float* rows = out + (lane / LPR + 16 * (i & 1)) * LD + nc;
+    if (slab) {
+#pragma unroll
+      for (int k = 0; k < RI; ++k) {
+        const long m = mrow + 16 * i + RPI * k;
+        const float* from = rows + RPI * k * LD;
+        if (m >= P.R) continue;
+        if (Q.R % 8 == 0) {
+          float v[8];
+          load_f32<8>(from, v);
+          if (n < Q.R) store_f32<8>(slab + m * Q.R + n, v);
+        } else {
+          for (int j = 0; j < 8 && n + j < Q.R; ++j) slab[m * Q.R + n + j] = from[j];
+        }
+      }
+    } else if (full) {
+      float v[RI][8], col[8];
+#pragma unroll
+      for (int k = 0; k < RI; ++k) load_f32<8>(rows + RPI * k * LD, v[k]);
+      if (e.xs) {
+        load_f32<8>(e.wsc + n, col);
+#pragma unroll
+        for (int k = 0; k < RI; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] *= xs[k] * col[j];
+      }
+      if (e.bias) {
+        load_f32<8>(e.bias + n, col);
+#pragma unroll
+        for (int k = 0; k < RI; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] += col[j];
+      }
+      if (e.z)
+#pragma unroll
+        for (int k = 0; k < RI; ++k)
+          if (mrow + 16 * i + RPI * k < P.R) store_bf16<8>(e.z + (mrow + 16 * i + RPI * k) * e.ldz + n, v[k]);
+#define DD_ACT_CASE(A_)                          \
+  case A_:                                       \
+    _Pragma("unroll") for (int k = 0; k < RI; ++k) { \
+      _Pragma("unroll") for (int j = 0; j < 8; ++j) v[k][j] = act_f<A_>(v[k][j]); \
+      __builtin_amdgcn_sched_barrier(0);         \
+    }                                            \
+    break;
+      switch (e.act) { DD_ACT_CASE(DD_ACT_ELU) DD_ACT_CASE(DD_ACT_SILU) DD_ACT_CASE(DD_ACT_GELU) }
+#undef DD_ACT_CASE
+#pragma unroll
+      for (int k = 0; k < RI; ++k) {
+        const long m = mrow + 16 * i + RPI * k;
+        if (m >= P.R) continue;
+        if (e.res) {
+          if (e.ytype == DD_F32) {
+            const f32x4 a = __builtin_bit_cast(f32x4, res[k][0]), b = __builtin_bit_cast(f32x4, res[k][1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[k][j] += a[j]; v[k][4 + j] += b[j]; }
+          } else {
+            const bf16x8 a = __builtin_bit_cast(bf16x8, res[k][0]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] += (float)a[j];
+          }
+        }
+        if (e.accumulate) {
+          float o[8];
+          if (e.ytype == DD_F32) load_f32<8>((const float*)e.y + m * e.ldy + n, o);
+          else load_bf16<8>((const __bf16*)e.y + m * e.ldy + n, o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] += o[j];
+        }
+        if (e.ytype == DD_F32) store_f32<8>((float*)e.y + m * e.ldy + n, v[k]);
+        else store_bf16<8>((__bf16*)e.y + m * e.ldy + n, v[k]);
+      }
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < RI; ++k)
+        if (mrow + 16 * i + RPI * k < P.R)
+          finish_ragged(e, mrow + 16 * i + RPI * k, n, Q.R, rows + RPI * k * LD);
+    }
+    if (i + 1 < 2 * MT) fetch(i + 1);
   }
 }
 
-// Sum of the partial results of a split contraction, slabs ascending, and the epilogue.
+// Sum of the partial results of a split contraction, slabs ascending, and the epilogue; N % V == 0.
+template <int V>
 __global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, Epi e) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long MN = M * N;
-  if (e.vec && N % 8 == 0) {
-    if (i * 8 >= MN) return;
-    float v[8], t[8];
-    load_f32<8>(slabs + i * 8, v);
-    for (int s = 1; s < S; ++s) {
-      load_f32<8>(slabs + s * MN + i * 8, t);
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * V, MN = M * N;
+  if (i >= MN) return;
+  float v[V], t[V];
+  load_f32<V>(slabs + i, v);
+#pragma unroll 4
+  for (int s = 1; s < S; ++s) {
+    load_f32<V>(slabs + s * MN + i, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += t[j];
-    }
-    finish<8>(e, i * 8 / N, i * 8 % N, v);
-  } else {
-    for (long q = i; q < MN; q += (long)gridDim.x * 256) {
-      float v[1] = {slabs[q]};
-      for (int s = 1; s < S; ++s) v[0] += slabs[s * MN + q];
-      finish<1>(e, q / N, q % N, v);
-    }
+    for (int j = 0; j < V; ++j) v[j] += t[j];
   }
+  finish<V>(e, i / N, i % N, v);
+}
+inline void sum_slabs(const float* slabs, int S, long M, long N, const Epi& e, hipStream_t st) {
+  const int v = e.vec == 8 && N % 8 == 0 ? 8 : e.vec >= 2 && N % 2 == 0 ? 2 : 1;
+  const unsigned grid = (unsigned)((M * N / v + 255) / 256);
+  if (v == 8) k_linear_finish<8><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
+  else if (v == 2) k_linear_finish<2><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
+  else k_linear_finish<1><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
 }
 
 // Splits of a contraction: none where the tiles alone fill the chip.
@@ -486,8 +598,7 @@ int tiled(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t 
       P, Q, K, kspan, tm, tn, parts > 1 ? ws : nullptr, e);
   DD_CHECK_LAUNCH(who);
   if (parts > 1) {
-    const long work = (long)P.R * Q.R / (e.vec && Q.R % 8 == 0 ? 8 : 1);
-    k_linear_finish<<<dd_ceil_div(work, 256), 256, 0, st>>>(ws, parts, P.R, Q.R, e);
+    sum_slabs(ws, parts, P.R, Q.R, e, st);
     DD_CHECK_LAUNCH(who);
   }
   return 0;
@@ -509,8 +620,7 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   k_linear_any<ES, P_RC, Q_RC><<<dim3(tiles.x, tiles.y, parts), 256, 0, st>>>(P, Q, K, kspan, parts > 1 ? ws : nullptr, e);
   DD_CHECK_LAUNCH(who);
   if (parts > 1) {
-    const long work = (long)P.R * Q.R / (e.vec && Q.R % 8 == 0 ? 8 : 1);
-    k_linear_finish<<<dd_ceil_div(work, 256), 256, 0, st>>>(ws, parts, P.R, Q.R, e);
+    sum_slabs(ws, parts, P.R, Q.R, e, st);
     DD_CHECK_LAUNCH(who);
   }
   return 0;
@@ -563,7 +673,15 @@ __global__ void __launch_bounds__(1024) k_bias_sum(const float* parts, int n, in
 }
 
 inline int mat_vec(const void* p, long ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
-inline bool out_vec(const void* p, long ld, int type) { return p == nullptr || rows_aligned(p, ld, type, 16); }
+// How many columns at a time (8, 2, 1) may be accessed in every one of the epilogue's operands?
+inline int columns_at_once(const Epi& e) {
+  for (int v = 8; v > 1; v = v == 8 ? 2 : 1) {
+    auto ok = [&](const void* p, long ld, int type) { return rows_aligned(p, ld, type, min(16, v * dtype_size(type))); };
+    if (ok(e.y, e.ldy, e.ytype) && ok(e.res, e.ldr, e.ytype) && ok(e.z, e.ldz, DD_BF16) && ok(e.bias, 0, DD_F32) &&
+        ok(e.wsc, 0, DD_F32)) return v;
+  }
+  return 1;
+}
 
 }  // namespace
 
@@ -582,8 +700,7 @@ extern "C" int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, i
   const int es = dtype_size(type);
   const Mat P{x, ldx, M, mat_vec(x, ldx, es)}, Q{w, ldw, N, mat_vec(w, ldw, es)};
   Epi e{y, ldy, y_type, bias, act, res, ldr, (__bf16*)z, ldz, x_scale, w_scale, 0, 0};
-  e.vec = out_vec(y, ldy, y_type) && out_vec(res, ldr, y_type) && out_vec(z, ldz, DD_BF16) && out_vec(bias, 0, DD_F32) &&
-          out_vec(w_scale, 0, DD_F32);
+  e.vec = columns_at_once(e);
   if (type == DD_BF16) return product<2, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
   return product<1, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
 }
@@ -597,7 +714,7 @@ extern "C" int dd_linear_bwd_data(const void* dz, long lddz, const void* w, long
   DD_REQUIRE(lddz >= N && ldw >= K && lddx >= K, "dd_linear_bwd_data: a leading dimension is too small");
   const Mat P{dz, lddz, M, mat_vec(dz, lddz, 2)}, Q{w, ldw, K, mat_vec(w, ldw, 2)};
   Epi e{dx, lddx, x_type};
-  e.vec = out_vec(dx, lddx, x_type);
+  e.vec = columns_at_once(e);
   return product<2, false, true>("dd_linear_bwd_data", P, Q, N, e, ws, ws_bytes, (hipStream_t)stream);
 }
 
@@ -611,7 +728,7 @@ extern "C" int dd_linear_bwd_weight(const void* dz, long lddz, const void* x, lo
   const Mat P{dz, lddz, N, mat_vec(dz, lddz, 2)}, Q{x, ldx, K, mat_vec(x, ldx, 2)};
   Epi e{dw, lddw, w_type};
   e.accumulate = accumulate;
-  e.vec = out_vec(dw, lddw, w_type);
+  e.vec = columns_at_once(e);
   return product<2, true, true>("dd_linear_bwd_weight", P, Q, M, e, ws, ws_bytes, (hipStream_t)stream);
 }
 
