@@ -8,7 +8,7 @@
 // sums in fp32.  All three products are P Q^T with different storage orders: an operand is
 // contraction-contiguous (KC) or row-contiguous (RC).
 #include "block_core.h"
-#include <stdlib.h>
+#include <type_traits>
 
 namespace {
 
@@ -214,6 +214,76 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
   }
 }
 
+// ---- few rows: single steps of serving -----------------------------------------------------------
+//
+// At most 64 rows, so the weights are read once and that read is the time.  A workgroup owns 16 weight
+// rows, its waves take turns along the contraction (32 bf16 / 128 e4m3 each, operands straight from
+// memory into the 16 x 16 instruction's registers, UNROLL steps requested before the first is used) and
+// add up in LDS.  One launch, no partial sums in memory.
+template <int ES, int MB>
+__global__ void __launch_bounds__(1024) k_linear_few(Mat P, Mat Q, int K, Epi e) {
+  constexpr int BK = ES == 2 ? 32 : 128, UNROLL = MB <= 2 ? 4 : 2, LANE = BK / 4;   // elements of a lane's operand
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  __shared__ float sh[16][MB * 16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int row = lane & 15, kl = (lane >> 4) * LANE;
+  const long n0 = (long)blockIdx.x * 16;
+  f32x4 acc[MB] = {};
+  const i32x4 zero = {};
+  constexpr int PER = 16 / ES;           // elements of a 16-byte load; K is a multiple of it
+  auto load = [&](const Mat& a, long r, int k, i32x4 v[LANE / PER]) {
+    const char* p = (const char*)a.p + (min(r, (long)a.R - 1) * a.ld + k) * ES;
+#pragma unroll
+    for (int j = 0; j < LANE / PER; ++j)
+      v[j] = r < a.R && k + j * PER < K ? *reinterpret_cast<const i32x4*>(p + 16 * j) : zero;
+  };
+  for (int k0 = wave * BK; k0 < K; k0 += waves * BK * UNROLL) {
+    i32x4 q[UNROLL][LANE / PER], x[UNROLL][MB][LANE / PER];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      load(Q, n0 + row, k0 + u * waves * BK + kl, q[u]);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) load(P, b * 16 + row, k0 + u * waves * BK + kl, x[u][b]);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        if constexpr (ES == 2) {
+          acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[u][0]), __builtin_bit_cast(bf16x8, x[u][b][0]), acc[b], 0, 0, 0);
+        } else {
+          const i32x8 w8 = __builtin_shufflevector(q[u][0], q[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const i32x8 x8 = __builtin_shufflevector(x[u][b][0], x[u][b][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[b], 0, 0, 0, 127, 0, 127);
+        }
+      }
+  }
+  // a lane holds columns 4 (lane >> 4) .. + 3 of row lane & 15
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sh[wave][b * 16 + row][4 * (lane >> 4) + j] = acc[b][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MB * 16 * 16; i += blockDim.x) {
+    const int m = i >> 4, c = i & 15;
+    if (m < P.R && n0 + c < Q.R) {
+      float v[1] = {sh[0][m][c]};
+      for (int w = 1; w < waves; ++w) v[0] += sh[w][m][c];
+      finish<1>(e, m, n0 + c, v);
+    }
+  }
+}
+
+// Rows of any alignment and length -> rows of whole 16-byte chunks, zeros behind; units of T (4 bytes
+// where the rows are aligned for it), `ldo` and `ldi` in units, 32 KB of a row per workgroup and pass.
+template <typename T>
+__global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int cols, T* out, int ldo) {
+  in += (long)blockIdx.x * ldi;
+  out += (long)blockIdx.x * ldo;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < ldo; c += 256) out[c] = c < cols ? in[c] : (T)0;
+}
+
 // ---- tiled kernel --------------------------------------------------------------------------------
 //
 // BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
@@ -243,8 +313,9 @@ struct TileCopy {
     base = (const char*)a.p + (RC ? k0 * a.ld + r0 : r0 * a.ld + k0) * ES;
     step = RC ? BK * a.ld * ES : ROWB;
     ldb = (unsigned)(a.ld * ES);
-    cols = (unsigned)((a.R - r0) * ES);
-    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
+    // (ragged ends are zeros up to the next whole chunk: the operand was packed)
+    cols = (unsigned)((a.R - r0) * ES + 15) & ~15u;
+    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + ((unsigned)((K - k0) * ES + 15) & ~15u);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = (i * NW + wave) * 64 + lane;
@@ -583,33 +654,102 @@ inline bool tileable(const Mat& a, bool rc, int K, int es) {
   return a.vec && (rc ? a.R : K) % (16 / es) == 0 && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
 }
 
-template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
-int tiled(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
-  const int bk = ROWB / ES, tm = dd_ceil_div(P.R, BM), tn = dd_ceil_div(Q.R, BN), ktiles = dd_ceil_div(K, bk);
-  const long tiles = (long)tm * tn;
-  int S = 1;
-  if (tiles < 192 && ktiles >= 16) {
-    S = (int)max(1l, min(256 / tiles, (long)ktiles / 8));
-    while (S > 1 && sizeof(float) * (size_t)P.R * Q.R * S > (ws ? ws_bytes : 0)) --S;
+// The tile shapes, and what a step of 128 contraction bytes takes when `slots` of them fill the chip
+// (microseconds, measured at 8192^3, 37500 x 1024 x 2048 and 2500 x 2048 x 1536) and beside that a tile's start and
+// epilogue.  256 x 256 is the fastest per output (1340 TFLOP/s, bf16); the small ones waste less where a
+// few tiles are left over for a last round.
+struct TileShape { int bm, bn, slots; float step, rest; };
+constexpr TileShape SHAPES[] = {{256, 256, 256, 1.6f, 7.f}, {128, 128, 512, 1.1f, 4.f}, {64, 128, 768, 0.8f, 3.f}};
+constexpr int N_SHAPES = 3;
+
+struct Plan { int shape, splits; float us; };
+inline Plan plan_product(long M, long N, int ksteps, bool rc_rows, size_t slab_room) {
+  Plan best{0, 1, 1e30f};
+  for (int i = 0; i < N_SHAPES; ++i) {
+    const TileShape& t = SHAPES[i];
+    if (rc_rows && t.bm % 128) continue;   // (the transposed tile's chunk permutation wants 16 chunks a row)
+    const long tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    for (int s = 1; s <= 16 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
+      if (s > 1 && sizeof(float) * (size_t)(M * N) * s > slab_room) break;
+      const long wgs = tiles * s, full = wgs / t.slots, left = wgs % t.slots;
+      const float steps = (float)((ksteps + s - 1) / s);
+      // a last round with one tile per CU or less has the CU's paths to itself
+      const float last = left == 0 ? 0.f : (left <= 256 && t.slots > 256 ? 0.65f * t.step * steps + t.rest : t.step * steps + t.rest);
+      float us = full * (t.step * steps + t.rest) + last;
+      if (s > 1) us += 6.f + (float)(M * N) * s * 8.f / 3.5e6f;   // partial sums out and in, one more launch
+      if (us < best.us) best = {i, s, us};
+    }
   }
-  const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
-  DD_REQUIRE(tiles * parts < (1l << 31), "dd_linear: too many tiles");
-  k_linear_tile<ES, P_RC, Q_RC, BM, BN, WM, WN><<<(unsigned)(tiles * parts), 64 * WM * WN, 0, st>>>(
-      P, Q, K, kspan, tm, tn, parts > 1 ? ws : nullptr, e);
+  return best;
+}
+
+template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
+int tiled(const char* who, Mat P, Mat Q, int K, int splits, const Epi& e, float* slabs, hipStream_t st) {
+  const int bk = ROWB / ES, tm = dd_ceil_div(P.R, BM), tn = dd_ceil_div(Q.R, BN), ksteps = dd_ceil_div(K, bk);
+  const int kspan = dd_ceil_div(ksteps, splits) * bk, parts = dd_ceil_div(K, kspan);
+  DD_REQUIRE((long)tm * tn * parts < (1l << 31), "dd_linear: too many tiles");
+  k_linear_tile<ES, P_RC, Q_RC, BM, BN, WM, WN><<<(unsigned)((long)tm * tn * parts), 64 * WM * WN, 0, st>>>(
+      P, Q, K, kspan, tm, tn, parts > 1 ? slabs : nullptr, e);
   DD_CHECK_LAUNCH(who);
   if (parts > 1) {
-    sum_slabs(ws, parts, P.R, Q.R, e, st);
+    sum_slabs(slabs, parts, P.R, Q.R, e, st);
     DD_CHECK_LAUNCH(who);
   }
   return 0;
 }
 
+// The operand with rows that the tiled kernel can read, copied into the workspace unless it has them
+// already; false: no room.
+template <int ES>
+bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
+  if (tileable(a, rc, K, ES)) return true;
+  const long rows = rc ? K : a.R;
+  const int cols = rc ? a.R : K, chunks = dd_ceil_div(cols, 16 / ES);
+  const size_t bytes = ((size_t)rows * chunks * 16 + 255) / 256 * 256;
+  if (bytes > room) return false;
+  const unsigned grid = (unsigned)rows;
+  if ((uintptr_t)a.p % 4 == 0 && a.ld * ES % 4 == 0 && cols * ES % 4 == 0)
+    k_linear_pack<unsigned><<<grid, 256, 0, st>>>((const unsigned*)a.p, a.ld * ES / 4, cols * ES / 4, (unsigned*)ws, chunks * 4);
+  else if (ES == 2)
+    k_linear_pack<unsigned short><<<grid, 256, 0, st>>>((const unsigned short*)a.p, a.ld, cols, (unsigned short*)ws, chunks * 8);
+  else
+    k_linear_pack<unsigned char><<<grid, 256, 0, st>>>((const unsigned char*)a.p, a.ld, cols, (unsigned char*)ws, chunks * 16);
+  a.p = ws;
+  a.ld = chunks * (16 / ES);
+  a.vec = 1;
+  ws += bytes;
+  room -= bytes;
+  return true;
+}
+
 template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
-  static const int force = getenv("DD_LIN_TILE") ? atoi(getenv("DD_LIN_TILE")) : -1;
-  if (K > 0 && tileable(P, P_RC, K, ES) && tileable(Q, Q_RC, K, ES) && force != 0) {
-    if (force == 1 || (force < 0 && (long)P.R * Q.R >= 256l * 256 * 128)) return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, P, Q, K, e, ws, ws_bytes, st);
-    if (force == 2 || force < 0) return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, P, Q, K, e, ws, ws_bytes, st);
+  if constexpr (!P_RC && !Q_RC)
+    if (P.R <= 64 && P.vec && Q.vec && K % (16 / ES) == 0) {
+      const int threads = 64 * max(4, min(16, K / (ES == 2 ? 64 : 256)));
+      const unsigned grid = dd_ceil_div(Q.R, 16);
+      if (P.R <= 16) k_linear_few<ES, 1><<<grid, threads, 0, st>>>(P, Q, K, e);
+      else if (P.R <= 32) k_linear_few<ES, 2><<<grid, threads, 0, st>>>(P, Q, K, e);
+      else k_linear_few<ES, 4><<<grid, min(threads, 512), 0, st>>>(P, Q, K, e);
+      DD_CHECK_LAUNCH(who);
+      return 0;
+    }
+  // The tiled kernel, on packed copies of operands whose rows are no whole 16-byte chunks where the
+  // product is large enough to pay for the copies (2500 x 2048 x 1542: 25 us more, against 190 us for the
+  // general kernel).
+  char* at = (char*)(((uintptr_t)ws + 255) / 256 * 256);
+  size_t room = ws && ws_bytes > 512 ? ws_bytes - 256 : 0;
+  if (K > 0 && ((tileable(P, P_RC, K, ES) && tileable(Q, Q_RC, K, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
+    Mat p = P, q = Q;
+    if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
+      const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), P_RC, room);
+      switch (plan.shape) {
+        case 0: return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
+        case 1: return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, p, q, K, plan.splits, e, (float*)at, st);
+        default:
+          if constexpr (!P_RC) return tiled<ES, P_RC, Q_RC, 64, 128, 1, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
+      }
+    }
   }
   const int bk = ROWB / ES;
   const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));

@@ -601,27 +601,32 @@ class HipOps:
     """(ptr, ld) of a [rows, cols] view on this device in one of `dtypes`; None: (0, 0)."""
     if t is None:
       return 0, 0
-    assert t.get_device() == self._index, f'{what} is on {t.device}, not on {self.device}'
-    assert t.shape == (rows, cols), f'{what} is {tuple(t.shape)}, not {(rows, cols)}'
-    assert t.dtype in dtypes, f'{what} is {t.dtype}, not one of {dtypes}'
-    return _mat(t)
+    if t.get_device() != self._index or t.shape != (rows, cols) or t.dtype not in dtypes:
+      raise AssertionError(f'{what} is {tuple(t.shape)} {t.dtype} on {t.device}, not {(rows, cols)} in one of {dtypes} '
+                           f'on {self.device}')
+    ld, unit = t.stride()
+    assert unit == 1 or cols == 1, f'{what}: the columns are strided ({unit})'
+    return t.data_ptr(), (ld if rows > 1 else max(cols, ld))
 
   def _flat(self, t, n, what, dtypes=(torch.float32,)):
     """Pointer of a contiguous tensor of n values; None: 0."""
     if t is None:
       return 0
-    assert t.get_device() == self._index, f'{what} is on {t.device}, not on {self.device}'
-    assert t.numel() == n and t.is_contiguous() and t.dtype in dtypes, f'{what}: {n} contiguous values of {dtypes} are needed'
+    if t.get_device() != self._index or t.numel() != n or t.dtype not in dtypes or not t.is_contiguous():
+      raise AssertionError(f'{what} is {tuple(t.shape)} {t.dtype} on {t.device}: {n} contiguous values in one of {dtypes} '
+                           f'are needed on {self.device}')
     return t.data_ptr()
 
   def _block_call(self, name, *args):
     """Launch on this device's current stream, whichever device is current."""
-    if torch.cuda.current_device() != self._index:
+    stream = torch._C._cuda_getCurrentRawStream(self._index)
+    if torch._C._cuda_getDevice() != self._index:
       with torch.cuda.device(self._index):
-        rc = getattr(self.lib, name)(*args, self.stream)
+        rc = getattr(self.lib, name)(*args, stream)
     else:
-      rc = getattr(self.lib, name)(*args, self.stream)
-    self._check(rc, name)
+      rc = getattr(self.lib, name)(*args, stream)
+    if rc != 0:
+      self._check(rc, name)
 
   def rms_norm_fwd(self, x, gamma, y, rstd=None, res=None, s=None, scale=None, eps=1e-6):
     """s = x + res (in res' type; s may be res or x), y = s / sqrt(mean(s^2) + eps) * gamma.  y in fp32,
