@@ -8,8 +8,16 @@
 // A step is the map x -> A x + B; maps compose associatively, so a workgroup's waves take consecutive
 // runs of STEPS time steps of the same channels, compose their run, exchange the pairs in LDS and then
 // run their steps from the state that reaches them: a step's operands are read once and its a, b stay
-// in registers.  Few sequences with many steps: the time axis is split over workgroups as well, whose
-// pairs a first launch puts into the workspace.
+// in registers.  Up to 64 steps are in flight at once, all loads issued before the first is used.  Few
+// sequences with many steps: the time axis is split over workgroups as well, whose pairs a first launch
+// puts into the workspace.
+//
+// Bound: HBM, with the vector unit close behind (two to three sigmoids and a tanh per element, a quarter
+// of the rate each for exponential and reciprocal).  Hence: restarts are a property of a row, the same for
+// all lanes, and are looked at once per run of steps - runs without one (nearly all) take plain
+// multiply-adds; and with bf16 operands 1 - sigmoid and 1 - 2 / (1 + e^2c) stand for the forms that keep
+// their relative precision near zero (absolute error 2 u of one, where the stored result is good to 2^-8
+// of itself).
 //
 // A restart is A == 0 EXACTLY and cuts whatever came before, non-finite values too (0 * NaN would
 // not); every other factor is kept at or above FLT_MIN, so that a product that underflows does not look
@@ -20,6 +28,7 @@
 namespace {
 
 constexpr int STEPS = 8;   // time steps of one wave between two exchanges
+constexpr int WAVES = 8;   // waves of a workgroup at most
 
 struct ScanArgs {
   const void* u; long ldu;
@@ -48,74 +57,130 @@ __device__ __forceinline__ void st(void* p, long off, const float v[VC]) {
   else store_bf16<VC>((__bf16*)p + off, v);
 }
 
-__device__ __forceinline__ float at_least_min(float a) { return a < FLT_MIN ? FLT_MIN : a; }
-__device__ __forceinline__ float apply(float A, float B, float x) { return A == 0.f ? B : __builtin_fmaf(A, x, B); }
+// FLT_MIN at least.  A NaN factor stays one; a product of factors may lose it (max), because by then it is
+// in the pair's other half, where it stays.
+__device__ __forceinline__ float factor(float a) { return a < FLT_MIN ? FLT_MIN : a; }
+__device__ __forceinline__ float at_least_min(float a) { return fmaxf(a, FLT_MIN); }
+__device__ __forceinline__ float apply(float A, float B, float x) { return A == 0.f ? B : fma_(A, x, B); }
 // (A2, B2) after (A1, B1), into (A1, B1)
 __device__ __forceinline__ void compose(float& A1, float& B1, float A2, float B2) {
   B1 = apply(A2, B2, B1);
   A1 = (A1 == 0.f || A2 == 0.f) ? 0.f : at_least_min(A1 * A2);
 }
 
-// decay and gate of one element
-__device__ __forceinline__ void gates(float v, bool restart, float& a, float& z) {
-  float q;
-  sigmoid2(v, z, q);
-  a = restart ? 0.f : at_least_min(q);
-}
-__device__ __forceinline__ float sigmoid1(float x) { float p, q; sigmoid2(x, p, q); return p; }
-
-// The pair of one element's step: forward b from the gates, backward a * dh.
-template <typename E, int VC, bool GATE, bool BWD>
-__device__ __forceinline__ void step_pair(const ScanArgs& p, long row, int d, bool restart, float a[VC], float b[VC]) {
-  float u[VC], z[VC];
-  ld<E, VC>(p.u, row * p.ldu + d, u);
-#pragma unroll
-  for (int j = 0; j < VC; ++j) gates(u[j] + p.shift, restart, a[j], z[j]);
-  if constexpr (BWD) {
-    ld<E, VC>(p.dh, row * p.lddh + d, b);
-#pragma unroll
-    for (int j = 0; j < VC; ++j) b[j] = a[j] * b[j];
+// z = sigmoid(u + shift) and the decay q = 1 - z; phi(c); sigmoid(i).  LOW: absolute precision is enough.
+template <bool LOW>
+__device__ __forceinline__ void gates(float u, float shift, float& z, float& q) {
+  if constexpr (LOW) {
+    z = fast_rcp(1.0f + __builtin_amdgcn_exp2f(fma_(u, -1.44269504088896341f, shift * -1.44269504088896341f)));
+    q = 1.0f - z;
   } else {
-    float c[VC], i[VC];
-    ld<E, VC>(p.c, row * p.ldc + d, c);
-    if constexpr (GATE) ld<E, VC>(p.i, row * p.ldi + d, i);
+    sigmoid2(u + shift, z, q);
+  }
+  q = factor(q);
+}
+template <bool LOW>
+__device__ __forceinline__ float phi_of(float c, int tanh_c) {
+  if (!tanh_c) return c;
+  if constexpr (LOW) return fma_(-2.0f, fast_rcp(1.0f + __builtin_amdgcn_exp2f(c * 2.88539008177792681f)), 1.0f);
+  else return tanh_f(c);
+}
+__device__ __forceinline__ float sigmoid1(float x) { return fast_rcp(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f)); }
+
+// Bit s: step o0 + s (in scan order, of `n`) of sequence b starts anew.  One load for the wave's run.
+template <bool BWD>
+__device__ __forceinline__ unsigned restarts(const ScanArgs& p, long b, int o0, int n, int lane) {
+  if (!p.first) return 0;
+  bool r = false;
+  if (lane < n) r = p.first[(b * p.T + (BWD ? p.T - 1 - o0 - lane : o0 + lane)) * p.fstride] != 0.f;
+  return (unsigned)__ballot(r);
+}
+
+// The pairs (a, b) of a run of up to STEPS steps in scan order, identity past n, zero a at restarts.
+// Forward b = gate phi(c); backward b = a dh.  z, q as in gates (backward keeps them).
+template <typename E, int VC, bool GATE, bool BWD>
+__device__ __forceinline__ void run_pairs(const ScanArgs& p, long b, int o0, int n, unsigned cut, int d, float z[STEPS][VC],
+                                          float q[STEPS][VC], float bb[STEPS][VC]) {
+  constexpr bool LOW = sizeof(E) == 2;
+  float u[STEPS][VC], c[STEPS][VC], i[STEPS][VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) b[j] = (GATE ? sigmoid1(i[j]) : z[j]) * (p.tanh_c ? tanh_f(c[j]) : c[j]);
+  for (int s = 0; s < STEPS; ++s) {
+    const int o = o0 + min(s, n - 1);
+    const long row = b * p.T + (BWD ? p.T - 1 - o : o);
+    ld<E, VC>(p.u, row * p.ldu + d, u[s]);
+    if constexpr (BWD) {
+      ld<E, VC>(p.dh, row * p.lddh + d, bb[s]);
+    } else {
+      ld<E, VC>(p.c, row * p.ldc + d, c[s]);
+      if constexpr (GATE) ld<E, VC>(p.i, row * p.ldi + d, i[s]);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+      gates<LOW>(u[s][j], p.shift, z[s][j], q[s][j]);
+      if constexpr (!BWD) bb[s][j] = (GATE ? sigmoid1(i[s][j]) : z[s][j]) * phi_of<LOW>(c[s][j], p.tanh_c);
+    }
+}
+
+// The run's composed pair.
+template <int VC, bool BWD>
+__device__ __forceinline__ void run_total(int n, unsigned cut, const float q[STEPS][VC], const float bb[STEPS][VC], float A[VC],
+                                          float B[VC]) {
+#pragma unroll
+  for (int j = 0; j < VC; ++j) { A[j] = 1.f; B[j] = 0.f; }
+  if (cut == 0 && n == STEPS) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < VC; ++j) {
+        const float a = q[s][j];
+        B[j] = BWD ? a * (B[j] + bb[s][j]) : fma_(a, B[j], bb[s][j]);
+        A[j] = at_least_min(A[j] * a);
+      }
+  } else {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+      if (s < n)
+#pragma unroll
+        for (int j = 0; j < VC; ++j) {
+          const float a = cut >> s & 1 ? 0.f : q[s][j];
+          compose(A[j], B[j], a, BWD ? (a == 0.f ? 0.f : a * bb[s][j]) : bb[s][j]);
+        }
   }
 }
 
 // First launch of a split time axis: the pairs of all splits but the last (in scan order), and in
 // slot 0 the initial state as a restart, so that a state updated in place is read before it is written.
 template <typename E, int VC, bool GATE, bool BWD>
-__global__ void __launch_bounds__(256) k_scan_pairs(ScanArgs p) {
-  __shared__ float2 sh[4][64 * VC];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(64 * WAVES) k_scan_pairs(ScanArgs p) {
+  __shared__ float2 sh[WAVES][64 * VC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int k = blockIdx.x % (p.splits - 1), g = (blockIdx.x / (p.splits - 1)) % p.groups;
   const long b = blockIdx.x / (p.splits - 1) / p.groups;
-  const int d = (g * 64 + lane) * VC;
-  const bool live = d < p.D;
-  const int len = p.span / 4;   // this wave's run, in scan order
+  const int d = min((g * 64 + lane) * VC, p.D - VC);
+  const bool live = (g * 64 + lane) * VC < p.D;
+  const int len = p.span / WAVES;   // this wave's steps, in scan order: a multiple of STEPS; the last split is not here
   float A[VC], Bv[VC];
 #pragma unroll
   for (int j = 0; j < VC; ++j) { A[j] = 1.f; Bv[j] = 0.f; }
-  if (live)
-#pragma unroll 4
-    for (int s = 0; s < len; ++s) {
-      const int o = k * p.span + wave * len + s;   // the last split is not here: o < T
-      const int t = BWD ? p.T - 1 - o : o;
-      const long row = b * p.T + t;
-      float a[VC], bb[VC];
-      step_pair<E, VC, GATE, BWD>(p, row, d, p.first && p.first[row * p.fstride] != 0.f, a, bb);
+  for (int s = 0; s < len; s += STEPS) {
+    const int o0 = k * p.span + wave * len + s;
+    float z[STEPS][VC], q[STEPS][VC], bb[STEPS][VC], a2[VC], b2[VC];
+    const unsigned cut = restarts<BWD>(p, b, o0, STEPS, lane);
+    run_pairs<E, VC, GATE, BWD>(p, b, o0, STEPS, cut, d, z, q, bb);
+    run_total<VC, BWD>(STEPS, cut, q, bb, a2, b2);
 #pragma unroll
-      for (int j = 0; j < VC; ++j) compose(A[j], Bv[j], a[j], bb[j]);
-    }
+    for (int j = 0; j < VC; ++j) compose(A[j], Bv[j], a2[j], b2[j]);
+  }
 #pragma unroll
   for (int j = 0; j < VC; ++j) sh[wave][lane * VC + j] = make_float2(A[j], Bv[j]);
   __syncthreads();
   if (wave == 0 && live)
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      for (int w = 1; w < 4; ++w) compose(A[j], Bv[j], sh[w][lane * VC + j].x, sh[w][lane * VC + j].y);
+      for (int w = 1; w < WAVES; ++w) compose(A[j], Bv[j], sh[w][lane * VC + j].x, sh[w][lane * VC + j].y);
       float2* out = p.pairs + b * p.splits * p.D + d + j;
       out[(long)(k + 1) * p.D] = make_float2(A[j], Bv[j]);
       if (k == 0) out[0] = make_float2(0.f, p.x0 ? p.x0[b * p.D + d + j] : 0.f);
@@ -131,6 +196,7 @@ __device__ __forceinline__ void start_state(const ScanArgs& p, long b, int k, in
     if (p.x0) load_f32<VC>(p.x0 + b * p.D + d, x);
     return;
   }
+#pragma unroll 8
   for (int s = 0; s <= k; ++s) {
     const float2* q = p.pairs + (b * p.splits + s) * p.D + d;
 #pragma unroll
@@ -160,9 +226,9 @@ __device__ __forceinline__ void exchange(float2 (*sh)[64 * VC], int wave, int wa
 }
 
 template <typename E, int VC, bool GATE>
-__global__ void __launch_bounds__(256) k_scan_fwd(ScanArgs p) {
-  __shared__ float2 sh[2][4][64 * VC];   // two buffers: one barrier per exchange
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+__global__ void __launch_bounds__(64 * WAVES) k_scan_fwd(ScanArgs p) {
+  __shared__ float2 sh[2][WAVES][64 * VC];   // two buffers: one barrier per exchange
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int k = blockIdx.x % p.splits, g = (blockIdx.x / p.splits) % p.groups;
   const long b = blockIdx.x / p.splits / p.groups;
   const int d = min((g * 64 + lane) * VC, p.D - VC);   // lanes past the last channel repeat it, and store nothing
@@ -172,38 +238,32 @@ __global__ void __launch_bounds__(256) k_scan_fwd(ScanArgs p) {
   start_state<VC>(p, b, k, d, x);
   int buf = 0;
   for (int base = k * p.span; base < end; base += waves * STEPS, buf ^= 1) {
-    float a[STEPS][VC], bb[STEPS][VC], A[VC], Bv[VC], in[VC];
+    const int o0 = base + wave * STEPS, n = min(STEPS, end - o0);   // n <= 0: a wave behind the end
+    float z[STEPS][VC], q[STEPS][VC], bb[STEPS][VC], A[VC], Bv[VC], in[VC];
+    const unsigned cut = restarts<false>(p, b, o0, n, lane);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int t = base + wave * STEPS + s;
-      const long row = b * p.T + min(t, end - 1);
-      step_pair<E, VC, GATE, false>(p, row, d, p.first && p.first[row * p.fstride] != 0.f, a[s], bb[s]);
-#pragma unroll
-      for (int j = 0; j < VC; ++j)
-        if (t >= end) { a[s][j] = 1.f; bb[s][j] = 0.f; }
+    for (int j = 0; j < VC; ++j) { A[j] = 1.f; Bv[j] = 0.f; }
+    if (n > 0) {
+      run_pairs<E, VC, GATE, false>(p, b, o0, n, cut, d, z, q, bb);
+      run_total<VC, false>(n, cut, q, bb, A, Bv);
     }
-#pragma unroll
-    for (int j = 0; j < VC; ++j) { A[j] = a[0][j]; Bv[j] = bb[0][j]; }
-#pragma unroll
-    for (int s = 1; s < STEPS; ++s)
-#pragma unroll
-      for (int j = 0; j < VC; ++j) compose(A[j], Bv[j], a[s][j], bb[s][j]);
     exchange<VC>(sh[buf], wave, waves, lane, A, Bv, x, in);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int t = base + wave * STEPS + s;
+      if (s >= n) break;
 #pragma unroll
-      for (int j = 0; j < VC; ++j) in[j] = apply(a[s][j], bb[s][j], in[j]);
-      if (live && t < end) st<E, VC>(p.h, (b * p.T + t) * p.ldh + d, in);
+      for (int j = 0; j < VC; ++j) in[j] = cut >> s & 1 ? bb[s][j] : fma_(q[s][j], in[j], bb[s][j]);
+      if (live) st<E, VC>(p.h, (b * p.T + o0 + s) * p.ldh + d, in);
     }
   }
   if (p.xT && live && k == p.splits - 1 && wave == 0) store_f32<VC>(p.xT + b * p.D + d, x);
 }
 
 template <typename E, int VC, bool GATE>
-__global__ void __launch_bounds__(256) k_scan_bwd(ScanArgs p) {
-  __shared__ float2 sh[2][4][64 * VC];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+__global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
+  constexpr bool LOW = sizeof(E) == 2;
+  __shared__ float2 sh[2][WAVES][64 * VC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int k = blockIdx.x % p.splits, g = (blockIdx.x / p.splits) % p.groups;
   const long b = blockIdx.x / p.splits / p.groups;
   const int d = min((g * 64 + lane) * VC, p.D - VC);
@@ -213,69 +273,59 @@ __global__ void __launch_bounds__(256) k_scan_bwd(ScanArgs p) {
   start_state<VC>(p, b, k, d, x);
   int buf = 0;
   for (int base = k * p.span; base < end; base += waves * STEPS, buf ^= 1) {
-    float u[STEPS][VC], dh[STEPS][VC], c[STEPS][VC], gi[STEPS][VC], hp[STEPS][VC], A[VC], Bv[VC], in[VC];
-    bool restart[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int t = p.T - 1 - min(base + wave * STEPS + s, end - 1);
-      const long row = b * p.T + t;
-      ld<E, VC>(p.u, row * p.ldu + d, u[s]);
-      ld<E, VC>(p.dh, row * p.lddh + d, dh[s]);
-      ld<E, VC>(p.c, row * p.ldc + d, c[s]);
-      if constexpr (GATE) ld<E, VC>(p.i, row * p.ldi + d, gi[s]);
-      if (t > 0) {
-        ld<E, VC>(p.h, (row - 1) * p.ldh + d, hp[s]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VC; ++j) hp[s][j] = 0.f;
-        if (p.h0) load_f32<VC>(p.h0 + b * p.D + d, hp[s]);
-      }
-      restart[s] = p.first && p.first[row * p.fstride] != 0.f;
-    }
+    const int o0 = base + wave * STEPS, n = min(STEPS, end - o0);
+    float z[STEPS][VC], q[STEPS][VC], dh[STEPS][VC], c[STEPS][VC], gi[STEPS][VC], hp[STEPS][VC], A[VC], Bv[VC], in[VC];
+    const unsigned cut = restarts<true>(p, b, o0, n, lane);
 #pragma unroll
     for (int j = 0; j < VC; ++j) { A[j] = 1.f; Bv[j] = 0.f; }
+    if (n > 0) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-      if (base + wave * STEPS + s < end)
+      for (int s = 0; s < STEPS; ++s) {
+        const long row = b * p.T + p.T - 1 - (o0 + min(s, n - 1));
+        ld<E, VC>(p.c, row * p.ldc + d, c[s]);
+        if constexpr (GATE) ld<E, VC>(p.i, row * p.ldi + d, gi[s]);
+        ld<E, VC>(p.h, max(row - 1, 0l) * p.ldh + d, hp[s]);
+      }
+      if (o0 + n == p.T) {   // the run's last step is the sequence's first: its state before is h0
+        float first[VC] = {};
+        if (p.h0) load_f32<VC>(p.h0 + b * p.D + d, first);
 #pragma unroll
-        for (int j = 0; j < VC; ++j) {
-          float a, z;
-          gates(u[s][j] + p.shift, restart[s], a, z);
-          compose(A[j], Bv[j], a, a * dh[s][j]);
-        }
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+          for (int j = 0; j < VC; ++j) hp[s][j] = s == n - 1 ? first[j] : hp[s][j];
+      }
+      run_pairs<E, VC, GATE, true>(p, b, o0, n, cut, d, z, q, dh);
+      run_total<VC, true>(n, cut, q, dh, A, Bv);
+    }
     exchange<VC>(sh[buf], wave, waves, lane, A, Bv, x, in);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int o = base + wave * STEPS + s;
-      if (o < end) {
-        float du[VC], dc[VC], di[VC];
+      if (s >= n) break;
+      const bool restart = cut >> s & 1;
+      float du[VC], dc[VC], di[VC];
 #pragma unroll
-        for (int j = 0; j < VC; ++j) {
-          float z, q;
-          sigmoid2(u[s][j] + p.shift, z, q);
-          const float a = restart[s] ? 0.f : at_least_min(q);
-          const float gr = dh[s][j] + in[j];             // d loss / d h[t]
-          in[j] = a == 0.f ? 0.f : a * gr;
-          const float phi = p.tanh_c ? tanh_f(c[s][j]) : c[s][j];
-          const float slope = p.tanh_c ? 1.f - phi * phi : 1.f;
-          const float before = restart[s] ? 0.f : hp[s][j];
-          if constexpr (GATE) {
-            float w, wq;
-            sigmoid2(gi[s][j], w, wq);
-            du[j] = -gr * before * z * q;
-            di[j] = gr * phi * w * wq;
-            dc[j] = gr * w * slope;
-          } else {
-            du[j] = gr * (phi - before) * z * q;
-            dc[j] = gr * z * slope;
-          }
+      for (int j = 0; j < VC; ++j) {
+        const float gr = dh[s][j] + in[j];             // d loss / d h[t]
+        in[j] = restart ? 0.f : q[s][j] * gr;
+        const float phi = phi_of<LOW>(c[s][j], p.tanh_c);
+        const float slope = p.tanh_c ? fma_(-phi, phi, 1.f) : 1.f;
+        const float before = restart ? 0.f : hp[s][j];
+        const float gz = gr * z[s][j];
+        if constexpr (GATE) {
+          const float w = sigmoid1(gi[s][j]), gw = gr * w;
+          du[j] = -gz * q[s][j] * before;
+          di[j] = gw * phi * (1.f - w);
+          dc[j] = gw * slope;
+        } else {
+          du[j] = gz * q[s][j] * (phi - before);
+          dc[j] = gz * slope;
         }
-        if (live) {
-          const long row = b * p.T + p.T - 1 - o;
-          st<E, VC>(p.du, row * p.lddu + d, du);
-          st<E, VC>(p.dc, row * p.lddc + d, dc);
-          if constexpr (GATE) st<E, VC>(p.di, row * p.lddi + d, di);
-        }
+      }
+      if (live) {
+        const long row = b * p.T + p.T - 1 - o0 - s;
+        st<E, VC>(p.du, row * p.lddu + d, du);
+        st<E, VC>(p.dc, row * p.lddc + d, dc);
+        if constexpr (GATE) st<E, VC>(p.di, row * p.lddi + d, di);
       }
     }
   }
@@ -283,14 +333,15 @@ __global__ void __launch_bounds__(256) k_scan_bwd(ScanArgs p) {
 }
 
 // Splits of the time axis: none where the channels alone give every CU a workgroup; else enough for
-// four workgroups per CU, each at least two exchanges (64 steps) long.
+// four workgroups per CU, each at least two exchanges of all waves long.
 inline void plan(ScanArgs& p) {
+  constexpr int PASS = WAVES * STEPS;
   const long wgs = (long)p.B * p.groups;
   p.splits = 1;
   p.span = p.T;
-  if (wgs < 256 && p.T >= 128) {
-    const long want = min((1024 + wgs - 1) / wgs, (long)p.T / 64);
-    p.span = dd_ceil_div(dd_ceil_div(p.T, want), 32) * 32;
+  if (wgs < 256 && p.T >= 4 * PASS) {
+    const long want = min((1024 + wgs - 1) / wgs, (long)p.T / (2 * PASS));
+    p.span = dd_ceil_div(dd_ceil_div(p.T, want), PASS) * PASS;
     p.splits = dd_ceil_div(p.T, p.span);
     if (p.splits == 1) p.span = p.T;
   }
@@ -306,28 +357,23 @@ int launch(ScanArgs& p, float* ws, size_t ws_bytes, hipStream_t stream) {
     DD_REQUIRE(ws_bytes >= sizeof(float2) * (size_t)p.B * p.splits * p.D, "dd_gated_scan: the workspace is too small");
     DD_REQUIRE((uintptr_t)ws % 8 == 0, "dd_gated_scan: the workspace is not 8-byte aligned");
     p.pairs = (float2*)ws;
-    k_scan_pairs<E, VC, GATE, BWD><<<(unsigned)((long)p.B * p.groups * (p.splits - 1)), 256, 0, stream>>>(p);
+    k_scan_pairs<E, VC, GATE, BWD><<<(unsigned)((long)p.B * p.groups * (p.splits - 1)), 64 * WAVES, 0, stream>>>(p);
     DD_CHECK_LAUNCH("dd_gated_scan(pairs)");
   }
-  const int threads = p.T <= STEPS ? 64 : 256;
+  const int threads = 64 * min(WAVES, dd_ceil_div(p.T, STEPS));
   if constexpr (BWD) k_scan_bwd<E, VC, GATE><<<(unsigned)wgs, threads, 0, stream>>>(p);
   else k_scan_fwd<E, VC, GATE><<<(unsigned)wgs, threads, 0, stream>>>(p);
   DD_CHECK_LAUNCH(BWD ? "dd_gated_scan_bwd" : "dd_gated_scan_fwd");
   return 0;
 }
 
+// bf16: two channels per lane (256 bytes of a row per wave) where that leaves two workgroups per CU.
 template <bool BWD>
 int dispatch(ScanArgs& p, int type, float* ws, size_t ws_bytes, hipStream_t st) {
-  const int w = 2 * dtype_size(type);
-  const bool pair = p.D % 2 == 0 && rows_aligned(p.u, p.ldu, type, w) && rows_aligned(p.c, p.ldc, type, w) &&
-                    rows_aligned(p.i, p.ldi, type, w) && rows_aligned(p.h, p.ldh, type, w) &&
-                    rows_aligned(p.dh, p.lddh, type, w) && rows_aligned(p.du, p.lddu, type, w) &&
-                    rows_aligned(p.dc, p.lddc, type, w) && rows_aligned(p.di, p.lddi, type, w) &&
-                    rows_aligned(p.x0, 0, DD_F32, 8) && rows_aligned(p.xT, 0, DD_F32, 8) && rows_aligned(p.h0, 0, DD_F32, 8);
 #define DD_SCAN(E_, VC_) \
   return p.i ? launch<E_, VC_, true, BWD>(p, ws, ws_bytes, st) : launch<E_, VC_, false, BWD>(p, ws, ws_bytes, st)
-  if (type == DD_F32) { if (pair) DD_SCAN(float, 2); DD_SCAN(float, 1); }
-  if (pair) DD_SCAN(__bf16, 2);
+  if (type == DD_F32) DD_SCAN(float, 1);
+  if (p.D % 2 == 0 && (long)p.B * dd_ceil_div(p.D, 128) >= 512) DD_SCAN(__bf16, 2);
   DD_SCAN(__bf16, 1);
 #undef DD_SCAN
 }

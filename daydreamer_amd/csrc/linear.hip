@@ -766,50 +766,43 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   return 0;
 }
 
-// dz = dy act'(z), and the workgroup's share of dbias.  act 0: dz == dy, only the column sums.
-template <int V>
+// dz = dy act'(z), and the workgroup's share of dbias; without an activation dz IS dy and only the column
+// sums are taken.  HBM-bound: 64 V columns per workgroup (1 KB of a row in one wave's access), four waves on
+// different rows, four rows requested at a time.
+template <int V, int ACT>
 __global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz,
-                                                 int act, float* parts, int M, int N, int rows_per) {
-  const long c = ((long)blockIdx.x * 256 + threadIdx.x) * V;
-  if (c >= N) return;
+                                                 float* parts, int M, int N, int rows_per) {
+  __shared__ float sh[3][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long c = ((long)blockIdx.x * 64 + lane) * V;
+  const long m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
   float sum[V] = {};
-  const long m0 = (long)blockIdx.y * rows_per, m1 = min((long)M, m0 + rows_per);
-  for (long m = m0; m < m1; ++m) {
-    float d[V], t[V];
-    load_bf16<V>(dy + m * ldy + c, d);
-    if (act != DD_ACT_NONE) {
-      load_bf16<V>(z + m * ldz + c, t);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        switch (act) {
-          case DD_ACT_ELU: d[j] *= act_slope<DD_ACT_ELU>(t[j]); break;
-          case DD_ACT_SILU: d[j] *= act_slope<DD_ACT_SILU>(t[j]); break;
-          default: d[j] *= act_slope<DD_ACT_GELU>(t[j]);
-        }
-      }
-      // bf16: the two products that read dz take bf16 operands
-      store_bf16<V>(dz + m * lddz + c, d);
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] += d[j];
-  }
-  if (parts) store_f32<V>(parts + (long)blockIdx.y * N + c, sum);
-}
-
-__global__ void __launch_bounds__(1024) k_bias_sum(const float* parts, int n, int N, void* out, int type, int accumulate) {
-  __shared__ float sh[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float t = 0.f;
   if (c < N)
-    for (int i = w; i < n; i += 16) t += parts[(long)i * N + c];
-  sh[w][lane] = t;
-  __syncthreads();
-  if (w || c >= N) return;
-  t = sh[0][lane];
+#pragma unroll 4
+    for (long m = (long)blockIdx.y * rows_per + wave; m < m1; m += 4) {
+      float d[V], t[V];
+      load_bf16<V>(dy + m * ldy + c, d);
+      if constexpr (ACT != DD_ACT_NONE) {
+        load_bf16<V>(z + m * ldz + c, t);
 #pragma unroll
-  for (int i = 1; i < 16; ++i) t += sh[i][lane];
-  if (type == DD_F32) { float* p = (float*)out + c; *p = accumulate ? *p + t : t; }
-  else { __bf16* p = (__bf16*)out + c; *p = (__bf16)(accumulate ? (float)*p + t : t); }
+        for (int j = 0; j < V; ++j) d[j] *= act_slope<ACT>(t[j]);
+        // bf16: the two products that read dz take bf16 operands
+        store_bf16<V>(dz + m * lddz + c, d);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += d[j];
+    }
+  if (!parts) return;
+  if (wave)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sh[wave - 1][lane * V + j] = sum[j];
+  __syncthreads();
+  if (wave || c >= N) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] += sh[w][lane * V + j];
+  store_f32<V>(parts + (long)blockIdx.y * N + c, sum);
 }
 
 inline int mat_vec(const void* p, long ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
@@ -883,21 +876,26 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
   DD_REQUIRE(M == 0 || (dy && ldy >= N), "dd_linear_act_bwd: dy is null or its leading dimension is below N");
   DD_REQUIRE(M == 0 || !act_on || (z && dz && ldz >= N && lddz >= N), "dd_linear_act_bwd: an activation needs z and dz");
   const hipStream_t st = (hipStream_t)stream;
-  const int al = 16;
-  const bool vec = N % 8 == 0 && rows_aligned(dy, ldy, DD_BF16, al) && rows_aligned(ws, 0, DD_F32, al) &&
-                   (!act_on || (rows_aligned(z, ldz, DD_BF16, al) && rows_aligned(dz, lddz, DD_BF16, al)));
-  const int cols = dd_ceil_div(dd_ceil_div(N, vec ? 8 : 1), 256);
-  const int parts = max(1, min(min(M, 512), dd_ceil_div(1024, cols)));
-  const int rows_per = dd_ceil_div(M, parts), n = rows_per ? dd_ceil_div(M, rows_per) : 0;
+  const bool vec = N % 8 == 0 && rows_aligned(dy, ldy, DD_BF16, 16) && rows_aligned(ws, 0, DD_F32, 16) &&
+                   (!act_on || (rows_aligned(z, ldz, DD_BF16, 16) && rows_aligned(dz, lddz, DD_BF16, 16)));
+  // 1024 workgroups, at least four rows each
+  const int cols = dd_ceil_div(N, vec ? 512 : 64);
+  const int rows_per = max(4, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
+  DD_REQUIRE(n <= 65535, "dd_linear_act_bwd: too many rows");
   DD_REQUIRE(!dbias || ws_bytes / sizeof(float) >= (size_t)n * N, "dd_linear_act_bwd: the workspace is too small");
   if (M > 0) {
     const dim3 grid(cols, n);
-    if (vec) k_act_bwd<8><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz, act, dbias ? ws : nullptr, M, N, rows_per);
-    else k_act_bwd<1><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz, act, dbias ? ws : nullptr, M, N, rows_per);
+#define DD_ACT_BWD(V_, A_)                                                                                              \
+  if (vec == (V_ == 8) && act == A_)                                                                                    \
+    k_act_bwd<V_, A_><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz,           \
+                                            dbias ? ws : nullptr, M, N, rows_per);
+    DD_ACT_BWD(8, DD_ACT_NONE) DD_ACT_BWD(8, DD_ACT_ELU) DD_ACT_BWD(8, DD_ACT_SILU) DD_ACT_BWD(8, DD_ACT_GELU)
+    DD_ACT_BWD(1, DD_ACT_NONE) DD_ACT_BWD(1, DD_ACT_ELU) DD_ACT_BWD(1, DD_ACT_SILU) DD_ACT_BWD(1, DD_ACT_GELU)
+#undef DD_ACT_BWD
     DD_CHECK_LAUNCH("dd_linear_act_bwd");
   }
   if (dbias) {
-    k_bias_sum<<<dd_ceil_div(N, 64), 1024, 0, st>>>(ws, n, N, dbias, bias_type, accumulate);
+    k_part_sum<<<dd_ceil_div(N, 32), 1024, 0, st>>>(ws, n, N, dbias, bias_type, accumulate);
     DD_CHECK_LAUNCH("dd_linear_act_bwd(dbias)");
   }
   return 0;

@@ -9,9 +9,8 @@
 //
 // Bound: HBM.  A row's elements stay in registers from their load to the last store - each input is
 // read once, each output written once - so a row belongs to one wave (C <= 2048), four (<= 8192) or
-// sixteen (<= 32768), 8 / 16 / 32 elements per lane.  The widest access that every operand's rows are
-// aligned for is used: 16 bytes (V = 8), two elements (V = 2: an even row length such as 1542 keeps
-// bf16 rows 4-byte aligned), or one.
+// sixteen (<= 32768), 8 / 16 / 32 elements per lane in vectors of eight (the last one of a ragged row
+// element by element).
 #include "block_core.h"
 
 namespace {
@@ -26,41 +25,53 @@ struct RmsArgs {
   int rows, C; float eps;
 };
 
-template <int V, int NC, bool ADD>
-__device__ __forceinline__ void load_row(const void* base, int type, long off, int l, int stride, int C, float v[NC][V]) {
+// Elements c = (l + stride i) 8 .. + 7 of a row as floats, zeros past C; added to v, or written to it.
+template <int NC, bool ADD>
+__device__ __forceinline__ void load_row(const void* base, int type, long off, int l, int stride, int C, float v[NC][8]) {
   if (type == DD_F32) {
     const float* p = (const float*)base + off;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (l + stride * i) * V;
-      float t[V] = {};
-      if (c < C) load_f32<V>(p + c, t);
+      const int c = (l + stride * i) * 8;
+      float t[8] = {};
+      if (c + 8 <= C) load_f32<8>(p + c, t);
+      else
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
+        for (int j = 0; j < 8; ++j) if (c + j < C) t[j] = p[c + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
     }
   } else {
     const __bf16* p = (const __bf16*)base + off;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (l + stride * i) * V;
-      float t[V] = {};
-      if (c < C) load_bf16<V>(p + c, t);
+      const int c = (l + stride * i) * 8;
+      float t[8] = {};
+      if (c + 8 <= C) load_bf16<8>(p + c, t);
+      else
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
+        for (int j = 0; j < 8; ++j) if (c + j < C) t[j] = (float)p[c + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
     }
   }
 }
 
-template <int V, int NC>
-__device__ __forceinline__ void store_row(void* base, int type, long off, int l, int stride, int C, const float v[NC][V]) {
+template <int V>
+__device__ __forceinline__ void store_as(void* base, int type, long at, const float* v) {
+  if (type == DD_F32) store_f32<V>((float*)base + at, v);
+  else if (type == DD_BF16) store_bf16<V>((__bf16*)base + at, v);
+  else store_e4m3<V>((unsigned char*)base + at, v);
+}
+template <int NC>
+__device__ __forceinline__ void store_row(void* base, int type, long off, int l, int stride, int C, const float v[NC][8]) {
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int c = (l + stride * i) * V;
-    if (c < C) {
-      if (type == DD_F32) store_f32<V>((float*)base + off + c, v[i]);
-      else if (type == DD_BF16) store_bf16<V>((__bf16*)base + off + c, v[i]);
-      else store_e4m3<V>((unsigned char*)base + off + c, v[i]);
-    }
+    const int c = (l + stride * i) * 8;
+    if (c + 8 <= C) store_as<8>(base, type, off + c, v[i]);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (c + j < C) store_as<1>(base, type, off + c + j, &v[i][j]);
   }
 }
 
@@ -77,46 +88,43 @@ __device__ __forceinline__ float row_reduce(float v, int wpr, float* red) {
   return t;
 }
 
-template <int V, int NC, bool NORM>
-__global__ void __launch_bounds__(1024) k_rms_fwd(RmsArgs a, int wpr) {
+template <int NC, bool NORM, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int wpr) {
   __shared__ float red[16];
   const int per = 64 * wpr, l = threadIdx.x % per;
   const long row = (long)blockIdx.x * (blockDim.x / per) + threadIdx.x / per;
   if (row >= a.rows) return;   // whole waves; with wpr > 1 a workgroup holds one row and never leaves
-  float v[NC][V];
-  load_row<V, NC, false>(a.x, a.xt, row * a.ldx, l, per, a.C, v);
-  if (a.r) load_row<V, NC, true>(a.r, a.rt, row * a.ldr, l, per, a.C, v);
+  float v[NC][8];
+  load_row<NC, false>(a.x, a.xt, row * a.ldx, l, per, a.C, v);
+  if (a.r) load_row<NC, true>(a.r, a.rt, row * a.ldr, l, per, a.C, v);
   if (a.s) {
     if (a.rt == DD_BF16)
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = (float)(__bf16)v[i][j];
-    store_row<V, NC>(a.s, a.rt, row * a.lds, l, per, a.C, v);
+        for (int j = 0; j < 8; ++j) v[i][j] = (float)(__bf16)v[i][j];
+    store_row<NC>(a.s, a.rt, row * a.lds, l, per, a.C, v);
   }
   if constexpr (NORM) {
-    float ss = 0.f;
+    float g[NC][8], ss = 0.f;
+    load_row<NC, false>(a.gamma, DD_F32, 0, l, per, a.C, g);
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) ss += v[i][j] * v[i][j];
+      for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
     const float rstd = 1.0f / sqrtf(row_reduce<false>(ss, wpr, red) / (float)a.C + a.eps);
     if (a.rstd && l == 0) a.rstd[row] = rstd;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = (l + per * i) * V;
-      float g[V] = {};
-      if (c < a.C) load_f32<V>(a.gamma + c, g);
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] *= rstd * g[j];
-    }
+      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * g[i][j];
   }
   if (a.yt == DD_E4M3) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(v[i][j]));
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
     m = row_reduce<true>(m, wpr, red);
     // a row of zeros (or of values whose reciprocal would overflow) is stored as zeros with scale 1
     const bool some = m >= 1e-30f;
@@ -125,12 +133,12 @@ __global__ void __launch_bounds__(1024) k_rms_fwd(RmsArgs a, int wpr) {
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const float t = v[i][j] * inv;   // at most 448 but for the roundings; a NaN stays one
         v[i][j] = t > E4M3_MAX ? E4M3_MAX : t < -E4M3_MAX ? -E4M3_MAX : t;
       }
   }
-  store_row<V, NC>(a.y, a.yt, row * a.ldy, l, per, a.C, v);
+  store_row<NC>(a.y, a.yt, row * a.ldy, l, per, a.C, v);
 }
 
 struct RmsBwdArgs {
@@ -145,28 +153,23 @@ struct RmsBwdArgs {
 
 // A workgroup strides over the rows; every lane keeps its columns' share of dgamma in registers, the
 // four waves of a workgroup are added in LDS, one partial row per workgroup goes to the workspace.
-template <int V, int NC>
-__global__ void __launch_bounds__(1024) k_rms_bwd(RmsBwdArgs a, int wpr) {
+template <int NC, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_rms_bwd(RmsBwdArgs a, int wpr) {
   extern __shared__ float sh[];   // 16 reduction slots | (wpr == 1) [4][C] partial sums
   const int per = 64 * wpr, l = threadIdx.x % per, rpb = blockDim.x / per, slot = threadIdx.x / per;
-  float g[NC][V], pg[NC][V];
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = (l + per * i) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) g[i][j] = pg[i][j] = 0.f;
-    if (c < a.C) load_f32<V>(a.gamma + c, g[i]);
-  }
+  float g[NC][8], pg[NC][8] = {};
+  load_row<NC, false>(a.gamma, DD_F32, 0, l, per, a.C, g);
   for (long row = (long)blockIdx.x * rpb + slot; row < a.rows; row += (long)gridDim.x * rpb) {
-    float dy[NC][V], n[NC][V];
-    load_row<V, NC, false>(a.dy, a.yt, row * a.ldy, l, per, a.C, dy);
-    load_row<V, NC, false>(a.s, a.rt, row * a.lds, l, per, a.C, n);
+    float dy[NC][8], n[NC][8], dr[NC][8] = {};
+    load_row<NC, false>(a.dy, a.yt, row * a.ldy, l, per, a.C, dy);
+    load_row<NC, false>(a.s, a.rt, row * a.lds, l, per, a.C, n);
+    if (a.dres) load_row<NC, false>(a.dres, a.rt, row * a.ldr, l, per, a.C, dr);
     const float rstd = a.rstd[row];
     float s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < 8; ++j) {
         n[i][j] *= rstd;
         pg[i][j] += dy[i][j] * n[i][j];
         dy[i][j] *= g[i][j];
@@ -176,20 +179,19 @@ __global__ void __launch_bounds__(1024) k_rms_bwd(RmsBwdArgs a, int wpr) {
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) dy[i][j] = rstd * (dy[i][j] - n[i][j] * s1);
-    if (a.dres) load_row<V, NC, true>(a.dres, a.rt, row * a.ldr, l, per, a.C, dy);
-    store_row<V, NC>(a.ds, a.rt, row * a.ldd, l, per, a.C, dy);
+      for (int j = 0; j < 8; ++j) dy[i][j] = dr[i][j] + rstd * (dy[i][j] - n[i][j] * s1);
+    store_row<NC>(a.ds, a.rt, row * a.ldd, l, per, a.C, dy);
   }
   if (!a.parts) return;
   float* out = a.parts + (long)blockIdx.x * a.C;
   if (wpr > 1) {
-    store_row<V, NC>(out, DD_F32, 0, l, per, a.C, pg);
+    store_row<NC>(out, DD_F32, 0, l, per, a.C, pg);
     return;
   }
   float* acc = sh + 16;
   for (int i = 0; i < NC; ++i)
-    for (int j = 0; j < V; ++j) {
-      const int c = (l + per * i) * V + j;
+    for (int j = 0; j < 8; ++j) {
+      const int c = (l + per * i) * 8 + j;
       if (c < a.C) acc[slot * a.C + c] = pg[i][j];
     }
   __syncthreads();
@@ -200,50 +202,24 @@ __global__ void __launch_bounds__(1024) k_rms_bwd(RmsBwdArgs a, int wpr) {
   }
 }
 
-// out[c] (+)= sum over the n partial rows, in a fixed order.
-__global__ void __launch_bounds__(1024) k_part_sum(const float* parts, int n, int C, float* out, int accumulate) {
-  __shared__ float sh[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float t = 0.f;
-  if (c < C)
-    for (int i = w; i < n; i += 16) t += parts[(long)i * C + c];
-  sh[w][lane] = t;
-  __syncthreads();
-  if (w == 0 && c < C) {
-    t = sh[0][lane];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) t += sh[i][lane];
-    out[c] = accumulate ? out[c] + t : t;
-  }
-}
-
-// Waves per row and elements per lane for C columns in vectors of V; 0: too wide.
-struct Shape { int wpr, e; };
-inline Shape row_shape(int C, int V) {
+// Waves per row and vectors per lane; wpr 0: too wide.
+struct Shape { int wpr, nc; };
+inline Shape row_shape(int C) {
   for (int wpr = 1; wpr <= 16; wpr *= 4)
-    for (int e = 8; e <= 32; e *= 2)
-      if ((long)dd_ceil_div(C, V) * V <= 64L * wpr * e) return {wpr, e};
+    for (int nc = 1; nc <= 4; nc *= 2)
+      if (C <= 512 * wpr * nc) return {wpr, nc};
   return {0, 0};
 }
 
 template <bool NORM>
 int launch_fwd(const RmsArgs& a, hipStream_t st) {
-  int v = 8;
-  while (v > 1 && !(a.C % v == 0 && rows_aligned(a.x, a.ldx, a.xt, min(16, v * dtype_size(a.xt))) &&
-                    rows_aligned(a.r, a.ldr, a.rt, min(16, v * dtype_size(a.rt))) &&
-                    rows_aligned(a.s, a.lds, a.rt, min(16, v * dtype_size(a.rt))) &&
-                    rows_aligned(a.gamma, 0, DD_F32, min(16, v * 4)) &&
-                    rows_aligned(a.y, a.ldy, a.yt, min(16, v * dtype_size(a.yt)))))
-    v = v == 8 ? 2 : 1;
-  const Shape sh = row_shape(a.C, v);
+  const Shape sh = row_shape(a.C);
   DD_REQUIRE(sh.wpr > 0, "dd_rms_norm_fwd / dd_quant_rows: more than 32768 columns");
   const int threads = sh.wpr == 16 ? 1024 : 256, rpb = threads / (64 * sh.wpr);
   const dim3 grid(dd_ceil_div(a.rows, rpb));
-#define DD_RMS_FWD(V_, E_) \
-  if (v == V_ && sh.e == E_) { k_rms_fwd<V_, E_ / V_, NORM><<<grid, threads, 0, st>>>(a, sh.wpr); }
-  DD_RMS_FWD(8, 8) DD_RMS_FWD(8, 16) DD_RMS_FWD(8, 32)
-  DD_RMS_FWD(2, 8) DD_RMS_FWD(2, 16) DD_RMS_FWD(2, 32)
-  DD_RMS_FWD(1, 8) DD_RMS_FWD(1, 16) DD_RMS_FWD(1, 32)
+#define DD_RMS_FWD(N_, T_) \
+  if (sh.nc == N_ && threads == T_) { k_rms_fwd<N_, NORM, T_><<<grid, T_, 0, st>>>(a, sh.wpr); }
+  DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(4, 256) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
 #undef DD_RMS_FWD
   DD_CHECK_LAUNCH(NORM ? "dd_rms_norm_fwd" : "dd_quant_rows");
   return 0;
@@ -288,31 +264,22 @@ extern "C" int dd_rms_norm_bwd(const void* dy, long ldy, int y_type, const void*
   if (rows == 0 && (!dgamma || accumulate)) return 0;
   DD_REQUIRE(rows == 0 || (dy && s && rstd && gamma && ds), "dd_rms_norm_bwd: null pointer");
   DD_REQUIRE(rows == 0 || (ldy >= C && lds >= C && ldd >= C && (!dres || ldr >= C)), "dd_rms_norm_bwd: a leading dimension below C");
-  int v = 8;
-  while (v > 1 && !(C % v == 0 && rows_aligned(dy, ldy, y_type, min(16, v * dtype_size(y_type))) &&
-                    rows_aligned(s, lds, res_type, min(16, v * dtype_size(res_type))) &&
-                    rows_aligned(dres, ldr, res_type, min(16, v * dtype_size(res_type))) &&
-                    rows_aligned(ds, ldd, res_type, min(16, v * dtype_size(res_type))) &&
-                    rows_aligned(ws, 0, DD_F32, min(16, v * 4)) && rows_aligned(gamma, 0, DD_F32, min(16, v * 4))))
-    v = v == 8 ? 2 : 1;
-  const Shape sh = row_shape(C, v);
+  const Shape sh = row_shape(C);
   DD_REQUIRE(sh.wpr > 0, "dd_rms_norm_bwd: more than 32768 columns");
   const int threads = sh.wpr == 16 ? 1024 : 256, rpb = threads / (64 * sh.wpr);
-  const int grid = min(dd_ceil_div(rows, rpb), 1024);
+  const int grid = min(dd_ceil_div(rows, rpb), 768);   // three workgroups per CU
   DD_REQUIRE(!dgamma || ws_bytes / sizeof(float) >= (size_t)grid * C, "dd_rms_norm_bwd: the workspace is too small");
   if (grid > 0) {
     const RmsBwdArgs a{dy, ldy, y_type, s, lds, res_type, dres, ldr, ds, ldd, rstd, gamma, dgamma ? ws : nullptr, rows, C};
     const size_t lds_bytes = (16 + (sh.wpr == 1 && dgamma ? (size_t)rpb * C : 0)) * sizeof(float);
-#define DD_RMS_BWD(V_, E_) \
-  if (v == V_ && sh.e == E_) { k_rms_bwd<V_, E_ / V_><<<grid, threads, lds_bytes, st>>>(a, sh.wpr); }
-    DD_RMS_BWD(8, 8) DD_RMS_BWD(8, 16) DD_RMS_BWD(8, 32)
-    DD_RMS_BWD(2, 8) DD_RMS_BWD(2, 16) DD_RMS_BWD(2, 32)
-    DD_RMS_BWD(1, 8) DD_RMS_BWD(1, 16) DD_RMS_BWD(1, 32)
+#define DD_RMS_BWD(N_, T_) \
+  if (sh.nc == N_ && threads == T_) { k_rms_bwd<N_, T_><<<grid, T_, lds_bytes, st>>>(a, sh.wpr); }
+    DD_RMS_BWD(1, 256) DD_RMS_BWD(2, 256) DD_RMS_BWD(4, 256) DD_RMS_BWD(2, 1024) DD_RMS_BWD(4, 1024)
 #undef DD_RMS_BWD
     DD_CHECK_LAUNCH("dd_rms_norm_bwd");
   }
   if (dgamma) {
-    k_part_sum<<<dd_ceil_div(C, 64), 1024, 0, st>>>(ws, grid, C, dgamma, accumulate);
+    k_part_sum<<<dd_ceil_div(C, 32), 1024, 0, st>>>(ws, grid, C, dgamma, DD_F32, accumulate);
     DD_CHECK_LAUNCH("dd_rms_norm_bwd(dgamma)");
   }
   return 0;

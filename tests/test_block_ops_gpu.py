@@ -289,8 +289,12 @@ def test_scan(hip, ref, B, T, D, gate, cand, dt):
   # e[t] = a e[t-1] + 32 u m[t] with m the recurrence of the magnitudes.
   _, _, a, restart, g, phi = ref._scan_gates(host[0], host[1], host[2], T, first, -1.0, cand)
   a = torch.where(restart, torch.zeros_like(a), a)
+  # bf16 operands: a is 1 - z with z good to 8 u, so off by 8 u of one, and phi is 1 - 2 r with r good to
+  # 8 u, off by 16 u of one: 8 u |h[t-1]| + 16 u gate more.
+  low = 1.0 if dt == BF16 else 0.0
   m = linear_recurrence(a, (g * phi).abs() + U, h0.double().abs())
-  e = linear_recurrence(a, 32 * U * m, torch.zeros(B, D).double())
+  mp = torch.cat([h0.double().abs()[:, None], m[:, :-1]], 1)
+  e = linear_recurrence(a, 32 * U * m + low * U * (8 * mp + 16 * g), torch.zeros(B, D).double())
   within(hs.t, h, e.reshape(B * T, D), 'h')
   within(hT, T1, e[:, -1], 'hT')
   d = Slot(B * T, n * D, dt, 0, 8 if D % 8 == 0 else 1)
@@ -304,17 +308,18 @@ def test_scan(hip, ref, B, T, D, gate, cand, dt):
   ref.gated_scan_bwd(dh, host[0], host[1], hq, want[0], want[1], T, i=host[2], di=want[2] if gate else None, h0=h0, dhT=dhT, dh0=w0, **kr)
   after = torch.cat([a[:, 1:], torch.ones_like(a[:, :1])], 1).flip(1)
   mg = linear_recurrence(after, dh.double().reshape(B, T, D).abs().flip(1), dhT.double().abs())
-  eg = linear_recurrence(after, 32 * U * mg, torch.zeros(B, D).double()).flip(1)
+  mgn = torch.cat([dhT.double().abs()[:, None], mg[:, :-1]], 1)
+  eg = linear_recurrence(after, 32 * U * mg + low * 8 * U * mgn, torch.zeros(B, D).double()).flip(1)
   mg = mg.flip(1)
   eg = eg + 64 * U * mg                                                        # and the factors below
   before = torch.cat([h0.double()[:, None], hq.double().reshape(B, T, D)[:, :-1]], 1).abs() + phi.abs()
   z = torch.sigmoid(host[0].double().reshape(B, T, D) - 1.0)
-  within(outs[0], want[0], (eg * before * z * (1 - z)).reshape(B * T, D), 'du')
+  within(outs[0], want[0], (eg * before * z * (1 - z) + low * U * mg * z * (8 * before + 16)).reshape(B * T, D), 'du')
   # 1 - tanh^2 cancels: its error is 16 u of one, not of itself
-  within(outs[1], want[1], (eg * g + 16 * U * mg * g).reshape(B * T, D), 'dc')
-  if gate:
-    within(outs[2], want[2], (eg * phi.abs() * g * (1 - g) + 16 * U * mg * U).reshape(B * T, D), 'di')
-  within(dh0, w0, a[:, 0] * eg[:, 0], 'dh0')
+  within(outs[1], want[1], (eg * g + (16 + 32 * low) * U * mg * g).reshape(B * T, D), 'dc')
+  if gate:   # 1 - sigmoid(i) the same way: 8 u of one
+    within(outs[2], want[2], (eg * phi.abs() * g * (1 - g) + U * mg * g * (8 * phi.abs() + 16 * low)).reshape(B * T, D), 'di')
+  within(dh0, w0, a[:, 0] * eg[:, 0] + low * 8 * U * mg[:, 0], 'dh0')
   hs.whole(), d.whole()
 
 
@@ -384,6 +389,28 @@ def test_restart_cuts_whatever_came_before(hip, T):
   assert bool(torch.isfinite(dc[:cut]).all()) and bool(torch.isnan(dc[cut:cut + 3]).all()) and bool(torch.isfinite(dh0).all())
   hip.gated_scan_fwd(u.cuda(), c.cuda(), h, T, h0=h0.cuda(), hT=hT2)
   assert bool(torch.isnan(h).all()) and bool(torch.isnan(hT2).all())
+
+
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('T', [12, 700])
+def test_a_nan_gate_is_not_lost(hip, T, gate):
+  """A NaN in the update gate reaches every later state, and every earlier gradient, of its channel - and
+  of no other."""
+  D = 64
+  for dt in (F32, BF16):
+    u, c, i, dh = (rnd(T, D, seed=k, dtype=dt).cuda() for k in range(4))
+    at = T // 2
+    u[at, 5] = float('nan')
+    h, du, dc, di = (torch.zeros(T, D, device='cuda', dtype=dt) for _ in range(4))
+    hT, dh0 = torch.zeros(1, D, device='cuda'), torch.zeros(1, D, device='cuda')
+    kw = dict(i=i) if gate else {}
+    hip.gated_scan_fwd(u, c, h, T, hT=hT, **kw)
+    clean = [k for k in range(D) if k != 5]
+    assert bool(torch.isnan(h[at:, 5]).all()) and bool(torch.isfinite(h[:at, 5]).all()) and bool(torch.isfinite(h[:, clean]).all())
+    assert bool(torch.isnan(hT[0, 5])) and bool(torch.isfinite(hT[0, clean]).all())
+    hip.gated_scan_bwd(dh, u, c, torch.zeros_like(h), du, dc, T, dh0=dh0, **(dict(i=i, di=di) if gate else {}))
+    assert bool(torch.isnan(dc[:at, 5]).all()) and bool(torch.isfinite(dc[at + 1:, 5]).all()) and bool(torch.isnan(dh0[0, 5]))
+    assert bool(torch.isfinite(dc[:, clean]).all()) and bool(torch.isfinite(dh0[0, clean]).all())
 
 
 def test_scan_saturated_gates(hip, ref):
