@@ -23,7 +23,6 @@ struct Epi {
   __bf16* z; long ldz;
   const float* xs; const float* wsc;
   int accumulate;
-  int vec;         // 8, 2 or 1 consecutive columns are aligned for every operand above
 };
 
 __device__ __forceinline__ float act_any(int act, float z) {
@@ -35,7 +34,7 @@ __device__ __forceinline__ float act_any(int act, float z) {
   }
 }
 
-// V <= e.vec consecutive outputs of row m from column n.
+// V consecutive outputs of row m from column n (any alignment).
 template <int V>
 __device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V]) {
   if (e.xs) {
@@ -84,19 +83,29 @@ __device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V])
   }
 }
 
-// Eight columns (fewer at the end of a row) of which not all are there or aligned; v in LDS.
+// The last columns of a row, fewer than eight; v in LDS.
 __device__ __forceinline__ void finish_ragged(const Epi& e, long m, long n, long N, const float* v) {
-  if (e.vec >= 2 && n + 8 <= N) {
 #pragma unroll 1
-    for (int j = 0; j < 8; j += 2) { float t[2] = {v[j], v[j + 1]}; finish<2>(e, m, n + j, t); }
-    return;
-  }
-#pragma unroll 1
-  for (int j = 0; j < 8 && n + j < N; ++j) { float t[1] = {v[j]}; finish<1>(e, m, n + j, t); }
+  for (int j = 0; n + j < N; ++j) { float t[1] = {v[j]}; finish<1>(e, m, n + j, t); }
 }
 
 // An operand: R rows (of the output's rows or columns), contraction length K.
-struct Mat { const void* p; long ld; int R; int vec; };
+struct Mat { const void* p; long ld; int R; };
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(1)));   // 16 bytes at any address
+
+// The first n (fewer than a chunk's) elements at p, zeros behind.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <int ES>
+__device__ __forceinline__ i32x4 partial_chunk(const char* p, int n) {
+  unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16 / ES; ++j)
+    if (j < n) {
+      if constexpr (ES == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
+      else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
+    }
+  return i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+}
 
 constexpr int ROWB = 128;         // bytes of the contraction per tile row
 constexpr int LROW = ROWB + 16;   // LDS row: 16 bytes more, so that 16-byte reads of 8 rows fall on different banks
@@ -111,32 +120,21 @@ __device__ __forceinline__ void stage(const Mat& a, long r0, long k0, int K, cha
     const int ch = threadIdx.x + it * 256;
     if constexpr (!RC) {
       const int r = ch >> 3, kc = (ch & 7) * PER;
-      uint4 v = make_uint4(0, 0, 0, 0);
+      i32x4 v = {0, 0, 0, 0};
       if (r0 + r < a.R) {
         const char* p = (const char*)a.p + ((r0 + r) * a.ld + k0 + kc) * ES;
-        if (a.vec && k0 + kc + PER <= K) {
-          v = *reinterpret_cast<const uint4*>(p);
-        } else {
-          unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (k0 + kc + j < K) {
-              if constexpr (ES == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
-              else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
-            }
-          v = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        if (k0 + kc + PER <= K) __builtin_memcpy(&v, p, 16);
+        else v = partial_chunk<ES>(p, (int)(K - k0 - kc));
       }
-      *reinterpret_cast<uint4*>(sh + r * LROW + kc * ES) = v;
+      *reinterpret_cast<i32x4*>(sh + r * LROW + kc * ES) = v;
     } else {
       // 8 consecutive rows of one k, written one by one into their K-contiguous rows
       const int k = ch >> 3, rr = (ch & 7) * 8;
       unsigned short e[8] = {};
       if (k0 + k < K) {
         const unsigned short* p = (const unsigned short*)a.p + (k0 + k) * a.ld + r0 + rr;
-        if (a.vec && r0 + rr + 8 <= a.R) {
-          const uint4 v = *reinterpret_cast<const uint4*>(p);
-          *reinterpret_cast<uint4*>(e) = v;
+        if (r0 + rr + 8 <= a.R) {
+          __builtin_memcpy(e, p, 16);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -206,7 +204,7 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
       float* p = slabs + ((long)blockIdx.z * P.R + m) * Q.R + n;
       for (int j = 0; j < 8; ++j)
         if (n + j < Q.R) p[j] = v[j];
-    } else if (e.vec == 8 && n + 8 <= Q.R) {
+    } else if (n + 8 <= Q.R) {
       finish<8>(e, m, n, v);
     } else {
       finish_ragged(e, m, n, Q.R, out + mr * 68 + nc);
@@ -223,19 +221,29 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
 template <int ES, int MB>
 __global__ void __launch_bounds__(1024) k_linear_few(Mat P, Mat Q, int K, Epi e) {
   constexpr int BK = ES == 2 ? 32 : 128, UNROLL = MB <= 2 ? 4 : 2, LANE = BK / 4;   // elements of a lane's operand
-  typedef int i32x4 __attribute__((ext_vector_type(4)));
   __shared__ float sh[16][MB * 16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int row = lane & 15, kl = (lane >> 4) * LANE;
   const long n0 = (long)blockIdx.x * 16;
   f32x4 acc[MB] = {};
   const i32x4 zero = {};
-  constexpr int PER = 16 / ES;           // elements of a 16-byte load; K is a multiple of it
+  constexpr int PER = 16 / ES;           // elements of a 16-byte load
   auto load = [&](const Mat& a, long r, int k, i32x4 v[LANE / PER]) {
     const char* p = (const char*)a.p + (min(r, (long)a.R - 1) * a.ld + k) * ES;
 #pragma unroll
-    for (int j = 0; j < LANE / PER; ++j)
-      v[j] = r < a.R && k + j * PER < K ? *reinterpret_cast<const i32x4*>(p + 16 * j) : zero;
+    for (int j = 0; j < LANE / PER; ++j) {
+      v[j] = zero;
+      if (r < a.R && k + (j + 1) * PER <= K) __builtin_memcpy(&v[j], p + 16 * j, 16);
+    }
+  };
+  auto multiply = [&](const i32x4 q[LANE / PER], const i32x4 x[LANE / PER], int b) {
+    if constexpr (ES == 2) {
+      acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[0]), __builtin_bit_cast(bf16x8, x[0]), acc[b], 0, 0, 0);
+    } else {
+      const i32x8 w8 = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      const i32x8 x8 = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[b], 0, 0, 0, 127, 0, 127);
+    }
   };
   for (int k0 = wave * BK; k0 < K; k0 += waves * BK * UNROLL) {
     i32x4 q[UNROLL][LANE / PER], x[UNROLL][MB][LANE / PER];
@@ -248,15 +256,19 @@ __global__ void __launch_bounds__(1024) k_linear_few(Mat P, Mat Q, int K, Epi e)
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        if constexpr (ES == 2) {
-          acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[u][0]), __builtin_bit_cast(bf16x8, x[u][b][0]), acc[b], 0, 0, 0);
-        } else {
-          const i32x8 w8 = __builtin_shufflevector(q[u][0], q[u][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          const i32x8 x8 = __builtin_shufflevector(x[u][b][0], x[u][b][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[b], 0, 0, 0, 127, 0, 127);
-        }
-      }
+      for (int b = 0; b < MB; ++b) multiply(q[u], x[u][b], b);
+  }
+  if (K % PER != 0 && wave == 0) {       // the contraction's last elements: one more step, in the first lanes' chunk
+    const int k = K - K % PER;
+    i32x4 q[LANE / PER] = {}, x[MB][LANE / PER] = {};
+    if (lane < 16) {
+      if (n0 + row < Q.R) q[0] = partial_chunk<ES>((const char*)Q.p + ((n0 + row) * Q.ld + k) * ES, K - k);
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+        if (b * 16 + row < P.R) x[b][0] = partial_chunk<ES>((const char*)P.p + ((b * 16 + row) * P.ld + k) * ES, K - k);
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b) multiply(q, x[b], b);
   }
   // a lane holds columns 4 (lane >> 4) .. + 3 of row lane & 15
 #pragma unroll
@@ -274,7 +286,7 @@ __global__ void __launch_bounds__(1024) k_linear_few(Mat P, Mat Q, int K, Epi e)
   }
 }
 
-// Rows of any alignment and length -> rows of whole 16-byte chunks, zeros behind; units of T (4 bytes
+// Rows -> rows of whole 16-byte chunks, zeros behind; units of T (4 bytes
 // where the rows are aligned for it), `ldo` and `ldi` in units, 32 KB of a row per workgroup and pass.
 template <typename T>
 __global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int cols, T* out, int ldo) {
@@ -289,7 +301,8 @@ __global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int 
 // BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
 // contraction per step.  A step's tiles come from global memory straight into LDS (16 bytes per lane,
 // no registers in between), two stages: while the instructions of one run, the next is in flight.
-// Reads past an operand's end give zeros (buffer descriptor) - no bounds checks in the loop.
+// Reads past an operand's end give zeros (buffer descriptor) - no bounds checks in the loop; rows may
+// start at any address.
 //
 // LDS holds 16-byte chunks; which chunk of its row a slot holds is permuted by the row, on the GLOBAL
 // address of the copy (the LDS side of a copy is fixed: base + lane * 16), so that the lanes of a read
@@ -313,9 +326,8 @@ struct TileCopy {
     base = (const char*)a.p + (RC ? k0 * a.ld + r0 : r0 * a.ld + k0) * ES;
     step = RC ? BK * a.ld * ES : ROWB;
     ldb = (unsigned)(a.ld * ES);
-    // (ragged ends are zeros up to the next whole chunk: the operand was packed)
-    cols = (unsigned)((a.R - r0) * ES + 15) & ~15u;
-    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + ((unsigned)((K - k0) * ES + 15) & ~15u);
+    cols = (unsigned)((a.R - r0) * ES + 3) & ~3u;   // (an odd length was packed: zeros behind)
+    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = (i * NW + wave) * 64 + lane;
@@ -338,9 +350,9 @@ struct TileCopy {
     unsigned bytes = rest > 0 ? size : 0u;
     if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
     const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, bytes, 0x00020000u};
-    if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks past the end are
-#pragma unroll                            // moved out of the descriptor's range
-      for (int i = 0; i < N; ++i) voff[i] = col >= rest ? 0x7fffffff : voff[i];
+    if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks that are not whole are
+#pragma unroll                            // moved out of the descriptor's range (mend_tail writes the one that is cut)
+      for (int i = 0; i < N; ++i) voff[i] = col + 16 / ES > rest ? 0x7fffffff : voff[i];
     base += step;
     if (!RC) size -= ROWB;
     return rs;
@@ -355,6 +367,18 @@ struct TileCopy {
     for (int i = 0; i < N; ++i) one(rs, lds, wave, i);
   }
 };
+// The chunk in which a KC operand's contraction ends (K is no multiple of a chunk), element by element into
+// its place in the tile of the last step; `threads` threads share the rows.
+template <int ES, int R_>
+__device__ __forceinline__ void mend_tail(const Mat& a, long r0, int K, int k0, char* tile, int threads) {
+  constexpr int PER = 16 / ES;
+  const int c = (K - k0) / PER, n = (K - k0) % PER;
+  for (int r = threadIdx.x; r < R_; r += threads) {
+    i32x4 v = {0, 0, 0, 0};
+    if (r0 + r < a.R) v = partial_chunk<ES>((const char*)a.p + ((r0 + r) * a.ld + k0 + c * PER) * ES, n);
+    *reinterpret_cast<i32x4*>(tile + r * ROWB + ((c ^ ((r >> 1) & 7)) << 4)) = v;
+  }
+}
 // Every copy of this wave has landed, and then every wave's; reads issued before are complete.
 __device__ __forceinline__ void sync_copies() {
   __builtin_amdgcn_sched_barrier(0);
@@ -395,7 +419,6 @@ struct Frag<1, false, R_> {
   // (which 32 of the 64 elements a lane holds, and in which order, is free: both operands agree)
   static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
     const int row = r + (lane & 31), x = (row >> 1) & 7, c = 4 * s + 2 * (lane >> 5);
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
     const i32x4 a = *reinterpret_cast<const i32x4*>(sh + row * ROWB + ((c ^ x) << 4));
     const i32x4 b = *reinterpret_cast<const i32x4*>(sh + row * ROWB + (((c + 1) ^ x) << 4));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -451,10 +474,19 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   // groups (in one go they would hold the waves up while the address unit works through them), and are
   // waited for at the end of step t + 1.  Operands of a group are read one group ahead, across the barrier
   // too, so that the matrix unit has work while the waves meet.
+  // (a contraction that ends inside a chunk: its last step's tiles are mended once they have landed)
+  const bool cut = kend == K && K % (16 / ES) != 0 && !(P_RC && Q_RC);
+  auto mend = [&](int stage) {
+    const int k0 = (int)kb + (steps - 1) * BK;
+    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + stage, NW * 64);
+    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + stage + BM * ROWB, NW * 64);
+    sync_copies();
+  };
   cp.issue(lds, wave, rest);
   cq.issue(lds + BM * ROWB, wave, rest);
   rest -= BK;
   sync_copies();
+  if (cut && steps == 1) mend(0);
   cp.issue(lds + STAGE, wave, rest);
 #pragma unroll
   for (int k = 0; k < NT + MH; ++k) read1(0, 0, k);
@@ -462,7 +494,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
     const int here = (t & 1) * STAGE, next = STAGE - here;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      if (g + 1 == GROUPS) sync_copies();
+      if (g + 1 == GROUPS) {
+        sync_copies();
+        if (cut && t + 2 == steps) mend(next);
+      }
       typename decltype(cp)::u32x4 rs;
       if (g == GROUPS - 1) rs = cp.begin(rest);
       if (g == 0) { rs = cq.begin(rest); rest -= BK; }
@@ -500,8 +535,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
   const int nc = (lane % LPR) * 8;
   const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
-  const bool full = e.vec == 8 && n + 8 <= Q.R;
-  uint4 res[RI][2];
+  const bool full = n + 8 <= Q.R;
+  u32x4u res[RI][2];
   float xs[RI];
   auto fetch = [&](int i) {
 #pragma unroll
@@ -511,10 +546,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
       if (e.xs) xs[k] = e.xs[m];
       if (e.res) {
         if (e.ytype == DD_F32) {
-          res[k][0] = reinterpret_cast<const uint4*>((const float*)e.res + m * e.ldr + n)[0];
-          res[k][1] = reinterpret_cast<const uint4*>((const float*)e.res + m * e.ldr + n)[1];
+          res[k][0] = reinterpret_cast<const u32x4u*>((const float*)e.res + m * e.ldr + n)[0];
+          res[k][1] = reinterpret_cast<const u32x4u*>((const float*)e.res + m * e.ldr + n)[1];
         } else {
-          res[k][0] = *reinterpret_cast<const uint4*>((const __bf16*)e.res + m * e.ldr + n);
+          res[k][0] = *reinterpret_cast<const u32x4u*>((const __bf16*)e.res + m * e.ldr + n);
         }
       }
     }
@@ -543,10 +578,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
         const long m = mrow + 16 * i + RPI * k;
         const float* from = rows + RPI * k * LD;
         if (m >= P.R) continue;
-        if (Q.R % 8 == 0) {
+        if (full) {
           float v[8];
           load_f32<8>(from, v);
-          if (n < Q.R) store_f32<8>(slab + m * Q.R + n, v);
+          store_f32<8>(slab + m * Q.R + n, v);
         } else {
           for (int j = 0; j < 8 && n + j < Q.R; ++j) slab[m * Q.R + n + j] = from[j];
         }
@@ -617,27 +652,31 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   }
 }
 
-// Sum of the partial results of a split contraction, slabs ascending, and the epilogue; N % V == 0.
+// Sum of the partial results of a split contraction, slabs ascending, and the epilogue: eight columns of a
+// row per thread, element by element where the row ends inside them.
 template <int V>
-__global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, Epi e) {
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * V, MN = M * N;
-  if (i >= MN) return;
+__device__ __forceinline__ void sum_and_finish(const float* slabs, int S, long M, long N, long m, long n, const Epi& e) {
+  const long at = m * N + n;
   float v[V], t[V];
-  load_f32<V>(slabs + i, v);
+  load_f32<V>(slabs + at, v);
 #pragma unroll 4
   for (int s = 1; s < S; ++s) {
-    load_f32<V>(slabs + s * MN + i, t);
+    load_f32<V>(slabs + s * M * N + at, t);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += t[j];
   }
-  finish<V>(e, i / N, i % N, v);
+  finish<V>(e, m, n, v);
+}
+__global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, int chunks, Epi e) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, m = i / chunks, n = i % chunks * 8;
+  if (m >= M) return;
+  if (n + 8 <= N) return sum_and_finish<8>(slabs, S, M, N, m, n, e);
+#pragma unroll 1
+  for (long j = n; j < N; ++j) sum_and_finish<1>(slabs, S, M, N, m, j, e);
 }
 inline void sum_slabs(const float* slabs, int S, long M, long N, const Epi& e, hipStream_t st) {
-  const int v = e.vec == 8 && N % 8 == 0 ? 8 : e.vec >= 2 && N % 2 == 0 ? 2 : 1;
-  const unsigned grid = (unsigned)((M * N / v + 255) / 256);
-  if (v == 8) k_linear_finish<8><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
-  else if (v == 2) k_linear_finish<2><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
-  else k_linear_finish<1><<<grid, 256, 0, st>>>(slabs, S, M, N, e);
+  const int chunks = dd_ceil_div(N, 8);
+  k_linear_finish<<<(unsigned)((M * chunks + 255) / 256), 256, 0, st>>>(slabs, S, M, N, chunks, e);
 }
 
 // Splits of a contraction: none where the tiles alone fill the chip.
@@ -648,10 +687,10 @@ inline int pick_splits(long tiles, int ktiles, size_t slab_bytes, size_t ws_byte
   return (int)max(s, 1l);
 }
 
-// Can the tiled kernel's copies read this operand?  16-byte chunks: aligned rows of whole chunks along
-// the contiguous axis; offsets within a tile below 2^31.
-inline bool tileable(const Mat& a, bool rc, int K, int es) {
-  return a.vec && (rc ? a.R : K) % (16 / es) == 0 && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
+// Can the tiled kernel's copies read this operand?  Offsets within a tile stay below 2^31; a copy takes whole
+// 4-byte units up to the operand's last byte, so RC rows (which nothing mends) have an even length.
+inline bool tileable(const Mat& a, bool rc, int es) {
+  return (!rc || a.R % 2 == 0) && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
 }
 
 // The tile shapes, and what a step of 128 contraction bytes takes when `slots` of them fill the chip
@@ -702,7 +741,7 @@ int tiled(const char* who, Mat P, Mat Q, int K, int splits, const Epi& e, float*
 // already; false: no room.
 template <int ES>
 bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
-  if (tileable(a, rc, K, ES)) return true;
+  if (tileable(a, rc, ES)) return true;
   const long rows = rc ? K : a.R;
   const int cols = rc ? a.R : K, chunks = dd_ceil_div(cols, 16 / ES);
   const size_t bytes = ((size_t)rows * chunks * 16 + 255) / 256 * 256;
@@ -716,7 +755,6 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
     k_linear_pack<unsigned char><<<grid, 256, 0, st>>>((const unsigned char*)a.p, a.ld, cols, (unsigned char*)ws, chunks * 16);
   a.p = ws;
   a.ld = chunks * (16 / ES);
-  a.vec = 1;
   ws += bytes;
   room -= bytes;
   return true;
@@ -725,7 +763,7 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
 template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
   if constexpr (!P_RC && !Q_RC)
-    if (P.R <= 64 && P.vec && Q.vec && K % (16 / ES) == 0) {
+    if (P.R <= 64 && K > 0) {
       const int threads = 64 * max(4, min(16, K / (ES == 2 ? 64 : 256)));
       const unsigned grid = dd_ceil_div(Q.R, 16);
       if (P.R <= 16) k_linear_few<ES, 1><<<grid, threads, 0, st>>>(P, Q, K, e);
@@ -734,12 +772,11 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
       DD_CHECK_LAUNCH(who);
       return 0;
     }
-  // The tiled kernel, on packed copies of operands whose rows are no whole 16-byte chunks where the
-  // product is large enough to pay for the copies (2500 x 2048 x 1542: 25 us more, against 190 us for the
-  // general kernel).
+  // The tiled kernel, on packed copies of transposed operands of odd length where the product is large enough
+  // to pay for them (about 6 us an operand at 2500 x 1541, against 100 us for the general kernel).
   char* at = (char*)(((uintptr_t)ws + 255) / 256 * 256);
   size_t room = ws && ws_bytes > 512 ? ws_bytes - 256 : 0;
-  if (K > 0 && ((tileable(P, P_RC, K, ES) && tileable(Q, Q_RC, K, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
+  if (K > 0 && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
     Mat p = P, q = Q;
     if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
       const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), P_RC, room);
@@ -767,53 +804,53 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
 }
 
 // dz = dy act'(z), and the workgroup's share of dbias; without an activation dz IS dy and only the column
-// sums are taken.  HBM-bound: 64 V columns per workgroup (1 KB of a row in one wave's access), four waves on
-// different rows, four rows requested at a time.
+// sums are taken.  HBM-bound: 512 columns per workgroup (1 KB of a row in one wave's access), four waves on
+// different rows, four rows requested at a time; the columns of a ragged row's end one by one.
 template <int V, int ACT>
+__device__ __forceinline__ void act_rows(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz, long c,
+                                         long m0, long m1, float sum[V]) {
+#pragma unroll 4
+  for (long m = m0; m < m1; m += 4) {
+    float d[V], t[V];
+    load_bf16<V>(dy + m * ldy + c, d);
+    if constexpr (ACT != DD_ACT_NONE) {
+      load_bf16<V>(z + m * ldz + c, t);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] *= act_slope<ACT>(t[j]);
+      // bf16: the two products that read dz take bf16 operands
+      store_bf16<V>(dz + m * lddz + c, d);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] += d[j];
+  }
+}
+template <int ACT>
 __global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz,
                                                  float* parts, int M, int N, int rows_per) {
-  __shared__ float sh[3][64 * V];
+  __shared__ float sh[4][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long c = ((long)blockIdx.x * 64 + lane) * V;
-  const long m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
-  float sum[V] = {};
-  if (c < N)
-#pragma unroll 4
-    for (long m = (long)blockIdx.y * rows_per + wave; m < m1; m += 4) {
-      float d[V], t[V];
-      load_bf16<V>(dy + m * ldy + c, d);
-      if constexpr (ACT != DD_ACT_NONE) {
-        load_bf16<V>(z + m * ldz + c, t);
+  const long c = ((long)blockIdx.x * 64 + lane) * 8;
+  const long m0 = (long)blockIdx.y * rows_per + wave, m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
+  float sum[8] = {};
+  if (c + 8 <= N) act_rows<8, ACT>(dy, ldy, z, ldz, dz, lddz, c, m0, m1, sum);
+  else
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] *= act_slope<ACT>(t[j]);
-        // bf16: the two products that read dz take bf16 operands
-        store_bf16<V>(dz + m * lddz + c, d);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += d[j];
-    }
+    for (int j = 0; j < 8; ++j)
+      if (c + j < N) act_rows<1, ACT>(dy, ldy, z, ldz, dz, lddz, c + j, m0, m1, sum + j);
   if (!parts) return;
-  if (wave)
 #pragma unroll
-    for (int j = 0; j < V; ++j) sh[wave - 1][lane * V + j] = sum[j];
+  for (int j = 0; j < 8; ++j) sh[wave][lane * 8 + j] = sum[j];
   __syncthreads();
-  if (wave || c >= N) return;
 #pragma unroll
-  for (int w = 0; w < 3; ++w)
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] += sh[w][lane * V + j];
-  store_f32<V>(parts + (long)blockIdx.y * N + c, sum);
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const long col = (long)blockIdx.x * 512 + i;
+    if (col < N) parts[(long)blockIdx.y * N + col] = sh[0][i] + sh[1][i] + sh[2][i] + sh[3][i];
+  }
 }
 
-inline int mat_vec(const void* p, long ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
-// How many columns at a time (8, 2, 1) may be accessed in every one of the epilogue's operands?
-inline int columns_at_once(const Epi& e) {
-  for (int v = 8; v > 1; v = v == 8 ? 2 : 1) {
-    auto ok = [&](const void* p, long ld, int type) { return rows_aligned(p, ld, type, min(16, v * dtype_size(type))); };
-    if (ok(e.y, e.ldy, e.ytype) && ok(e.res, e.ldr, e.ytype) && ok(e.z, e.ldz, DD_BF16) && ok(e.bias, 0, DD_F32) &&
-        ok(e.wsc, 0, DD_F32)) return v;
-  }
-  return 1;
+inline bool in_range(int M, int N, int K) {
+  constexpr int MOST = 1 << 30;
+  return M >= 0 && N > 0 && K > 0 && M <= MOST && N <= MOST && K <= MOST;
 }
 
 }  // namespace
@@ -821,7 +858,7 @@ inline int columns_at_once(const Epi& e) {
 extern "C" int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
                              const float* w_scale, const float* bias, int act, const void* res, long ldr, void* y, long ldy,
                              int y_type, void* z, long ldz, int M, int N, int K, float* ws, size_t ws_bytes, void* stream) {
-  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_fwd: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(in_range(M, N, K), "dd_linear_fwd: M >= 0, N > 0 and K > 0 (2^30 at most) are needed");
   DD_REQUIRE(type == DD_BF16 || type == DD_E4M3, "dd_linear_fwd: x and w are bf16 or e4m3 (fp32: dd_gemm_f32)");
   DD_REQUIRE(y_type == DD_BF16 || y_type == DD_F32, "dd_linear_fwd: y is bf16 or fp32");
   DD_REQUIRE(act >= DD_ACT_NONE && act <= DD_ACT_GELU, "dd_linear_fwd: unknown activation");
@@ -830,38 +867,34 @@ extern "C" int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, i
   if (M == 0) return 0;
   DD_REQUIRE(x && w && y, "dd_linear_fwd: null x, w or y");
   DD_REQUIRE(ldx >= K && ldw >= K && ldy >= N && (!res || ldr >= N) && (!z || ldz >= N), "dd_linear_fwd: a leading dimension is too small");
-  const int es = dtype_size(type);
-  const Mat P{x, ldx, M, mat_vec(x, ldx, es)}, Q{w, ldw, N, mat_vec(w, ldw, es)};
-  Epi e{y, ldy, y_type, bias, act, res, ldr, (__bf16*)z, ldz, x_scale, w_scale, 0, 0};
-  e.vec = columns_at_once(e);
+  const Mat P{x, ldx, M}, Q{w, ldw, N};
+  Epi e{y, ldy, y_type, bias, act, res, ldr, (__bf16*)z, ldz, x_scale, w_scale, 0};
   if (type == DD_BF16) return product<2, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
   return product<1, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int dd_linear_bwd_data(const void* dz, long lddz, const void* w, long ldw, void* dx, long lddx, int x_type, int M,
                                   int N, int K, float* ws, size_t ws_bytes, void* stream) {
-  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_bwd_data: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(in_range(M, N, K), "dd_linear_bwd_data: M >= 0, N > 0 and K > 0 (2^30 at most) are needed");
   DD_REQUIRE(x_type == DD_BF16 || x_type == DD_F32, "dd_linear_bwd_data: dx is bf16 or fp32");
   if (M == 0) return 0;
   DD_REQUIRE(dz && w && dx, "dd_linear_bwd_data: null pointer");
   DD_REQUIRE(lddz >= N && ldw >= K && lddx >= K, "dd_linear_bwd_data: a leading dimension is too small");
-  const Mat P{dz, lddz, M, mat_vec(dz, lddz, 2)}, Q{w, ldw, K, mat_vec(w, ldw, 2)};
+  const Mat P{dz, lddz, M}, Q{w, ldw, K};
   Epi e{dx, lddx, x_type};
-  e.vec = columns_at_once(e);
   return product<2, false, true>("dd_linear_bwd_data", P, Q, N, e, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int dd_linear_bwd_weight(const void* dz, long lddz, const void* x, long ldx, void* dw, long lddw, int w_type,
                                     int accumulate, int M, int N, int K, float* ws, size_t ws_bytes, void* stream) {
-  DD_REQUIRE(M >= 0 && N > 0 && K > 0, "dd_linear_bwd_weight: M >= 0, N > 0 and K > 0 are needed");
+  DD_REQUIRE(in_range(M, N, K), "dd_linear_bwd_weight: M >= 0, N > 0 and K > 0 (2^30 at most) are needed");
   DD_REQUIRE(w_type == DD_BF16 || w_type == DD_F32, "dd_linear_bwd_weight: dw is bf16 or fp32");
   if (M == 0 && accumulate) return 0;
   DD_REQUIRE(dw && (M == 0 || (dz && x)), "dd_linear_bwd_weight: null pointer");
   DD_REQUIRE(lddw >= K && (M == 0 || (lddz >= N && ldx >= K)), "dd_linear_bwd_weight: a leading dimension is too small");
-  const Mat P{dz, lddz, N, mat_vec(dz, lddz, 2)}, Q{x, ldx, K, mat_vec(x, ldx, 2)};
+  const Mat P{dz, lddz, N}, Q{x, ldx, K};
   Epi e{dw, lddw, w_type};
   e.accumulate = accumulate;
-  e.vec = columns_at_once(e);
   return product<2, true, true>("dd_linear_bwd_weight", P, Q, M, e, ws, ws_bytes, (hipStream_t)stream);
 }
 
@@ -876,21 +909,19 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
   DD_REQUIRE(M == 0 || (dy && ldy >= N), "dd_linear_act_bwd: dy is null or its leading dimension is below N");
   DD_REQUIRE(M == 0 || !act_on || (z && dz && ldz >= N && lddz >= N), "dd_linear_act_bwd: an activation needs z and dz");
   const hipStream_t st = (hipStream_t)stream;
-  const bool vec = N % 8 == 0 && rows_aligned(dy, ldy, DD_BF16, 16) && rows_aligned(ws, 0, DD_F32, 16) &&
-                   (!act_on || (rows_aligned(z, ldz, DD_BF16, 16) && rows_aligned(dz, lddz, DD_BF16, 16)));
   // 1024 workgroups, at least four rows each
-  const int cols = dd_ceil_div(N, vec ? 512 : 64);
+  const int cols = dd_ceil_div(N, 512);
   const int rows_per = max(4, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
   DD_REQUIRE(n <= 65535, "dd_linear_act_bwd: too many rows");
   DD_REQUIRE(!dbias || ws_bytes / sizeof(float) >= (size_t)n * N, "dd_linear_act_bwd: the workspace is too small");
   if (M > 0) {
     const dim3 grid(cols, n);
-#define DD_ACT_BWD(V_, A_)                                                                                              \
-  if (vec == (V_ == 8) && act == A_)                                                                                    \
-    k_act_bwd<V_, A_><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz,           \
-                                            dbias ? ws : nullptr, M, N, rows_per);
-    DD_ACT_BWD(8, DD_ACT_NONE) DD_ACT_BWD(8, DD_ACT_ELU) DD_ACT_BWD(8, DD_ACT_SILU) DD_ACT_BWD(8, DD_ACT_GELU)
-    DD_ACT_BWD(1, DD_ACT_NONE) DD_ACT_BWD(1, DD_ACT_ELU) DD_ACT_BWD(1, DD_ACT_SILU) DD_ACT_BWD(1, DD_ACT_GELU)
+#define DD_ACT_BWD(A_)                                                                                          \
+  case A_:                                                                                                      \
+    k_act_bwd<A_><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz,       \
+                                        dbias ? ws : nullptr, M, N, rows_per);                                  \
+    break;
+    switch (act) { DD_ACT_BWD(DD_ACT_NONE) DD_ACT_BWD(DD_ACT_ELU) DD_ACT_BWD(DD_ACT_SILU) DD_ACT_BWD(DD_ACT_GELU) }
 #undef DD_ACT_BWD
     DD_CHECK_LAUNCH("dd_linear_act_bwd");
   }

@@ -144,7 +144,7 @@ def test_norm_rows_do_not_mix(hip):
 
 # ---- product --------------------------------------------------------------------------------------
 
-LINEAR_SHAPES = [(1300, 1030, 520), (2500, 520, 1542), (130, 2048, 1544), (5000, 1024, 72), (257, 129, 8200), (1, 1, 1), (1, 64, 512), (3, 5, 7), (8, 2048, 1024), (17, 130, 40), (33, 96, 1542), (64, 64, 64), (65, 65, 65),
+LINEAR_SHAPES = [(1300, 301, 1031), (20, 70, 1031), (50, 40, 4100), (1300, 1030, 520), (2500, 520, 1542), (130, 2048, 1544), (5000, 1024, 72), (257, 129, 8200), (1, 1, 1), (1, 64, 512), (3, 5, 7), (8, 2048, 1024), (17, 130, 40), (33, 96, 1542), (64, 64, 64), (65, 65, 65),
                  (100, 256, 4096), (129, 515, 72), (300, 200, 1030), (257, 1024, 512), (1000, 384, 640)]
 
 
@@ -205,7 +205,7 @@ def test_linear_gradients(hip, ref, M, N, K, act, pt):
   within(dw.t, 2 * before.cpu().double(), dot_error(gq.t(), x.t(), M) * 2 + HALF[pt] * 4 * before.cpu().double().abs(), 'accumulate')
 
 
-@pytest.mark.parametrize('M,N,K', [(1, 16, 16), (5, 7, 9), (32, 1024, 4096), (16, 48, 128), (65, 130, 200), (300, 257, 1030), (700, 512, 256), (2100, 1040, 1030), (3000, 1000, 528)])
+@pytest.mark.parametrize('M,N,K', [(1, 16, 16), (5, 7, 9), (32, 1024, 4096), (16, 48, 128), (65, 130, 200), (300, 257, 1030), (700, 512, 256), (2100, 1040, 1030), (3000, 1000, 528), (700, 300, 4111), (20, 33, 515)])
 @pytest.mark.parametrize('act', [None, 'gelu'])
 def test_linear_e4m3(hip, ref, M, N, K, act):
   x, w = rnd(M, K, seed=1, scale=60.0).clamp(-448, 448).to(FP8), rnd(N, K, seed=2, scale=60.0).clamp(-448, 448).to(FP8)
