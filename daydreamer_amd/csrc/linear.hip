@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int 
 //
 // BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
 // contraction per step.  A step's tiles come from global memory straight into LDS (16 bytes per lane,
-// no registers in between), two stages: while the instructions of one run, the next is in flight.
+// no registers in between), two steps ahead for P (three tiles of it), one for Q (two): 160 KB at
+// 256 x 256, the whole LDS, 80 KB and two workgroups per CU at 128 x 128.
 // Reads past an operand's end give zeros (buffer descriptor) - no bounds checks in the loop; rows may
 // start at any address.
 //
@@ -379,10 +380,13 @@ __device__ __forceinline__ void mend_tail(const Mat& a, long r0, int K, int k0, 
     *reinterpret_cast<i32x4*>(tile + r * ROWB + ((c ^ ((r >> 1) & 7)) << 4)) = v;
   }
 }
-// Every copy of this wave has landed, and then every wave's; reads issued before are complete.
+// Every copy of this wave but the LATER newest has landed, and then every wave's; reads issued before are
+// complete.
+template <int LATER = 0>
 __device__ __forceinline__ void sync_copies() {
+  static_assert(LATER < 16, "");
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt 0, lgkmcnt 0
+  __builtin_amdgcn_s_waitcnt(0x0070 | LATER);   // vmcnt LATER, lgkmcnt 0
   asm volatile("s_barrier" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
@@ -431,9 +435,9 @@ __device__ __forceinline__ f32x16 mma(i32x8 q, i32x8 p, f32x16 c) {
 
 template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
-  constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, STAGE = (BM + BN) * ROWB;
+  constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, UP = BM * ROWB, UQ = BN * ROWB;
   constexpr int STEPS = ES == 2 ? 4 : 2, BK = ROWB / ES;
-  __shared__ __attribute__((aligned(1024))) char sh[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char sh[3 * UP + 2 * UQ];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles, four
   // columns wide, so that its L2 serves the rows and weights that its 32 running tiles share
@@ -455,57 +459,57 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   cq.init(Q, n0, kb, K, wave, lane);
   const unsigned lds = (unsigned)(uintptr_t)(DD_LDS char*)sh;
   f32x16 acc[MT][NT] = {};
-  int rest = kend - (int)kb;   // of the step that is copied next
+  int rest_p = kend - (int)kb, rest_q = rest_p;   // of the step that is copied next
   // A group: one contraction step of the instruction, all of the wave's rows (e4m3: half of them, its
   // operands are twice as large).  Two register sets.
   constexpr int H = ES == 2 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
   typename Frag<ES, P_RC, BM>::T p[2][MH];
   typename Frag<ES, Q_RC, BN>::T q[2][NT];
   // one of a group's NT + MH operands
-  auto read1 = [&](int stage, int g, int k) {
-    const char* a = sh + stage;
+  auto read1 = [&](int at_p, int at_q, int g, int k) {
     if (k < NT) {
-      if (g % H == 0) q[(g / H) & 1][k] = Frag<ES, Q_RC, BN>::read(a + BM * ROWB, wn + 32 * k, g / H, lane);
+      if (g % H == 0) q[(g / H) & 1][k] = Frag<ES, Q_RC, BN>::read(sh + at_q, wn + 32 * k, g / H, lane);
     } else {
-      p[g & 1][k - NT] = Frag<ES, P_RC, BM>::read(a, wm + 32 * (k - NT + (g % H) * MH), g / H, lane);
+      p[g & 1][k - NT] = Frag<ES, P_RC, BM>::read(sh + at_p, wm + 32 * (k - NT + (g % H) * MH), g / H, lane);
     }
   };
-  // Step t + 2's copies are issued as soon as step t's stage is free, behind the instructions of two
-  // groups (in one go they would hold the waves up while the address unit works through them), and are
-  // waited for at the end of step t + 1.  Operands of a group are read one group ahead, across the barrier
-  // too, so that the matrix unit has work while the waves meet.
+  // The waves meet once a step, before its last group: step t + 1 has landed, step t's tiles are free but for
+  // the last group's operands, which are in registers.  Behind the instructions of that group and of the
+  // next one the copies of Q (step t + 2) and P (t + 3) are issued - a few behind each row of instructions: in
+  // one go they would hold the waves up while the address unit works through them.  Operands are read one
+  // group ahead, across the barrier too, so that the matrix unit has work while the waves meet.
   // (a contraction that ends inside a chunk: its last step's tiles are mended once they have landed)
   const bool cut = kend == K && K % (16 / ES) != 0 && !(P_RC && Q_RC);
-  auto mend = [&](int stage) {
+  auto mend = [&](int at_p, int at_q) {
     const int k0 = (int)kb + (steps - 1) * BK;
-    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + stage, NW * 64);
-    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + stage + BM * ROWB, NW * 64);
+    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + at_p, NW * 64);
+    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + at_q, NW * 64);
     sync_copies();
   };
-  cp.issue(lds, wave, rest);
-  cq.issue(lds + BM * ROWB, wave, rest);
-  rest -= BK;
-  sync_copies();
-  if (cut && steps == 1) mend(0);
-  cp.issue(lds + STAGE, wave, rest);
+  int p0 = 0, p1 = UP, p2 = 2 * UP, q0 = 3 * UP, q1 = 3 * UP + UQ;
+  cp.issue(lds + p0, wave, rest_p); rest_p -= BK;
+  cq.issue(lds + q0, wave, rest_q); rest_q -= BK;
+  cp.issue(lds + p1, wave, rest_p); rest_p -= BK;
+  sync_copies<TileCopy<ES, P_RC, BM, NW>::N>();
+  if (cut && steps == 1) mend(p0, q0);
+  cq.issue(lds + q1, wave, rest_q); rest_q -= BK;
 #pragma unroll
-  for (int k = 0; k < NT + MH; ++k) read1(0, 0, k);
+  for (int k = 0; k < NT + MH; ++k) read1(p0, q0, 0, k);
   for (int t = 0; t < steps; ++t) {
-    const int here = (t & 1) * STAGE, next = STAGE - here;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (g + 1 == GROUPS) {
-        sync_copies();
-        if (cut && t + 2 == steps) mend(next);
+        sync_copies<TileCopy<ES, P_RC, BM, NW>::N>();
+        if (cut && t + 2 == steps) mend(p1, q1);
       }
       typename decltype(cp)::u32x4 rs;
-      if (g == GROUPS - 1) rs = cp.begin(rest);
-      if (g == 0) { rs = cq.begin(rest); rest -= BK; }
+      if (g == GROUPS - 1) { rs = cq.begin(rest_q); rest_q -= BK; }
+      if (g == 0) { rs = cp.begin(rest_p); rest_p -= BK; }
 #pragma unroll
       for (int i = 0; i < MH; ++i) {
 #pragma unroll
         for (int k = i * (NT + MH) / MH; k < (i + 1) * (NT + MH) / MH; ++k)
-          read1(g + 1 < GROUPS ? here : next, g + 1 < GROUPS ? g + 1 : 0, k);
+          read1(g + 1 < GROUPS ? p0 : p1, g + 1 < GROUPS ? q0 : q1, g + 1 < GROUPS ? g + 1 : 0, k);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -513,13 +517,16 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < cp.N; ++k)
-          if (g == GROUPS - 1 && k >= i * cp.N / MH && k < (i + 1) * cp.N / MH) cp.one(rs, lds + here, wave, k);
+          if (g == 0 && k >= i * cp.N / MH && k < (i + 1) * cp.N / MH) cp.one(rs, lds + p2, wave, k);
 #pragma unroll
         for (int k = 0; k < cq.N; ++k)
-          if (g == 0 && k >= i * cq.N / MH && k < (i + 1) * cq.N / MH) cq.one(rs, lds + next + BM * ROWB, wave, k);
+          if (g == GROUPS - 1 && k >= i * cq.N / MH && k < (i + 1) * cq.N / MH) cq.one(rs, lds + q0, wave, k);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    const int tp = p0, tq = q0;
+    p0 = p1; p1 = p2; p2 = tp;
+    q0 = q1; q1 = tq;
   }
   sync_copies();
 
@@ -530,7 +537,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   // accumulators move down - because copies of three activations would not fit the instruction cache.
   constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI;
   static_assert(RI * RPI == 16, "a half is whole rows of every lane");
-  static_assert(NW * 32 * LD * 4 <= 2 * STAGE, "the epilogue's LDS");
+  static_assert(NW * 32 * LD * 4 <= 3 * UP + 2 * UQ, "the epilogue's LDS");
   float* out = reinterpret_cast<float*>(sh) + wave * 32 * LD;
   float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
   const int nc = (lane % LPR) * 8;
@@ -693,27 +700,26 @@ inline bool tileable(const Mat& a, bool rc, int es) {
   return (!rc || a.R % 2 == 0) && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
 }
 
-// The tile shapes, and what a step of 128 contraction bytes takes when `slots` of them fill the chip
-// (microseconds, measured at 8192^3, 37500 x 1024 x 2048 and 2500 x 2048 x 1536) and beside that a tile's start and
-// epilogue.  256 x 256 is the fastest per output (1340 TFLOP/s, bf16); the small ones waste less where a
-// few tiles are left over for a last round.
-struct TileShape { int bm, bn, slots; float step, rest; };
-constexpr TileShape SHAPES[] = {{256, 256, 256, 1.6f, 7.f}, {128, 128, 512, 1.1f, 4.f}, {64, 128, 768, 0.8f, 3.f}};
-constexpr int N_SHAPES = 3;
+// The two tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and
+// the rest of a tile (start, epilogue) take then, in microseconds (measured: 256 x 256 at 8192^3 and 37500 x
+// 1024 x 2048, 128 x 128 at 37500 x 1024 x 2048).  The large one is faster per output (1390 against 1140
+// TFLOP/s, bf16, 8192^3); the small one fills the chip with fewer rows and wastes less in a last round
+// (2500 x 2048 x 1536: 25 against 36 us).
+struct TileShape { int side, slots; float step, rest; };
+constexpr TileShape SHAPES[] = {{256, 256, 1.48f, 10.f}, {128, 512, 0.96f, 4.5f}};
 
 struct Plan { int shape, splits; float us; };
-inline Plan plan_product(long M, long N, int ksteps, bool rc_rows, size_t slab_room) {
+inline Plan plan_product(long M, long N, int ksteps, size_t slab_room) {
   Plan best{0, 1, 1e30f};
-  for (int i = 0; i < N_SHAPES; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const TileShape& t = SHAPES[i];
-    if (rc_rows && t.bm % 128) continue;   // (the transposed tile's chunk permutation wants 16 chunks a row)
-    const long tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const long tiles = ((M + t.side - 1) / t.side) * ((N + t.side - 1) / t.side);
     for (int s = 1; s <= 16 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
       if (s > 1 && sizeof(float) * (size_t)(M * N) * s > slab_room) break;
       const long wgs = tiles * s, full = wgs / t.slots, left = wgs % t.slots;
       const float steps = (float)((ksteps + s - 1) / s);
-      // a last round with one tile per CU or less has the CU's paths to itself
-      const float last = left == 0 ? 0.f : (left <= 256 && t.slots > 256 ? 0.65f * t.step * steps + t.rest : t.step * steps + t.rest);
+      // a last round with a CU to itself is faster per step
+      const float last = left == 0 ? 0.f : t.rest + steps * t.step * (left <= t.slots / 2 && t.slots > 256 ? 0.65f : 1.f);
       float us = full * (t.step * steps + t.rest) + last;
       if (s > 1) us += 6.f + (float)(M * N) * s * 8.f / 3.5e6f;   // partial sums out and in, one more launch
       if (us < best.us) best = {i, s, us};
@@ -779,13 +785,9 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   if (K > 0 && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
     Mat p = P, q = Q;
     if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
-      const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), P_RC, room);
-      switch (plan.shape) {
-        case 0: return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
-        case 1: return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, p, q, K, plan.splits, e, (float*)at, st);
-        default:
-          if constexpr (!P_RC) return tiled<ES, P_RC, Q_RC, 64, 128, 1, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
-      }
+      const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), room);
+      if (plan.shape == 0) return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
+      return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, p, q, K, plan.splits, e, (float*)at, st);
     }
   }
   const int bk = ROWB / ES;
