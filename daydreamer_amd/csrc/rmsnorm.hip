@@ -8,9 +8,12 @@
 // derivative of what the forward pass computed; all arithmetic is fp32.
 //
 // Bound: HBM.  A row's elements stay in registers from their load to the last store - each input is
-// read once, each output written once - so a row belongs to one wave (C <= 2048), four (<= 8192) or
-// sixteen (<= 32768), 8 / 16 / 32 elements per lane in vectors of eight (the last one of a ragged row
-// element by element).
+// read once, each output written once - so a row belongs to one wave (C <= 1024), four (<= 4096) or
+// sixteen (<= 32768), 8 or 16 elements per lane (32 past 16384) in vectors of eight: with 32 in a lane of
+// fewer waves too few fit a CU (backward, 20001 x 1542: 101 us).  The last vector of a ragged row
+// ends at the row's end and so overlaps the one before it: both lanes hold and store the same values there,
+// the sums over a row count them once.  (Element by element, its loads came one round trip after the other:
+// 20001 x 1542 bf16, backward, 141 us; now 63, at the 52 of its bytes.)
 #include "block_core.h"
 
 namespace {
@@ -25,36 +28,39 @@ struct RmsArgs {
   int rows, C; float eps;
 };
 
-// Elements c = (l + stride i) 8 .. + 7 of a row as floats, zeros past C; added to v, or written to it.
-template <int NC, bool ADD>
-__device__ __forceinline__ void load_row(const void* base, int type, long off, int l, int stride, int C, float v[NC][8]) {
-  if (type == DD_F32) {
-    const float* p = (const float*)base + off;
+// Where vector i of lane l starts in a row of C, and how many of its elements belong to the vector before;
+// `on`: there is such a vector.  Rows shorter than a vector are read element by element.
+struct Place { int at, dup; bool on; };
+__device__ __forceinline__ Place place(int i, int l, int stride, int C) {
+  const int c = (l + stride * i) * 8;
+  const int over = C >= 8 ? max(0, c + 8 - C) : 0;
+  return {c - over, over, c < C};
+}
+
+template <typename T, int NC>
+__device__ __forceinline__ void load_as(const T* p, int l, int stride, int C, float v[NC][8]) {
+  if (C >= 8) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (l + stride * i) * 8;
-      float t[8] = {};
-      if (c + 8 <= C) load_f32<8>(p + c, t);
-      else
+      const Place q = place(i, l, stride, C);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (c + j < C) t[j] = p[c + j];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      if (q.on) {
+        if constexpr (sizeof(T) == 4) load_f32<8>(p + q.at, v[i]);
+        else load_bf16<8>(p + q.at, v[i]);
+      }
     }
   } else {
-    const __bf16* p = (const __bf16*)base + off;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = (l + stride * i) * 8;
-      float t[8] = {};
-      if (c + 8 <= C) load_bf16<8>(p + c, t);
-      else
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (c + j < C) t[j] = (float)p[c + j];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = ADD ? v[i][j] + t[j] : t[j];
-    }
+      for (int j = 0; j < 8; ++j) v[i][j] = i == 0 && l == 0 && j < C ? (float)p[j] : 0.f;
   }
+}
+template <int NC>
+__device__ __forceinline__ void load_row(const void* base, int type, long off, int l, int stride, int C, float v[NC][8]) {
+  if (type == DD_F32) load_as<float, NC>((const float*)base + off, l, stride, C, v);
+  else load_as<__bf16, NC>((const __bf16*)base + off, l, stride, C, v);
 }
 
 template <int V>
@@ -67,11 +73,11 @@ template <int NC>
 __device__ __forceinline__ void store_row(void* base, int type, long off, int l, int stride, int C, const float v[NC][8]) {
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int c = (l + stride * i) * 8;
-    if (c + 8 <= C) store_as<8>(base, type, off + c, v[i]);
+    const Place q = place(i, l, stride, C);
+    if (!q.on) continue;
+    if (C >= 8) store_as<8>(base, type, off + q.at, v[i]);
     else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) if (c + j < C) store_as<1>(base, type, off + c + j, &v[i][j]);
+      for (int j = 0; j < C; ++j) store_as<1>(base, type, off + j, &v[i][j]);
   }
 }
 
@@ -80,6 +86,8 @@ template <bool MAX>
 __device__ __forceinline__ float row_reduce(float v, int wpr, float* red) {
   v = MAX ? wave_max(v) : wave_sum(v);
   if (wpr == 1) return v;
+  // What this wave read is in registers before another wave stores it (s over res: vectors overlap).
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();   // the previous reduction's values have been read
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -94,30 +102,36 @@ __global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int wpr) {
   const int per = 64 * wpr, l = threadIdx.x % per;
   const long row = (long)blockIdx.x * (blockDim.x / per) + threadIdx.x / per;
   if (row >= a.rows) return;   // whole waves; with wpr > 1 a workgroup holds one row and never leaves
-  float v[NC][8];
-  load_row<NC, false>(a.x, a.xt, row * a.ldx, l, per, a.C, v);
-  if (a.r) load_row<NC, true>(a.r, a.rt, row * a.ldr, l, per, a.C, v);
-  if (a.s) {
-    if (a.rt == DD_BF16)
+  float v[NC][8], t[NC][8];
+  load_row<NC>(a.x, a.xt, row * a.ldx, l, per, a.C, v);
+  if (a.r) {
+    load_row<NC>(a.r, a.rt, row * a.ldr, l, per, a.C, t);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] += t[i][j];
+  }
+  if constexpr (NORM) {
+    if (a.s && a.rt == DD_BF16)
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = (float)(__bf16)v[i][j];
-    store_row<NC>(a.s, a.rt, row * a.lds, l, per, a.C, v);
-  }
-  if constexpr (NORM) {
-    float g[NC][8], ss = 0.f;
-    load_row<NC, false>(a.gamma, DD_F32, 0, l, per, a.C, g);
+    float ss = 0.f;
+    load_row<NC>(a.gamma, DD_F32, 0, l, per, a.C, t);
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+    for (int i = 0; i < NC; ++i) {
+      const int dup = place(i, l, per, a.C).dup;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+      for (int j = 0; j < 8; ++j) ss += j >= dup ? v[i][j] * v[i][j] : 0.f;
+    }
     const float rstd = 1.0f / sqrtf(row_reduce<false>(ss, wpr, red) / (float)a.C + a.eps);
+    if (a.s) store_row<NC>(a.s, a.rt, row * a.lds, l, per, a.C, v);
     if (a.rstd && l == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * g[i][j];
+      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * t[i][j];
   }
   if (a.yt == DD_E4M3) {
     float m = 0.f;
@@ -154,27 +168,29 @@ struct RmsBwdArgs {
 // A workgroup strides over the rows; every lane keeps its columns' share of dgamma in registers, the
 // four waves of a workgroup are added in LDS, one partial row per workgroup goes to the workspace.
 template <int NC, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_bwd(RmsBwdArgs a, int wpr) {
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 4 : NC == 1 ? 6 : 4) k_rms_bwd(RmsBwdArgs a, int wpr) {
   extern __shared__ float sh[];   // 16 reduction slots | (wpr == 1) [4][C] partial sums
   const int per = 64 * wpr, l = threadIdx.x % per, rpb = blockDim.x / per, slot = threadIdx.x / per;
   float g[NC][8], pg[NC][8] = {};
-  load_row<NC, false>(a.gamma, DD_F32, 0, l, per, a.C, g);
+  load_row<NC>(a.gamma, DD_F32, 0, l, per, a.C, g);
   for (long row = (long)blockIdx.x * rpb + slot; row < a.rows; row += (long)gridDim.x * rpb) {
     float dy[NC][8], n[NC][8], dr[NC][8] = {};
-    load_row<NC, false>(a.dy, a.yt, row * a.ldy, l, per, a.C, dy);
-    load_row<NC, false>(a.s, a.rt, row * a.lds, l, per, a.C, n);
-    if (a.dres) load_row<NC, false>(a.dres, a.rt, row * a.ldr, l, per, a.C, dr);
+    load_row<NC>(a.dy, a.yt, row * a.ldy, l, per, a.C, dy);
+    load_row<NC>(a.s, a.rt, row * a.lds, l, per, a.C, n);
+    if (a.dres) load_row<NC>(a.dres, a.rt, row * a.ldr, l, per, a.C, dr);
     const float rstd = a.rstd[row];
     float s1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+    for (int i = 0; i < NC; ++i) {
+      const int dup = place(i, l, per, a.C).dup;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         n[i][j] *= rstd;
         pg[i][j] += dy[i][j] * n[i][j];
         dy[i][j] *= g[i][j];
-        s1 += dy[i][j] * n[i][j];
+        s1 += j >= dup ? dy[i][j] * n[i][j] : 0.f;
       }
+    }
     s1 = row_reduce<false>(s1, wpr, sh) / (float)a.C;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -189,11 +205,13 @@ __global__ void __launch_bounds__(THREADS) k_rms_bwd(RmsBwdArgs a, int wpr) {
     return;
   }
   float* acc = sh + 16;
-  for (int i = 0; i < NC; ++i)
-    for (int j = 0; j < 8; ++j) {
-      const int c = (l + per * i) * 8 + j;
-      if (c < a.C) acc[slot * a.C + c] = pg[i][j];
-    }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const Place q = place(i, l, per, a.C);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (q.on && q.at + j < a.C) acc[slot * a.C + q.at + j] = pg[i][j];
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
     float t = acc[c];
@@ -206,7 +224,7 @@ __global__ void __launch_bounds__(THREADS) k_rms_bwd(RmsBwdArgs a, int wpr) {
 struct Shape { int wpr, nc; };
 inline Shape row_shape(int C) {
   for (int wpr = 1; wpr <= 16; wpr *= 4)
-    for (int nc = 1; nc <= 4; nc *= 2)
+    for (int nc = 1; nc <= (wpr == 16 ? 4 : 2); nc *= 2)
       if (C <= 512 * wpr * nc) return {wpr, nc};
   return {0, 0};
 }
@@ -219,7 +237,7 @@ int launch_fwd(const RmsArgs& a, hipStream_t st) {
   const dim3 grid(dd_ceil_div(a.rows, rpb));
 #define DD_RMS_FWD(N_, T_) \
   if (sh.nc == N_ && threads == T_) { k_rms_fwd<N_, NORM, T_><<<grid, T_, 0, st>>>(a, sh.wpr); }
-  DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(4, 256) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
+  DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(1, 1024) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
 #undef DD_RMS_FWD
   DD_CHECK_LAUNCH(NORM ? "dd_rms_norm_fwd" : "dd_quant_rows");
   return 0;
@@ -267,14 +285,16 @@ extern "C" int dd_rms_norm_bwd(const void* dy, long ldy, int y_type, const void*
   const Shape sh = row_shape(C);
   DD_REQUIRE(sh.wpr > 0, "dd_rms_norm_bwd: more than 32768 columns");
   const int threads = sh.wpr == 16 ? 1024 : 256, rpb = threads / (64 * sh.wpr);
-  const int grid = min(dd_ceil_div(rows, rpb), 768);   // three workgroups per CU
+  // as many workgroups as are resident at once (more leave a ragged last round: 20001 x 1542 with 768, 1024,
+  // 1536 workgroups 90, 76, 63 us; 20000 x 1024, two vectors a lane, 59, 60, 66)
+  const int grid = min(dd_ceil_div(rows, rpb), threads == 1024 ? 256 : sh.nc == 1 ? 1536 : 768);
   DD_REQUIRE(!dgamma || ws_bytes / sizeof(float) >= (size_t)grid * C, "dd_rms_norm_bwd: the workspace is too small");
   if (grid > 0) {
     const RmsBwdArgs a{dy, ldy, y_type, s, lds, res_type, dres, ldr, ds, ldd, rstd, gamma, dgamma ? ws : nullptr, rows, C};
     const size_t lds_bytes = (16 + (sh.wpr == 1 && dgamma ? (size_t)rpb * C : 0)) * sizeof(float);
 #define DD_RMS_BWD(N_, T_) \
   if (sh.nc == N_ && threads == T_) { k_rms_bwd<N_, T_><<<grid, T_, lds_bytes, st>>>(a, sh.wpr); }
-    DD_RMS_BWD(1, 256) DD_RMS_BWD(2, 256) DD_RMS_BWD(4, 256) DD_RMS_BWD(2, 1024) DD_RMS_BWD(4, 1024)
+    DD_RMS_BWD(1, 256) DD_RMS_BWD(2, 256) DD_RMS_BWD(1, 1024) DD_RMS_BWD(2, 1024) DD_RMS_BWD(4, 1024)
 #undef DD_RMS_BWD
     DD_CHECK_LAUNCH("dd_rms_norm_bwd");
   }

@@ -57,7 +57,7 @@ def within(out, want, tol, what=''):
 
 # ---- norm -----------------------------------------------------------------------------------------
 
-NORM_SHAPES = [(1, 1), (3, 7), (8, 64), (5, 1542), (130, 1024), (257, 512), (6, 2050), (2, 8192), (3, 9001), (1, 32768)]
+NORM_SHAPES = [(4, 8), (3, 9), (700, 1542), (2, 515), (3, 1025), (2, 4097), (1, 16390), (1, 1), (3, 7), (8, 64), (5, 1542), (130, 1024), (257, 512), (6, 2050), (2, 8192), (3, 9001), (1, 32768)]
 
 
 @pytest.mark.parametrize('rows,C', NORM_SHAPES)
