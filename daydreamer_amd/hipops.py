@@ -16,6 +16,7 @@ import torch
 
 _LIB_PATH = pathlib.Path(__file__).parent / 'libdaydreamer_hip.so'
 _lib = None
+_block = None
 
 c_f = ctypes.c_float
 c_d = ctypes.c_double
@@ -149,6 +150,13 @@ def load_library():
   if lib.dd_version() != ABI_VERSION:   # a stale build: signatures below may not match
     raise RuntimeError(f'{_LIB_PATH} has ABI version {lib.dd_version()}, this binding needs '
                        f'{ABI_VERSION}: rebuild it (make -C daydreamer_amd/csrc)')
+  global _block
+  try:   # native binding of the residual recurrent block (csrc/block_bind.cpp)
+    from . import _block
+  except ImportError as e:
+    raise RuntimeError(f'daydreamer_amd/_block.so not found or not loadable ({e}): build it with '
+                       f'__graft_entry__.build() (make -C daydreamer_amd/csrc).') from e
+  _block.bind(lib._handle)
   _lib = lib
   return lib
 
@@ -169,12 +177,6 @@ def _vec(t):
   """(ptr, stride) of a 1-D view."""
   assert t.dim() == 1, t.shape
   return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else 1)
-
-
-# storage types and activations of the residual recurrent block (include/daydreamer_hip.h)
-_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
-_REAL = (torch.float32, torch.bfloat16)
-_ACT = {None: 0, 'none': 0, 'elu': 1, 'silu': 2, 'gelu': 3}
 
 
 def onehot_sample_host(x, u, G, C, unimix, mode=0):
@@ -266,6 +268,7 @@ class HipOps:
     self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
     self.ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=self.device)
     self.ws_bytes = ws_bytes
+    self._ws_ptr = self.ws.data_ptr()
     self.trace = None  # list of (label, flops, start_event, end_event) when profiling
 
   def mark_exact(self, t, lo, hi):
@@ -597,166 +600,59 @@ class HipOps:
 
   # ---- residual recurrent block -----------------------------------------------------
 
-  def _view(self, t, rows, cols, dtypes, what):
-    """(ptr, ld) of a [rows, cols] view on this device in one of `dtypes`; None: (0, 0)."""
-    if t is None:
-      return 0, 0
-    if t.get_device() != self._index or t.shape != (rows, cols) or t.dtype not in dtypes:
-      raise AssertionError(f'{what} is {tuple(t.shape)} {t.dtype} on {t.device}, not {(rows, cols)} in one of {dtypes} '
-                           f'on {self.device}')
-    ld, unit = t.stride()
-    assert unit == 1 or cols == 1, f'{what}: the columns are strided ({unit})'
-    return t.data_ptr(), (ld if rows > 1 else max(cols, ld))
-
-  def _flat(self, t, n, what, dtypes=(torch.float32,)):
-    """Pointer of a contiguous tensor of n values; None: 0."""
-    if t is None:
-      return 0
-    if t.get_device() != self._index or t.numel() != n or t.dtype not in dtypes or not t.is_contiguous():
-      raise AssertionError(f'{what} is {tuple(t.shape)} {t.dtype} on {t.device}: {n} contiguous values in one of {dtypes} '
-                           f'are needed on {self.device}')
-    return t.data_ptr()
-
-  def _block_call(self, name, *args):
-    """Launch on this device's current stream, whichever device is current."""
+  def _launch(self, name, *args):
+    """Run an entry of the native binding on this device's current stream, whichever device is current."""
+    fn = getattr(_block, name)
     stream = torch._C._cuda_getCurrentRawStream(self._index)
-    if torch._C._cuda_getDevice() != self._index:
-      with torch.cuda.device(self._index):
-        rc = getattr(self.lib, name)(*args, stream)
-    else:
-      rc = getattr(self.lib, name)(*args, stream)
-    if rc != 0:
-      self._check(rc, name)
+    if torch._C._cuda_getDevice() == self._index:
+      return fn(self._index, stream, *args)
+    with torch.cuda.device(self._index):
+      fn(self._index, stream, *args)
 
   def rms_norm_fwd(self, x, gamma, y, rstd=None, res=None, s=None, scale=None, eps=1e-6):
-    """s = x + res (in res' type; s may be res or x), y = s / sqrt(mean(s^2) + eps) * gamma.  y in fp32,
-    bf16, or e4m3 with scale [rows] (= max|y| / 448 per row).  rstd [rows] is what rms_norm_bwd reads."""
-    assert x.dim() == 2, x.shape
-    rows, C = x.shape
-    st = res.dtype if res is not None else s.dtype if s is not None else x.dtype
-    xp, ldx = self._view(x, rows, C, _REAL, 'x')
-    rp, ldr = self._view(res, rows, C, _REAL, 'res')
-    sp, lds = self._view(s, rows, C, (st,), 's')
-    yp, ldy = self._view(y, rows, C, _DT, 'y')
-    self._block_call(
-        'dd_rms_norm_fwd', xp, ldx, _DT[x.dtype], rp, ldr, _DT[st], sp, lds, self._flat(gamma, C, 'gamma'), yp, ldy,
-        _DT[y.dtype], self._flat(rstd, rows, 'rstd'), self._flat(scale, rows, 'scale'), rows, C, eps)
+    """s = x + res (in res' type; s may be res or x), y = s / sqrt(mean(s^2) + eps) * gamma.  x, res fp32 or
+    bf16; y fp32, bf16, or e4m3 with scale [rows] (= max|y| / 448 per row).  rstd [rows] is what
+    rms_norm_bwd reads."""
+    self._launch('rms_norm_fwd', x, gamma, y, rstd, res, s, scale, eps)
 
   def rms_norm_bwd(self, dy, s, rstd, gamma, ds, dgamma=None, dres=None, accumulate=False):
     """ds = dres + the norm's gradient at s: the gradient of x and of res (in s' type; ds may be dres).
     dgamma [C] is written, or added to with `accumulate`."""
-    assert s.dim() == 2, s.shape
-    rows, C = s.shape
-    yp, ldy = self._view(dy, rows, C, _REAL, 'dy')
-    sp, lds = self._view(s, rows, C, _REAL, 's')
-    rp, ldr = self._view(dres, rows, C, (s.dtype,), 'dres')
-    dp, ldd = self._view(ds, rows, C, (s.dtype,), 'ds')
-    self._block_call(
-        'dd_rms_norm_bwd', yp, ldy, _DT[dy.dtype], sp, lds, _DT[s.dtype], self._flat(rstd, rows, 'rstd'),
-        self._flat(gamma, C, 'gamma'), rp, ldr, dp, ldd, self._flat(dgamma, C, 'dgamma'), int(accumulate), rows, C,
-        self.ws.data_ptr(), self.ws_bytes)
+    self._launch('rms_norm_bwd', dy, s, rstd, gamma, ds, dgamma, dres, accumulate, self._ws_ptr, self.ws_bytes)
 
   def quant_rows(self, x, q, scale):
     """q = e4m3(x / scale), scale[row] = max|x[row]| / 448: the operands of linear_fwd's 8-bit form."""
-    assert x.dim() == 2, x.shape
-    rows, C = x.shape
-    xp, ldx = self._view(x, rows, C, _REAL, 'x')
-    qp, ldq = self._view(q, rows, C, (torch.float8_e4m3fn,), 'q')
-    assert scale is not None
-    self._block_call('dd_quant_rows', xp, ldx, _DT[x.dtype], qp, ldq, self._flat(scale, rows, 'scale'), rows, C)
+    self._launch('quant_rows', x, q, scale)
 
   def linear_fwd(self, x, w, y, bias=None, act=None, res=None, z=None, x_scale=None, w_scale=None):
     """y = act(x @ w^T * x_scale[:, None] * w_scale + bias) + res.  x [M, K] and w [N, K] bf16, or e4m3
-    with their scales; y bf16 or fp32, res in y's type (res may be y); act None, 'elu', 'silu' or 'gelu'.
-    z (bf16): the activation's argument, kept for linear_bwd."""
-    assert x.dim() == 2 and w.dim() == 2, (x.shape, w.shape)
-    (M, K), N = x.shape, w.shape[0]
-    assert x.dtype in (torch.bfloat16, torch.float8_e4m3fn), f'x is {x.dtype}: bf16 or e4m3 (fp32: gemm)'
-    xp, ldx = self._view(x, M, K, (x.dtype,), 'x')
-    wp, ldw = self._view(w, N, K, (x.dtype,), 'w')
-    yp, ldy = self._view(y, M, N, _REAL, 'y')
-    rp, ldr = self._view(res, M, N, (y.dtype,), 'res')
-    zp, ldz = self._view(z, M, N, (torch.bfloat16,), 'z')
-    self._block_call(
-        'dd_linear_fwd', xp, ldx, wp, ldw, _DT[x.dtype], self._flat(x_scale, M, 'x_scale'),
-        self._flat(w_scale, N, 'w_scale'), self._flat(bias, N, 'bias'), _ACT[act], rp, ldr, yp, ldy, _DT[y.dtype],
-        zp, ldz, M, N, K, self.ws.data_ptr(), self.ws_bytes)
+    with their scales (fp32 operands: `gemm`); y bf16 or fp32, res in y's type (res may be y); act None,
+    'elu', 'silu' or 'gelu'.  z (bf16): the activation's argument, kept for linear_bwd."""
+    self._launch('linear_fwd', x, w, y, bias, act, res, z, x_scale, w_scale, self._ws_ptr, self.ws_bytes)
 
   def linear_bwd(self, dy, x, w, dx=None, dw=None, dbias=None, act=None, z=None, dz=None, accumulate=False):
     """Gradients of linear_fwd's bf16 form (the gradient of res is dy): dx bf16 or fp32, dw and dbias fp32
     or bf16 (written, or added to with `accumulate`).  With an activation z is what linear_fwd kept and
     dz (bf16) receives dy * act'(z); dz may be dy or z."""
-    assert x.dim() == 2 and w.dim() == 2, (x.shape, w.shape)
-    (M, K), N = x.shape, w.shape[0]
-    bf = (torch.bfloat16,)
-    dyp, lddy = self._view(dy, M, N, bf, 'dy')
-    xp, ldx = self._view(x, M, K, bf, 'x')
-    wp, ldw = self._view(w, N, K, bf, 'w')
-    dxp, lddx = self._view(dx, M, K, _REAL, 'dx')
-    dwp, lddw = self._view(dw, N, K, _REAL, 'dw')
-    code = _ACT[act]
-    if code:
-      assert z is not None and dz is not None, 'an activation needs z and dz'
-    zp, ldz = self._view(z, M, N, bf, 'z') if code else (0, 0)
-    gp, ldg = self._view(dz, M, N, bf, 'dz') if code else (dyp, lddy)
-    db = self._flat(dbias, N, 'dbias', _REAL)
-    ws = self.ws.data_ptr(), self.ws_bytes
-    if code or db:
-      self._block_call('dd_linear_act_bwd', dyp, lddy, zp, ldz, code, gp, ldg, db,
-                       _DT[dbias.dtype] if db else 0, int(accumulate), M, N, *ws)
-    if dx is not None:
-      self._block_call('dd_linear_bwd_data', gp, ldg, wp, ldw, dxp, lddx, _DT[dx.dtype], M, N, K, *ws)
-    if dw is not None:
-      self._block_call('dd_linear_bwd_weight', gp, ldg, xp, ldx, dwp, lddw, _DT[dw.dtype], int(accumulate), M, N, K, *ws)
-
-  def _scan_args(self, u, T, first, cand):
-    assert u.dim() == 2, u.shape
-    rows, D = u.shape
-    assert T > 0 and rows % T == 0, f'{rows} rows are no sequences of {T} steps'
-    assert cand in ('tanh', None), cand
-    fp, fs = 0, 0
-    if first is not None:
-      assert first.get_device() == self._index and first.dtype == torch.float32 and first.shape == (rows,), 'first: fp32 [rows]'
-      fp, fs = _vec(first)
-    return rows, D, rows // T, fp, fs
+    self._launch('linear_bwd', dy, x, w, dx, dw, dbias, act, z, dz, accumulate, self._ws_ptr, self.ws_bytes)
 
   def gated_scan_fwd(self, u, c, h, T, i=None, first=None, h0=None, hT=None, shift=-1.0, cand='tanh'):
     """h[t] = sigmoid(-u - shift) h[t-1] + gate * cand(c[t]), gate = sigmoid(u + shift) or sigmoid(i), for
     sequences of T steps (rows b * T + t).  u, c, i, h: [B * T, D], all fp32 or all bf16 (column slices
     of one product's output, as a rule); first [B * T] fp32: non-zero restarts from zero; h0, hT [B, D]
-    fp32: the state before and after (hT may be h0)."""
-    rows, D, B, fp, fs = self._scan_args(u, T, first, cand)
-    dt = (u.dtype,)
-    up, ldu = self._view(u, rows, D, _REAL, 'u')
-    cp, ldc = self._view(c, rows, D, dt, 'c')
-    ip, ldi = self._view(i, rows, D, dt, 'i')
-    hp, ldh = self._view(h, rows, D, dt, 'h')
-    self._block_call(
-        'dd_gated_scan_fwd', up, ldu, cp, ldc, ip, ldi, _DT[u.dtype], fp, fs, self._flat(h0, B * D, 'h0'), hp, ldh,
-        self._flat(hT, B * D, 'hT'), B, T, D, shift, int(cand == 'tanh'), self.ws.data_ptr(), self.ws_bytes)
+    fp32: the state before and after (hT may be h0); cand 'tanh' or None."""
+    self._launch('gated_scan_fwd', u, c, h, T, i, first, h0, hT, shift, cand, self._ws_ptr, self.ws_bytes)
 
   def gated_step(self, u, c, h, h0, hT, i=None, first=None, shift=-1.0, cand='tanh'):
     """One step of gated_scan_fwd for [B, D] rows: the form of serving; hT may be h0."""
-    self.gated_scan_fwd(u, c, h, 1, i=i, first=first, h0=h0, hT=hT, shift=shift, cand=cand)
+    self._launch('gated_scan_fwd', u, c, h, 1, i, first, h0, hT, shift, cand, self._ws_ptr, self.ws_bytes)
 
   def gated_scan_bwd(self, dh, u, c, h, du, dc, T, i=None, di=None, first=None, h0=None, dhT=None, dh0=None,
                      shift=-1.0, cand='tanh'):
     """Gradients of gated_scan_fwd from dh [B * T, D] and dhT [B, D], with the h it wrote: du, dc, di in the
     operands' type, dh0 [B, D] fp32 (may be dhT)."""
-    rows, D, B, fp, fs = self._scan_args(u, T, first, cand)
-    dt = (u.dtype,)
-    up, ldu = self._view(u, rows, D, _REAL, 'u')
-    gp, ldg = self._view(dh, rows, D, dt, 'dh')
-    cp, ldc = self._view(c, rows, D, dt, 'c')
-    ip, ldi = self._view(i, rows, D, dt, 'i')
-    hp, ldh = self._view(h, rows, D, dt, 'h')
-    dup, lddu = self._view(du, rows, D, dt, 'du')
-    dcp, lddc = self._view(dc, rows, D, dt, 'dc')
-    dip, lddi = self._view(di, rows, D, dt, 'di')
-    self._block_call(
-        'dd_gated_scan_bwd', gp, ldg, up, ldu, cp, ldc, ip, ldi, hp, ldh, _DT[u.dtype], fp, fs,
-        self._flat(h0, B * D, 'h0'), self._flat(dhT, B * D, 'dhT'), dup, lddu, dcp, lddc, dip, lddi,
-        self._flat(dh0, B * D, 'dh0'), B, T, D, shift, int(cand == 'tanh'), self.ws.data_ptr(), self.ws_bytes)
+    self._launch('gated_scan_bwd', dh, u, c, h, du, dc, T, i, di, first, h0, dhT, dh0, shift, cand, self._ws_ptr,
+                 self.ws_bytes)
 
   # ---- fused observe scan ----------------------------------------------------------
 

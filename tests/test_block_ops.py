@@ -191,6 +191,28 @@ def test_scan_refusals():
   assert 'null' in refused('dd_gated_scan_bwd', None, 8, P, 8, P, 8, None, 0, *tail, None, 0, *more)
 
 
+def test_native_binding_refuses_before_it_calls():
+  """The checks of daydreamer_amd._block come before any launch: tensors of the host, other types and
+  wrong argument counts raise, and nothing is followed."""
+  hipops.load_library()
+  from daydreamer_amd import _block
+  x, g = torch.zeros(2, 8), torch.zeros(8)
+  with pytest.raises(AssertionError, match='x is not on device 0'):
+    _block.rms_norm_fwd(0, 0, x, g, x.clone(), None, None, None, None, 1e-6)
+  with pytest.raises(AssertionError, match='not on device'):
+    _block.linear_fwd(0, 0, x.bfloat16(), x.bfloat16(), x, None, None, None, None, None, None, 0, 0)
+  with pytest.raises(AssertionError, match='x is no tensor'):
+    _block.quant_rows(0, 0, 3, x, g)
+  with pytest.raises(AssertionError, match='2 rows are no sequences of 3 steps'):
+    _block.gated_scan_fwd(0, 0, x, x, x, 3, None, None, None, None, -1.0, 'tanh', 0, 0)
+  with pytest.raises(AssertionError, match='has 1 axes'):
+    _block.rms_norm_bwd(0, 0, g, g, g, g, g, None, None, 0, 0, 0)
+  with pytest.raises(AssertionError, match='arguments are needed'):
+    _block.linear_bwd(0, 0, x)
+  with pytest.raises(TypeError):
+    _block.gated_scan_fwd(0, 0, x, x, x, 'T', None, None, None, None, -1.0, 'tanh', 0, 0)
+
+
 def test_empty_calls_do_nothing():
   lib = hipops.load_library()
   assert lib.dd_rms_norm_fwd(*norm_args(rows=0, x=None, y=None)) == 0
