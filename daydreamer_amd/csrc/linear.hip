@@ -212,80 +212,6 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
   }
 }
 
-// ---- few rows: single steps of serving -----------------------------------------------------------
-//
-// At most 64 rows, so the weights are read once and that read is the time.  A workgroup owns 16 weight
-// rows, its waves take turns along the contraction (32 bf16 / 128 e4m3 each, operands straight from
-// memory into the 16 x 16 instruction's registers, UNROLL steps requested before the first is used) and
-// add up in LDS.  One launch, no partial sums in memory.
-template <int ES, int MB>
-__global__ void __launch_bounds__(1024) k_linear_few(Mat P, Mat Q, int K, Epi e) {
-  constexpr int BK = ES == 2 ? 32 : 128, UNROLL = MB <= 2 ? 4 : 2, LANE = BK / 4;   // elements of a lane's operand
-  __shared__ float sh[16][MB * 16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int row = lane & 15, kl = (lane >> 4) * LANE;
-  const long n0 = (long)blockIdx.x * 16;
-  f32x4 acc[MB] = {};
-  const i32x4 zero = {};
-  constexpr int PER = 16 / ES;           // elements of a 16-byte load
-  auto load = [&](const Mat& a, long r, int k, i32x4 v[LANE / PER]) {
-    const char* p = (const char*)a.p + (min(r, (long)a.R - 1) * a.ld + k) * ES;
-#pragma unroll
-    for (int j = 0; j < LANE / PER; ++j) {
-      v[j] = zero;
-      if (r < a.R && k + (j + 1) * PER <= K) __builtin_memcpy(&v[j], p + 16 * j, 16);
-    }
-  };
-  auto multiply = [&](const i32x4 q[LANE / PER], const i32x4 x[LANE / PER], int b) {
-    if constexpr (ES == 2) {
-      acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[0]), __builtin_bit_cast(bf16x8, x[0]), acc[b], 0, 0, 0);
-    } else {
-      const i32x8 w8 = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      const i32x8 x8 = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[b], 0, 0, 0, 127, 0, 127);
-    }
-  };
-  for (int k0 = wave * BK; k0 < K; k0 += waves * BK * UNROLL) {
-    i32x4 q[UNROLL][LANE / PER], x[UNROLL][MB][LANE / PER];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      load(Q, n0 + row, k0 + u * waves * BK + kl, q[u]);
-#pragma unroll
-      for (int b = 0; b < MB; ++b) load(P, b * 16 + row, k0 + u * waves * BK + kl, x[u][b]);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int b = 0; b < MB; ++b) multiply(q[u], x[u][b], b);
-  }
-  if (K % PER != 0 && wave == 0) {       // the contraction's last elements: one more step, in the first lanes' chunk
-    const int k = K - K % PER;
-    i32x4 q[LANE / PER] = {}, x[MB][LANE / PER] = {};
-    if (lane < 16) {
-      if (n0 + row < Q.R) q[0] = partial_chunk<ES>((const char*)Q.p + ((n0 + row) * Q.ld + k) * ES, K - k);
-#pragma unroll
-      for (int b = 0; b < MB; ++b)
-        if (b * 16 + row < P.R) x[b][0] = partial_chunk<ES>((const char*)P.p + ((b * 16 + row) * P.ld + k) * ES, K - k);
-    }
-#pragma unroll
-    for (int b = 0; b < MB; ++b) multiply(q, x[b], b);
-  }
-  // a lane holds columns 4 (lane >> 4) .. + 3 of row lane & 15
-#pragma unroll
-  for (int b = 0; b < MB; ++b)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sh[wave][b * 16 + row][4 * (lane >> 4) + j] = acc[b][j];
-  __syncthreads();
-  for (int i = threadIdx.x; i < MB * 16 * 16; i += blockDim.x) {
-    const int m = i >> 4, c = i & 15;
-    if (m < P.R && n0 + c < Q.R) {
-      float v[1] = {sh[0][m][c]};
-      for (int w = 1; w < waves; ++w) v[0] += sh[w][m][c];
-      finish<1>(e, m, n0 + c, v);
-    }
-  }
-}
-
 // Rows -> rows of whole 16-byte chunks, zeros behind; units of T (4 bytes
 // where the rows are aligned for it), `ldo` and `ldi` in units, 32 KB of a row per workgroup and pass.
 template <typename T>
@@ -318,14 +244,17 @@ template <int ES, bool RC, int R_, int NW>
 struct TileCopy {
   static constexpr int N = R_ / 8 / NW, BK = ROWB / ES;   // copies per wave and step
   const char* base;      // tile's first byte of the next step
-  long step;             // bytes per step
+  long step;             // bytes from a step to the next
   unsigned size;         // bytes from base to the end of the tile's last row (KC) or of a whole step (RC)
   unsigned ldb, cols;    // RC: bytes of a row, of the tile's part of it and what is behind
   int voff[N];
-  int col;               // KC: contraction elements in front of the lane's chunk, for the parities of the row
-  __device__ __forceinline__ void init(const Mat& a, long r0, long k0, int K, int wave, int lane) {
+  // KC: contraction elements in front of the lane's chunk (a single wave: in even and odd blocks of 8 rows;
+  // an even number of waves: a wave's blocks are all even or all odd)
+  int col[1 + NW % 2];
+  // the tile at (r0, k0); `apart`: steps of 128 bytes (KC) from one copy to the next
+  __device__ __forceinline__ void init(const Mat& a, long r0, long k0, int K, int wave, int lane, int apart = 1) {
     base = (const char*)a.p + (RC ? k0 * a.ld + r0 : r0 * a.ld + k0) * ES;
-    step = RC ? BK * a.ld * ES : ROWB;
+    step = RC ? BK * a.ld * ES : ROWB * apart;
     ldb = (unsigned)(a.ld * ES);
     cols = (unsigned)((a.R - r0) * ES + 3) & ~3u;   // (an odd length was packed: zeros behind)
     size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
@@ -340,22 +269,22 @@ struct TileCopy {
         voff[i] = (int)(r * ldb) + c * 16;
       }
     }
-    // NW is even: (r >> 1) & 7 = 4 (wave & 1) + (lane >> 4) for every copy
-    col = ((lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7)) * (16 / ES);
+#pragma unroll
+    for (int i = 0; i < 1 + NW % 2; ++i) col[i] = ((lane & 7) ^ ((4 * ((i * NW + wave) & 1) + (lane >> 4)) & 7)) * (16 / ES);
   }
   // The copies of the next step into LDS offset `lds`; rest: contraction elements left (none: zeros).
   // Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that
   // it cannot tell apart from the copy's target; the one wait that is needed is sync_copies.
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  __device__ __forceinline__ u32x4 begin(int rest) {
+  __device__ __forceinline__ u32x4 begin(int rest, int wave) {
     unsigned bytes = rest > 0 ? size : 0u;
     if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
     const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, bytes, 0x00020000u};
     if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks that are not whole are
 #pragma unroll                            // moved out of the descriptor's range (mend_tail writes the one that is cut)
-      for (int i = 0; i < N; ++i) voff[i] = col + 16 / ES > rest ? 0x7fffffff : voff[i];
+      for (int i = 0; i < N; ++i) voff[i] = col[i % (1 + NW % 2)] + 16 / ES > rest ? 0x7fffffff : voff[i];
     base += step;
-    if (!RC) size -= ROWB;
+    if (!RC) size -= (unsigned)step;
     return rs;
   }
   __device__ __forceinline__ void one(const u32x4& rs, unsigned lds, int wave, int i) const {
@@ -363,18 +292,18 @@ struct TileCopy {
                  :: "s"(lds + (i * NW + wave) * 1024), "v"(voff[i]), "s"(rs) : "memory");
   }
   __device__ __forceinline__ void issue(unsigned lds, int wave, int rest) {
-    const u32x4 rs = begin(rest);
+    const u32x4 rs = begin(rest, wave);
 #pragma unroll
     for (int i = 0; i < N; ++i) one(rs, lds, wave, i);
   }
 };
 // The chunk in which a KC operand's contraction ends (K is no multiple of a chunk), element by element into
-// its place in the tile of the last step; `threads` threads share the rows.
+// its place in the tile of the last step; `threads` threads, this one the thread-th, share the rows.
 template <int ES, int R_>
-__device__ __forceinline__ void mend_tail(const Mat& a, long r0, int K, int k0, char* tile, int threads) {
+__device__ __forceinline__ void mend_tail(const Mat& a, long r0, int K, int k0, char* tile, int thread, int threads) {
   constexpr int PER = 16 / ES;
   const int c = (K - k0) / PER, n = (K - k0) % PER;
-  for (int r = threadIdx.x; r < R_; r += threads) {
+  for (int r = thread; r < R_; r += threads) {
     i32x4 v = {0, 0, 0, 0};
     if (r0 + r < a.R) v = partial_chunk<ES>((const char*)a.p + ((r0 + r) * a.ld + k0 + c * PER) * ES, n);
     *reinterpret_cast<i32x4*>(tile + r * ROWB + ((c ^ ((r >> 1) & 7)) << 4)) = v;
@@ -482,8 +411,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   const bool cut = kend == K && K % (16 / ES) != 0 && !(P_RC && Q_RC);
   auto mend = [&](int at_p, int at_q) {
     const int k0 = (int)kb + (steps - 1) * BK;
-    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + at_p, NW * 64);
-    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + at_q, NW * 64);
+    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + at_p, threadIdx.x, NW * 64);
+    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + at_q, threadIdx.x, NW * 64);
     sync_copies();
   };
   int p0 = 0, p1 = UP, p2 = 2 * UP, q0 = 3 * UP, q1 = 3 * UP + UQ;
@@ -503,8 +432,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
         if (cut && t + 2 == steps) mend(p1, q1);
       }
       typename decltype(cp)::u32x4 rs;
-      if (g == GROUPS - 1) { rs = cq.begin(rest_q); rest_q -= BK; }
-      if (g == 0) { rs = cp.begin(rest_p); rest_p -= BK; }
+      if (g == GROUPS - 1) { rs = cq.begin(rest_q, wave); rest_q -= BK; }
+      if (g == 0) { rs = cp.begin(rest_p, wave); rest_p -= BK; }
 #pragma unroll
       for (int i = 0; i < MH; ++i) {
 #pragma unroll
@@ -659,6 +588,93 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   }
 }
 
+// ---- few rows: single steps of serving -----------------------------------------------------------
+//
+// At most 64 rows, so the weights are read once and that read is the time.  A workgroup owns 16 weight
+// rows; its waves take turns along the contraction, 128 bytes of every row at a time, each with two LDS
+// buffers of its own: no barrier, the next turn's copies are in flight while 16 x 16 instructions work on
+// this one's.  At the end the waves add up in LDS: one launch, no partial sums in memory.  (Operands straight
+// into registers would have 16 different rows in every quarter of a load: 18 bytes per clock and CU instead of
+// 60; 32 x 1024 x 4096 bf16 13 us.)
+template <int ES, int MB, int WV>
+__global__ void __launch_bounds__(64 * WV) k_linear_few(Mat P, Mat Q, int K, Epi e) {
+  constexpr int BK = ROWB / ES, TURN = (16 + 16 * MB) * ROWB, COPIES = 2 + 2 * MB;
+  __shared__ __attribute__((aligned(1024))) char sh[WV * 2 * TURN];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, g = lane >> 4, swz = (row >> 1) & 7;
+  const long n0 = (long)blockIdx.x * 16;
+  const int steps = (K + BK - 1) / BK, turns = wave < steps ? (steps - wave + WV - 1) / WV : 0;
+  char* mine = sh + wave * 2 * TURN;
+  const unsigned lds = (unsigned)(uintptr_t)(DD_LDS char*)mine;
+  TileCopy<ES, false, 16, 1> cq;
+  TileCopy<ES, false, 16 * MB, 1> cp;
+  int rest = K - wave * BK;
+  cq.init(Q, n0, (long)wave * BK, K, 0, lane, WV);
+  cp.init(P, 0, (long)wave * BK, K, 0, lane, WV);
+  auto copy = [&](int buf) {
+    cq.issue(lds + buf * TURN, 0, rest);
+    cp.issue(lds + buf * TURN + 16 * ROWB, 0, rest);
+    rest -= WV * BK;
+  };
+  f32x4 acc[MB] = {};
+  copy(0);
+  copy(1);
+  for (int t = 0; t < turns; ++t) {
+    char* a = mine + (t & 1) * TURN;
+    __builtin_amdgcn_s_waitcnt(0x0f70 | COPIES);   // all but the next turn's copies have landed
+    asm volatile("" ::: "memory");
+    const int k0 = (wave + t * WV) * BK;
+    if (K % (16 / ES) != 0 && k0 + BK > K) {        // the contraction ends inside a chunk
+      mend_tail<ES, 16>(Q, n0, K, k0, a, lane, 64);
+      mend_tail<ES, 16 * MB>(P, 0, K, k0, a + 16 * ROWB, lane, 64);
+      __builtin_amdgcn_s_waitcnt(0xc07f);           // lgkmcnt 0
+      asm volatile("" ::: "memory");
+    }
+    auto chunk = [&](int r, int c) { return *reinterpret_cast<const i32x4*>(a + (r + row) * ROWB + ((c ^ swz) << 4)); };
+    i32x4 q[2], x[MB][2];
+    // bf16: chunks g, 4 + g for the two instructions; e4m3: any two that both operands agree on
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      q[j] = chunk(0, 4 * j + g);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) x[b][j] = chunk(16 + 16 * b, 4 * j + g);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);             // read before the buffer is copied into again
+    asm volatile("" ::: "memory");
+    copy(t & 1);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      if constexpr (ES == 2) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[j]), __builtin_bit_cast(bf16x8, x[b][j]), acc[b], 0, 0, 0);
+      } else {
+        const i32x8 w8 = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const i32x8 x8 = __builtin_shufflevector(x[b][0], x[b][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[b], 0, 0, 0, 127, 0, 127);
+      }
+    }
+  }
+  sync_copies();   // (the copies behind the end wrote zeros)
+  // a lane holds columns 4 g .. + 3 of row lane & 15
+  float* out = reinterpret_cast<float*>(sh);
+  static_assert(WV * MB * 16 * 17 * 4 <= WV * 2 * TURN, "the sums fit the copies' LDS");
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[((wave * MB + b) * 16 + row) * 17 + 4 * g + j] = acc[b][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MB * 256; i += 64 * WV) {
+    const int m = i >> 4, c = i & 15;
+    if (m < P.R && n0 + c < Q.R) {
+      float v[1] = {out[m * 17 + c]};
+#pragma unroll
+      for (int w = 1; w < WV; ++w) v[0] += out[(w * MB * 16 + m) * 17 + c];
+      finish<1>(e, m, n0 + c, v);
+    }
+  }
+}
+
 // Sum of the partial results of a split contraction, slabs ascending, and the epilogue: eight columns of a
 // row per thread, element by element where the row ends inside them.
 template <int V>
@@ -769,12 +785,11 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
 template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
   if constexpr (!P_RC && !Q_RC)
-    if (P.R <= 64 && K > 0) {
-      const int threads = 64 * max(4, min(16, K / (ES == 2 ? 64 : 256)));
+    if (P.R <= 64 && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
       const unsigned grid = dd_ceil_div(Q.R, 16);
-      if (P.R <= 16) k_linear_few<ES, 1><<<grid, threads, 0, st>>>(P, Q, K, e);
-      else if (P.R <= 32) k_linear_few<ES, 2><<<grid, threads, 0, st>>>(P, Q, K, e);
-      else k_linear_few<ES, 4><<<grid, min(threads, 512), 0, st>>>(P, Q, K, e);
+      if (P.R <= 16) k_linear_few<ES, 1, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
+      else if (P.R <= 32) k_linear_few<ES, 2, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
+      else k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
       DD_CHECK_LAUNCH(who);
       return 0;
     }
