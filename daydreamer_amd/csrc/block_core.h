@@ -135,15 +135,14 @@ __device__ __forceinline__ float expm1_neg(float x) {
   return x > -0.3f ? s : fast_exp(x) - 1.0f;
 }
 
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), with Abramowitz and Stegun's 7.1.26 for erf
-// (absolute error 1.5e-7, so 0.75e-7 here) on the same exponential.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
+// Phi(-|z|), Phi(z) = (1 + erf(z / sqrt 2)) / 2, and e = exp(-z^2 / 2), with Abramowitz and Stegun's 7.1.26
+// for erf (absolute error 1.5e-7, so 0.75e-7 here) on the same exponential.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
   const float t = fast_rcp(fma_(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
   e = __builtin_amdgcn_exp2f(-0.5f * 1.44269504088896341f * z * z);
   float q = fma_(t, 0.5f * 1.061405429f, -0.5f * 1.453152027f);
   q = fma_(t, q, 0.5f * 1.421413741f); q = fma_(t, q, -0.5f * 0.284496736f); q = fma_(t, q, 0.5f * 0.254829592f);
-  q *= e * t;
-  return z >= 0.f ? 1.0f - q : q;
+  return q * (e * t);
 }
 
 // out[c] (+)= sum of n partial rows: 32 columns and 32 row lanes per workgroup, eight loads in flight per
@@ -171,7 +170,10 @@ __device__ __forceinline__ float act_f(float z) {
   float p, q;
   if constexpr (ACT == DD_ACT_ELU) return z > 0.f ? z : expm1_neg(z);
   if constexpr (ACT == DD_ACT_SILU) { sigmoid2(z, p, q); return z * p; }
-  if constexpr (ACT == DD_ACT_GELU) return z * normal_cdf(z, q);
+  if constexpr (ACT == DD_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    p = normal_tail(z, q);
+    return fma_(-fminf(fabsf(z), 3e38f), p, fmaxf(z, 0.0f));   // (infinity: 0 of it)
+  }
   return z;
 }
 template <int ACT>
@@ -179,7 +181,10 @@ __device__ __forceinline__ float act_slope(float z) {
   float p, q;
   if constexpr (ACT == DD_ACT_ELU) return z > 0.f ? 1.0f : fast_exp(z);
   if constexpr (ACT == DD_ACT_SILU) { sigmoid2(z, p, q); return p * (1.0f + z * q); }
-  if constexpr (ACT == DD_ACT_GELU) { p = normal_cdf(z, q); return p + z * q * 0.39894228040143268f; }
+  if constexpr (ACT == DD_ACT_GELU) {
+    p = normal_tail(z, q);
+    return (z >= 0.f ? 1.0f - p : p) + z * q * 0.39894228040143268f;
+  }
   return 1.0f;
 }
 

@@ -51,7 +51,7 @@ __device__ __forceinline__ void finish(const Epi& e, long m, long n, float v[V])
     for (int j = 0; j < V; ++j) v[j] += b[j];
   }
   // the pre-activation is kept in bf16 for the backward pass (the derivative is read from it: an
-  // error of 2^-9 relative, the size of the rounding of the gradients themselves)
+  // error of 2^-8 relative at most, the size of the rounding of the gradients themselves)
   if (e.z) store_bf16<V>(e.z + m * e.ldz + n, v);
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = act_any(e.act, v[j]);
@@ -236,9 +236,10 @@ __global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int 
 // fall on different banks:
 //   KC operand: tile [R][128 B], slot c of row r holds chunk c ^ ((r >> 1) & 7); a lane reads 16 bytes
 //     (8 bf16 or 16 e4m3 of its row)
-//   RC operand: tile [64 k][R], slot c of row k holds chunk c ^ ((k & 3) << 2); read by the transposing
-//     LDS load: 4 k of one row per lane, two loads for the 8 k an instruction wants
+//   RC operand: tile [64 k][R], slot c of row k holds chunk c ^ rc_swizzle(k); read by the transposing LDS
+//     load: 4 k of one row per lane, two loads for the 8 k an instruction wants
 #define DD_LDS __attribute__((address_space(3)))
+__device__ __forceinline__ int rc_swizzle(int k) { return ((k & 3) << 2) ^ ((k >> 2) & 2); }
 
 template <int ES, bool RC, int R_, int NW>
 struct TileCopy {
@@ -262,7 +263,7 @@ struct TileCopy {
     for (int i = 0; i < N; ++i) {
       const int id = (i * NW + wave) * 64 + lane;
       if constexpr (RC) {
-        const int k = id / (R_ / 8), c = (id % (R_ / 8)) ^ ((k & 3) << 2);
+        const int k = id / (R_ / 8), c = (id % (R_ / 8)) ^ rc_swizzle(k);
         voff[i] = (int)(k * ldb) + c * 16;
       } else {
         const int r = id >> 3, c = (id & 7) ^ ((r >> 1) & 7);
@@ -320,52 +321,66 @@ __device__ __forceinline__ void sync_copies() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The instruction operand of rows r .. r + 31 and contraction step s (16 bf16: ES 2, 64 e4m3: ES 1).
+// The matrix instruction, by element size: rows of an operand block, accumulator, and the operand of rows
+// r .. r + ROWS - 1 and contraction step s (32 bf16, 64 e4m3).  bf16 takes the 16 x 16 form: it needs more
+// operands per product than 32 x 32 but moves half the accumulators, and under the chip's power cap that is
+// clock (8192^3: 766 against 811 us).
+template <int ES>
+struct Inst;
+template <>
+struct Inst<2> {
+  static constexpr int ROWS = 16;
+  typedef f32x4 Acc;
+  typedef bf16x8 Op;
+};
+template <>
+struct Inst<1> {
+  static constexpr int ROWS = 32;
+  typedef f32x16 Acc;
+  typedef i32x8 Op;
+};
 template <int ES, bool RC, int R_>
 struct Frag;
 template <int R_>
 struct Frag<2, false, R_> {
-  typedef bf16x8 T;
-  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
-    const int row = r + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((row >> 1) & 7);
+  static __device__ __forceinline__ bf16x8 read(const char* sh, int r, int s, int lane) {
+    const int row = r + (lane & 15), c = (4 * s + (lane >> 4)) ^ ((row >> 1) & 7);
     return *reinterpret_cast<const bf16x8*>(sh + row * ROWB + c * 16);
   }
 };
 template <int R_>
 struct Frag<2, true, R_> {
-  typedef bf16x8 T;
-  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
+  static __device__ __forceinline__ bf16x8 read(const char* sh, int r, int s, int lane) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    const int k = s * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);   // & 3 is the lane's alone
-    const int row = r + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    const int at = k * (R_ * 2) + (((row >> 3) ^ ((k & 3) << 2)) << 4) + (row & 4) * 2;
+    const int k = s * 32 + (lane >> 4) * 8 + ((lane & 15) >> 2), row = r + (lane & 3) * 4;
+    const int at = k * (R_ * 2) + (((row >> 3) ^ rc_swizzle(k)) << 4) + (row & 4) * 2;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DD_LDS s16x4*)(sh + at));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DD_LDS s16x4*)(sh + at + 4 * R_ * 2));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DD_LDS s16x4*)(sh + at + 4 * R_ * 2));   // k + 4: the same swizzle
     const s16x8 t = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     return __builtin_bit_cast(bf16x8, t);
   }
 };
 template <int R_>
 struct Frag<1, false, R_> {
-  typedef i32x8 T;
   // (which 32 of the 64 elements a lane holds, and in which order, is free: both operands agree)
-  static __device__ __forceinline__ T read(const char* sh, int r, int s, int lane) {
+  static __device__ __forceinline__ i32x8 read(const char* sh, int r, int s, int lane) {
     const int row = r + (lane & 31), x = (row >> 1) & 7, c = 4 * s + 2 * (lane >> 5);
     const i32x4 a = *reinterpret_cast<const i32x4*>(sh + row * ROWB + ((c ^ x) << 4));
     const i32x4 b = *reinterpret_cast<const i32x4*>(sh + row * ROWB + (((c + 1) ^ x) << 4));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
-__device__ __forceinline__ f32x16 mma(bf16x8 q, bf16x8 p, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, p, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(bf16x8 q, bf16x8 p, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, p, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(i32x8 q, i32x8 p, f32x16 c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(q, p, c, 0, 0, 0, 127, 0, 127);
 }
 
 template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
-  constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, UP = BM * ROWB, UQ = BN * ROWB;
-  constexpr int STEPS = ES == 2 ? 4 : 2, BK = ROWB / ES;
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
+  typedef Inst<ES> I;
+  constexpr int NW = WM * WN, MT = BM / WM / I::ROWS, NT = BN / WN / I::ROWS, UP = BM * ROWB, UQ = BN * ROWB;
+  constexpr int STEPS = 2, BK = ROWB / ES;
   __shared__ __attribute__((aligned(1024))) char sh[3 * UP + 2 * UQ];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles, four
@@ -387,19 +402,18 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   cp.init(P, m0, kb, K, wave, lane);
   cq.init(Q, n0, kb, K, wave, lane);
   const unsigned lds = (unsigned)(uintptr_t)(DD_LDS char*)sh;
-  f32x16 acc[MT][NT] = {};
+  typename I::Acc acc[MT][NT] = {};
   int rest_p = kend - (int)kb, rest_q = rest_p;   // of the step that is copied next
-  // A group: one contraction step of the instruction, all of the wave's rows (e4m3: half of them, its
-  // operands are twice as large).  Two register sets.
-  constexpr int H = ES == 2 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
-  typename Frag<ES, P_RC, BM>::T p[2][MH];
-  typename Frag<ES, Q_RC, BN>::T q[2][NT];
+  // A group: one contraction step of the instruction, all of the wave's rows, or half of them where two register
+  // sets of all would not fit.
+  constexpr int H = ES == 2 && MT <= 4 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
+  typename I::Op p[2][MH], q[2][NT];
   // one of a group's NT + MH operands
   auto read1 = [&](int at_p, int at_q, int g, int k) {
     if (k < NT) {
-      if (g % H == 0) q[(g / H) & 1][k] = Frag<ES, Q_RC, BN>::read(sh + at_q, wn + 32 * k, g / H, lane);
+      if (g % H == 0) q[(g / H) & 1][k] = Frag<ES, Q_RC, BN>::read(sh + at_q, wn + I::ROWS * k, g / H, lane);
     } else {
-      p[g & 1][k - NT] = Frag<ES, P_RC, BM>::read(sh + at_p, wm + 32 * (k - NT + (g % H) * MH), g / H, lane);
+      p[g & 1][k - NT] = Frag<ES, P_RC, BM>::read(sh + at_p, wm + I::ROWS * (k - NT + (g % H) * MH), g / H, lane);
     }
   };
   // The waves meet once a step, before its last group: step t + 1 has landed, step t's tiles are free but for
@@ -459,15 +473,15 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
   }
   sync_copies();
 
-  // 32 rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds
-  // four consecutive columns of one row); LPR lanes finish a row, 8 columns each, in two halves of RI rows
-  // per lane.  What they need from memory is requested before
-  // the exchange through LDS.  The loop stays rolled - the next
-  // accumulators move down - because copies of three activations would not fit the instruction cache.
-  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI;
-  static_assert(RI * RPI == 16, "a half is whole rows of every lane");
-  static_assert(NW * 32 * LD * 4 <= 3 * UP + 2 * UQ, "the epilogue's LDS");
-  float* out = reinterpret_cast<float*>(sh) + wave * 32 * LD;
+  // Sixteen rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds four
+  // consecutive columns of one row); LPR lanes finish a row, 8 columns each, RI rows per lane.  What they
+  // need from memory is requested before the exchange through LDS.  Only the writes to LDS know which
+  // accumulators they take; the rest of the loop stays rolled, because copies of three activations would
+  // not fit the instruction cache.
+  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI, ROWS = I::ROWS;
+  static_assert(RI * RPI == 16, "sixteen rows are whole rows of every lane");
+  static_assert(NW * ROWS * LD * 4 <= 3 * UP + 2 * UQ, "the epilogue's LDS");
+  float* out = reinterpret_cast<float*>(sh) + wave * ROWS * LD;
   float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
   const int nc = (lane % LPR) * 8;
   const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
@@ -491,23 +505,24 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
     }
   };
   fetch(0);
+  constexpr int HALVES = MT * ROWS / 16, PER = ROWS / 16;   // sixteens of rows, and of an accumulator block
 #pragma unroll 1
-  for (int i = 0; i < 2 * MT; ++i) {
-    if (i % 2 == 0) {
+  for (int i = 0; i < HALVES; ++i) {
+    if (i % PER == 0) {
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      for (int k = 0; k < MT; ++k)
+        if (i == k * PER)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 v = {acc[0][j][4 * g], acc[0][j][4 * g + 1], acc[0][j][4 * g + 2], acc[0][j][4 * g + 3]};
-          *reinterpret_cast<f32x4*>(out + (lane & 31) * LD + 32 * j + 8 * g + 4 * (lane >> 5)) = v;
-        }
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int k = 0; k + 1 < MT; ++k) acc[k][j] = acc[k + 1][j];
-      }
+            for (int g = 0; g < PER * PER; ++g) {   // 16 x 16: one run of four columns, 32 x 32: four, 8 apart
+              const f32x4 v = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
+              *reinterpret_cast<f32x4*>(out + (lane % ROWS) * LD + ROWS * j + 8 * g + 4 * (lane / ROWS)) = v;
+            }
       __builtin_amdgcn_wave_barrier();
     }
-    const float* rows = out + (lane / LPR + 16 * (i & 1)) * LD + nc;
+    const float* rows = out + (lane / LPR + 16 * (i % PER)) * LD + nc;
     if (slab) {
 #pragma unroll
       for (int k = 0; k < RI; ++k) {
@@ -526,19 +541,19 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
       float v[RI][8], col[8];
 #pragma unroll
       for (int k = 0; k < RI; ++k) load_f32<8>(rows + RPI * k * LD, v[k]);
+      float bias[8] = {};
+      if (e.bias) load_f32<8>(e.bias + n, bias);
       if (e.xs) {
         load_f32<8>(e.wsc + n, col);
 #pragma unroll
         for (int k = 0; k < RI; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] *= xs[k] * col[j];
-      }
-      if (e.bias) {
-        load_f32<8>(e.bias + n, col);
+          for (int j = 0; j < 8; ++j) v[k][j] = fma_(v[k][j] * xs[k], col[j], bias[j]);
+      } else {
 #pragma unroll
         for (int k = 0; k < RI; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] += col[j];
+          for (int j = 0; j < 8; ++j) v[k][j] += bias[j];
       }
       if (e.z)
 #pragma unroll
@@ -584,7 +599,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_linear_tile(Mat P, Mat Q, int 
         if (mrow + 16 * i + RPI * k < P.R)
           finish_ragged(e, mrow + 16 * i + RPI * k, n, Q.R, rows + RPI * k * LD);
     }
-    if (i + 1 < 2 * MT) fetch(i + 1);
+    if (i + 1 < HALVES) fetch(i + 1);
   }
 }
 
@@ -718,11 +733,11 @@ inline bool tileable(const Mat& a, bool rc, int es) {
 
 // The two tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and
 // the rest of a tile (start, epilogue) take then, in microseconds (measured: 256 x 256 at 8192^3 and 37500 x
-// 1024 x 2048, 128 x 128 at 37500 x 1024 x 2048).  The large one is faster per output (1390 against 1140
+// 1024 x 2048, 128 x 128 at 37500 x 1024 x 2048).  The large one is faster per output (1430 against 1140
 // TFLOP/s, bf16, 8192^3); the small one fills the chip with fewer rows and wastes less in a last round
 // (2500 x 2048 x 1536: 25 against 36 us).
 struct TileShape { int side, slots; float step, rest; };
-constexpr TileShape SHAPES[] = {{256, 256, 1.48f, 10.f}, {128, 512, 0.96f, 4.5f}};
+constexpr TileShape SHAPES[] = {{256, 256, 1.38f, 10.f}, {128, 512, 0.96f, 4.5f}};
 
 struct Plan { int shape, splits; float us; };
 inline Plan plan_product(long M, long N, int ksteps, size_t slab_room) {
@@ -802,7 +817,7 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
     if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
       const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), room);
       if (plan.shape == 0) return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
-      return tiled<ES, P_RC, Q_RC, 128, 128, 2, 2>(who, p, q, K, plan.splits, e, (float*)at, st);
+      return tiled<ES, P_RC, Q_RC, 128, 128, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
     }
   }
   const int bk = ROWB / ES;
