@@ -241,6 +241,14 @@ __global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int 
 #define DD_LDS __attribute__((address_space(3)))
 __device__ __forceinline__ int rc_swizzle(int k) { return ((k & 3) << 2) ^ ((k >> 2) & 2); }
 
+// 16 bytes per lane from a buffer descriptor's range to LDS, lane after lane from offset `lds`; zeros past the range.
+// Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that it cannot
+// tell apart from the copy's target; the waits that are needed are written out.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void copy16(const u32x4& rs, unsigned lds, int voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(rs) : "memory");
+}
+
 template <int ES, bool RC, int R_, int NW>
 struct TileCopy {
   static constexpr int N = R_ / 8 / NW, BK = ROWB / ES;   // copies per wave and step
@@ -274,9 +282,6 @@ struct TileCopy {
     for (int i = 0; i < 1 + NW % 2; ++i) col[i] = ((lane & 7) ^ ((4 * ((i * NW + wave) & 1) + (lane >> 4)) & 7)) * (16 / ES);
   }
   // The copies of the next step into LDS offset `lds`; rest: contraction elements left (none: zeros).
-  // Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that
-  // it cannot tell apart from the copy's target; the one wait that is needed is sync_copies.
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   __device__ __forceinline__ u32x4 begin(int rest, int wave) {
     unsigned bytes = rest > 0 ? size : 0u;
     if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
@@ -289,8 +294,7 @@ struct TileCopy {
     return rs;
   }
   __device__ __forceinline__ void one(const u32x4& rs, unsigned lds, int wave, int i) const {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(lds + (i * NW + wave) * 1024), "v"(voff[i]), "s"(rs) : "memory");
+    copy16(rs, lds + (i * NW + wave) * 1024, voff[i]);
   }
   __device__ __forceinline__ void issue(unsigned lds, int wave, int rest) {
     const u32x4 rs = begin(rest, wave);
@@ -377,11 +381,11 @@ __device__ __forceinline__ f32x16 mma(i32x8 q, i32x8 p, f32x16 c) {
 }
 
 template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
+__global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
   typedef Inst<ES> I;
   constexpr int NW = WM * WN, MT = BM / WM / I::ROWS, NT = BN / WN / I::ROWS, UP = BM * ROWB, UQ = BN * ROWB;
-  constexpr int STEPS = 2, BK = ROWB / ES;
-  __shared__ __attribute__((aligned(1024))) char sh[3 * UP + 2 * UQ];
+  constexpr int STEPS = 2, BK = ROWB / ES, LDS = 3 * UP + 2 * UQ;
+  __shared__ __attribute__((aligned(1024))) char sh[LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Consecutive workgroups go to the eight XCDs in turn: each XCD gets a contiguous run of tiles, four
   // columns wide, so that its L2 serves the rows and weights that its 32 running tiles share
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_tile(Mat P, Mat Q, i
         sync_copies<TileCopy<ES, P_RC, BM, NW>::N>();
         if (cut && t + 2 == steps) mend(p1, q1);
       }
-      typename decltype(cp)::u32x4 rs;
+      u32x4 rs;
       if (g == GROUPS - 1) { rs = cq.begin(rest_q, wave); rest_q -= BK; }
       if (g == 0) { rs = cp.begin(rest_p, wave); rest_p -= BK; }
 #pragma unroll
@@ -474,91 +478,119 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_tile(Mat P, Mat Q, i
   sync_copies();
 
   // Sixteen rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds four
-  // consecutive columns of one row); LPR lanes finish a row, 8 columns each, RI rows per lane.  What they
-  // need from memory is requested before the exchange through LDS.  Only the writes to LDS know which
-  // accumulators they take; the rest of the loop stays rolled, because copies of three activations would
-  // not fit the instruction cache.
-  constexpr int W = BN / WN, LD = W + 4, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI, ROWS = I::ROWS;
+  // consecutive columns of one row); LPR lanes finish a row, 8 columns each, RI rows per lane.  The residual's
+  // tile - the part of it that these lanes finish - comes into the wave's LDS in one burst (fp32: in two), as
+  // the tiles did: requested sixteen rows at a time it cost a memory latency each (37500 x 2048 x 1024 with a
+  // residual: 222 us).  Only the writes to LDS know which accumulators they take; the rest of the
+  // loop stays rolled, because copies of three activations would not fit the instruction cache.
+  constexpr int W = BN / WN, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI, ROWS = I::ROWS, WROWS = BM / WM, HALVES = WROWS / 16;
+  constexpr int OUT = 16 * W * 4, RES = LDS / NW - OUT;   // bytes of a wave
   static_assert(RI * RPI == 16, "sixteen rows are whole rows of every lane");
-  static_assert(NW * ROWS * LD * 4 <= 3 * UP + 2 * UQ, "the epilogue's LDS");
-  float* out = reinterpret_cast<float*>(sh) + wave * ROWS * LD;
-  float* slab = slabs ? slabs + (long)split * P.R * Q.R : nullptr;
+  static_assert(RES >= WROWS * W * 2, "the residual's LDS");
+  char* mine = sh + wave * (OUT + RES);
+  float* out = reinterpret_cast<float*>(mine);
+  // 16-byte chunk c of row r, permuted by the row so that the writes of 16 rows fall on different banks
+  auto at = [&](int r, int c) { return out + r * W + ((c ^ (r & (W / 4 - 1))) << 2); };
   const int nc = (lane % LPR) * 8;
   const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
   const bool full = n + 8 <= Q.R;
-  u32x4u res[RI][2];
-  float xs[RI];
-  auto fetch = [&](int i) {
-#pragma unroll
-    for (int k = 0; k < RI; ++k) {
-      const long m = mrow + 16 * i + RPI * k;
-      if (!full || slab || m >= P.R) continue;
-      if (e.xs) xs[k] = e.xs[m];
-      if (e.res) {
-        if (e.ytype == DD_F32) {
-          res[k][0] = reinterpret_cast<const u32x4u*>((const float*)e.res + m * e.ldr + n)[0];
-          res[k][1] = reinterpret_cast<const u32x4u*>((const float*)e.res + m * e.ldr + n)[1];
-        } else {
-          res[k][0] = *reinterpret_cast<const u32x4u*>((const __bf16*)e.res + m * e.ldr + n);
-        }
-      }
-    }
-  };
-  fetch(0);
-  constexpr int HALVES = MT * ROWS / 16, PER = ROWS / 16;   // sixteens of rows, and of an accumulator block
+  const int es = e.ytype == DD_F32 ? 4 : 2, burst = e.ytype == DD_F32 ? HALVES / 2 : HALVES;
+  auto fetch = [&](int i) {   // the residual's rows 16 i .. 16 (i + burst) - 1 of the wave
+    const int rows = (int)min((long)burst * 16, P.R - (m0 + wm + 16 * i)), cols = (int)min((long)W, Q.R - (n0 + wn));
+    const unsigned ldb = (unsigned)(e.ldr * es);
+    const char* base = (const char*)e.res + ((m0 + wm + 16 * i) * e.ldr + n0 + wn) * es;
+    const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu,
+                      rows > 0 && cols > 0 ? (rows - 1) * ldb + cols * es : 0u, 0x00020000u};
+    const unsigned to = lds + wave * (OUT + RES) + OUT, step = 1024 / (W * es) * ldb,
+                   v = es == 4 ? lane / (W / 4) * ldb + lane % (W / 4) * 16 : lane / (W / 8) * ldb + lane % (W / 8) * 16;
 #pragma unroll 1
-  for (int i = 0; i < HALVES; ++i) {
-    if (i % PER == 0) {
-      __builtin_amdgcn_wave_barrier();
+    for (int k = 0; k < WROWS * W * 2 / 1024; ++k) copy16(rs, to + k * 1024, (int)(v + k * step));
+  };
+  // the sums of sixteen rows: lane's RI rows of 8 columns
+  const int lr = lane / LPR;
+  float v[RI][8];
+  auto exchange = [&](int i) {
+    constexpr int PER = ROWS / 16;   // sixteens of an accumulator block
+    // (a bit, not i / PER == k: the compiler would index the accumulators by i, in memory)
+    const unsigned which = 1u << i / PER;
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int k = 0; k < MT; ++k)
-        if (i == k * PER)
+    for (int k = 0; k < MT; ++k)
+      if (which >> k & 1 && (PER == 1 || (lane % 32) / 16 == i % PER))
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int g = 0; g < PER * PER; ++g) {   // 16 x 16: one run of four columns, 32 x 32: four, 8 apart
-              const f32x4 v = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
-              *reinterpret_cast<f32x4*>(out + (lane % ROWS) * LD + ROWS * j + 8 * g + 4 * (lane / ROWS)) = v;
-            }
-      __builtin_amdgcn_wave_barrier();
-    }
-    const float* rows = out + (lane / LPR + 16 * (i % PER)) * LD + nc;
-    if (slab) {
+          for (int g = 0; g < PER * PER; ++g) {   // 16 x 16: one run of four columns, 32 x 32: four, 8 apart
+            const f32x4 t = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
+            *reinterpret_cast<f32x4*>(at(lane % 16, (ROWS * j + 8 * g) / 4 + lane / ROWS)) = t;
+          }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < RI; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(at(lr + RPI * k, nc / 4 + h));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][4 * h + j] = t[j];
+      }
+  };
+  if (slabs) {
+    float* slab = slabs + ((long)split * P.R + mrow) * Q.R + n;
+#pragma unroll 1
+    for (int i = 0; i < HALVES; ++i) {
+      exchange(i);
 #pragma unroll
       for (int k = 0; k < RI; ++k) {
-        const long m = mrow + 16 * i + RPI * k;
-        const float* from = rows + RPI * k * LD;
-        if (m >= P.R) continue;
+        if (mrow + 16 * i + RPI * k >= P.R) continue;
+        float* to = slab + (long)(16 * i + RPI * k) * Q.R;
         if (full) {
-          float v[8];
-          load_f32<8>(from, v);
-          store_f32<8>(slab + m * Q.R + n, v);
+          store_f32<8>(to, v[k]);
         } else {
-          for (int j = 0; j < 8 && n + j < Q.R; ++j) slab[m * Q.R + n + j] = from[j];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n + j < Q.R) to[j] = v[k][j];
         }
       }
-    } else if (full) {
-      float v[RI][8], col[8];
+    }
+    return;
+  }
+  float bias[8] = {}, col[8], xs[(WROWS + 63) / 64];
+  if (full && e.bias) load_f32<8>(e.bias + n, bias);
+  if (e.xs) {
+    if (full) load_f32<8>(e.wsc + n, col);
 #pragma unroll
-      for (int k = 0; k < RI; ++k) load_f32<8>(rows + RPI * k * LD, v[k]);
-      float bias[8] = {};
-      if (e.bias) load_f32<8>(e.bias + n, bias);
-      if (e.xs) {
-        load_f32<8>(e.wsc + n, col);
+    for (int k = 0; k < (WROWS + 63) / 64; ++k) xs[k] = e.xs[min(m0 + wm + 64 * k + lane, (long)P.R - 1)];
+  }
+  const int left = (int)min((long)WROWS, P.R - mrow);   // rows from the lane's first one on
+#pragma unroll 1
+  for (int i = 0; i < HALVES; ++i) {
+    if (e.res && i % burst == 0) fetch(i);
+    exchange(i);
+    if (e.xs) {
+      if (i % 4 == 0 && i > 0) xs[0] = xs[(WROWS - 1) / 64];
 #pragma unroll
-        for (int k = 0; k < RI; ++k)
+      for (int k = 0; k < RI; ++k) {
+        const float s = __shfl(xs[0], (16 * i + RPI * k + lr) & 63);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] = fma_(v[k][j] * xs[k], col[j], bias[j]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < RI; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] += bias[j];
+        for (int j = 0; j < 8; ++j) v[k][j] = fma_(v[k][j] * s, col[j], bias[j]);
       }
-      if (e.z)
+    } else {
+#pragma unroll
+      for (int k = 0; k < RI; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] += bias[j];
+    }
+    if (e.res && i % burst == 0) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // the burst has landed
+      asm volatile("" ::: "memory");
+    }
+    if (full) {
+      if (e.z) {
+        __bf16* to = e.z + (mrow + 16 * i) * e.ldz + n;
 #pragma unroll
         for (int k = 0; k < RI; ++k)
-          if (mrow + 16 * i + RPI * k < P.R) store_bf16<8>(e.z + (mrow + 16 * i + RPI * k) * e.ldz + n, v[k]);
+          if (16 * i + RPI * k < left) store_bf16<8>(to + RPI * k * e.ldz, v[k]);
+      }
 #define DD_ACT_CASE(A_)                          \
   case A_:                                       \
     _Pragma("unroll") for (int k = 0; k < RI; ++k) { \
@@ -568,38 +600,59 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_tile(Mat P, Mat Q, i
     break;
       switch (e.act) { DD_ACT_CASE(DD_ACT_ELU) DD_ACT_CASE(DD_ACT_SILU) DD_ACT_CASE(DD_ACT_GELU) }
 #undef DD_ACT_CASE
+      if (e.res) {
+        const char* r = mine + OUT + ((16 * (i % burst) + lr) * W + nc) * es;
 #pragma unroll
-      for (int k = 0; k < RI; ++k) {
-        const long m = mrow + 16 * i + RPI * k;
-        if (m >= P.R) continue;
-        if (e.res) {
-          if (e.ytype == DD_F32) {
-            const f32x4 a = __builtin_bit_cast(f32x4, res[k][0]), b = __builtin_bit_cast(f32x4, res[k][1]);
+        for (int k = 0; k < RI; ++k) {
+          float t[8];
+          if (e.ytype == DD_F32) load_f32<8>((const float*)r + RPI * k * W, t);
+          else load_bf16<8>((const __bf16*)r + RPI * k * W, t);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[k][j] += a[j]; v[k][4 + j] += b[j]; }
-          } else {
-            const bf16x8 a = __builtin_bit_cast(bf16x8, res[k][0]);
+          for (int j = 0; j < 8; ++j) v[k][j] += t[j];
+        }
+      }
+      if (e.ytype == DD_F32) {
+        float* to = (float*)e.y + (mrow + 16 * i) * e.ldy + n;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[k][j] += (float)a[j];
+        for (int k = 0; k < RI; ++k, to += RPI * e.ldy) {
+          if (16 * i + RPI * k >= left) continue;
+          if (e.accumulate) {
+            float o[8];
+            load_f32<8>(to, o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] += o[j];
           }
+          store_f32<8>(to, v[k]);
         }
-        if (e.accumulate) {
-          float o[8];
-          if (e.ytype == DD_F32) load_f32<8>((const float*)e.y + m * e.ldy + n, o);
-          else load_bf16<8>((const __bf16*)e.y + m * e.ldy + n, o);
+      } else {
+        __bf16* to = (__bf16*)e.y + (mrow + 16 * i) * e.ldy + n;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] += o[j];
+        for (int k = 0; k < RI; ++k, to += RPI * e.ldy) {
+          if (16 * i + RPI * k >= left) continue;
+          if (e.accumulate) {
+            float o[8];
+            load_bf16<8>(to, o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] += o[j];
+          }
+          store_bf16<8>(to, v[k]);
         }
-        if (e.ytype == DD_F32) store_f32<8>((float*)e.y + m * e.ldy + n, v[k]);
-        else store_bf16<8>((__bf16*)e.y + m * e.ldy + n, v[k]);
       }
     } else {
 #pragma unroll 1
       for (int k = 0; k < RI; ++k)
-        if (mrow + 16 * i + RPI * k < P.R)
-          finish_ragged(e, mrow + 16 * i + RPI * k, n, Q.R, rows + RPI * k * LD);
+        if (16 * i + RPI * k < left)
+#pragma unroll 1
+          for (int j = 0; n + j < Q.R; ++j) {
+            float t[1] = {at(lr + RPI * k, (nc + j) / 4)[j & 3]};
+            finish<1>(e, mrow + 16 * i + RPI * k, n + j, t);
+          }
     }
-    if (i + 1 < HALVES) fetch(i + 1);
+    // (the reads of this burst are complete before the next one overwrites it)
+    if (e.res && (i + 1) % burst == 0) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      asm volatile("" ::: "memory");
+    }
   }
 }
 
@@ -812,7 +865,7 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   // to pay for them (about 6 us an operand at 2500 x 1541, against 100 us for the general kernel).
   char* at = (char*)(((uintptr_t)ws + 255) / 256 * 256);
   size_t room = ws && ws_bytes > 512 ? ws_bytes - 256 : 0;
-  if (K > 0 && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
+  if (K > 0 && (!e.res || e.ldr < (1l << 20)) && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
     Mat p = P, q = Q;
     if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
       const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), room);
