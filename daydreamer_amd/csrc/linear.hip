@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
   int rest_p = kend - (int)kb, rest_q = rest_p;   // of the step that is copied next
   // A group: one contraction step of the instruction, all of the wave's rows, or half of them where two register
   // sets of all would not fit.
-  constexpr int H = ES == 2 && MT <= 4 ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
+  constexpr int H = MT % 2 || (ES == 2 && MT <= 4) ? 1 : 2, MH = MT / H, GROUPS = STEPS * H;
   typename I::Op p[2][MH], q[2][NT];
   // one of a group's NT + MH operands
   auto read1 = [&](int at_p, int at_q, int g, int k) {
@@ -784,20 +784,21 @@ inline bool tileable(const Mat& a, bool rc, int es) {
   return (!rc || a.R % 2 == 0) && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
 }
 
-// The two tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and
-// the rest of a tile (start, epilogue) take then, in microseconds (measured: 256 x 256 at 8192^3 and 37500 x
-// 1024 x 2048, 128 x 128 at 37500 x 1024 x 2048).  The large one is faster per output (1430 against 1140
-// TFLOP/s, bf16, 8192^3); the small one fills the chip with fewer rows and wastes less in a last round
-// (2500 x 2048 x 1536: 25 against 36 us).
-struct TileShape { int side, slots; float step, rest; };
-constexpr TileShape SHAPES[] = {{256, 256, 1.38f, 10.f}, {128, 512, 0.96f, 4.5f}};
+// The tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and the
+// rest of a tile (start, epilogue) take then, in microseconds (fitted to bf16 products of 2500 to 37500 rows).
+// 256 x 256 is the fastest per output (1430 against 1140 TFLOP/s of 128 x 128, 8192^3); the small ones fill the
+// chip with fewer rows and waste less in a last round (2500 x 2048 x 1536: 192 x 128 22, 128 x 128 26, 256 x 256
+// 36 us; 2500 x 1024 x 1024: 13.5, 12.4, 21).  192 rows are for P by rows: the transposing reads' swizzle
+// wants a power of two.
+struct TileShape { int rows, cols, slots; float step, rest; };
+constexpr TileShape SHAPES[] = {{256, 256, 256, 1.38f, 10.f}, {128, 128, 512, 0.96f, 4.5f}, {192, 128, 256, 0.62f, 6.5f}};
 
 struct Plan { int shape, splits; float us; };
-inline Plan plan_product(long M, long N, int ksteps, size_t slab_room) {
+inline Plan plan_product(long M, long N, int ksteps, size_t slab_room, int shapes) {
   Plan best{0, 1, 1e30f};
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < shapes; ++i) {
     const TileShape& t = SHAPES[i];
-    const long tiles = ((M + t.side - 1) / t.side) * ((N + t.side - 1) / t.side);
+    const long tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
     for (int s = 1; s <= 16 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
       if (s > 1 && sizeof(float) * (size_t)(M * N) * s > slab_room) break;
       const long wgs = tiles * s, full = wgs / t.slots, left = wgs % t.slots;
@@ -851,6 +852,46 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
 }
 
 template <int ES, bool P_RC, bool Q_RC>
+int planned(const char* who, const Mat& P, const Mat& Q, int K, const Plan& plan, const Epi& e, float* slabs, hipStream_t st) {
+  if constexpr (!P_RC)
+    if (plan.shape == 2) return tiled<ES, P_RC, Q_RC, 192, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
+  if (plan.shape == 1) return tiled<ES, P_RC, Q_RC, 128, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
+  return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, P, Q, K, plan.splits, e, slabs, st);
+}
+// The tiled products.  Where the last round of tiles would leave most of the chip idle, whole rounds take
+// the first rows and a launch of its own, with a plan of its own, the rest (37500 x 1024 x 2048, 2.3 rounds:
+// bf16 166 -> 161, e4m3 102 -> 94 us; its dx 150 -> 138).
+template <int ES, bool P_RC, bool Q_RC>
+int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, size_t room, hipStream_t st) {
+  const int ksteps = dd_ceil_div(K, ROWB / ES), shapes = P_RC ? 2 : 3;
+  Plan all = plan_product(P.R, Q.R, ksteps, room, shapes), head{}, tail{};
+  long cut = 0;
+  float best = 0.95f * all.us;
+  for (int i = 0; i < shapes; ++i) {
+    const TileShape& t = SHAPES[i];
+    const long tm = dd_ceil_div(P.R, t.rows), tn = dd_ceil_div(Q.R, t.cols), full = tm * tn / t.slots;
+    const long rows = full * t.slots / tn * t.rows;   // of whole rounds
+    if (full == 0 || rows == 0 || rows >= P.R) continue;
+    const Plan rest = plan_product(P.R - rows, Q.R, ksteps, room, shapes);
+    const float us = full * (t.step * ksteps + t.rest) + rest.us + 2.f;
+    if (us < best) { best = us; cut = rows; head = {i, 1, us}; tail = rest; }
+  }
+  if (cut == 0) return planned<ES, P_RC, Q_RC>(who, P, Q, K, all, e, slabs, st);
+  Mat p = P;
+  p.R = (int)cut;
+  if (const int rc = planned<ES, P_RC, Q_RC>(who, p, Q, K, head, e, slabs, st)) return rc;
+  p.p = (const char*)P.p + (P_RC ? cut : cut * P.ld) * ES;
+  p.R = P.R - (int)cut;
+  Epi f = e;
+  const long es = e.ytype == DD_F32 ? 4 : 2;
+  f.y = (char*)e.y + cut * e.ldy * es;
+  if (e.res) f.res = (const char*)e.res + cut * e.ldr * es;
+  if (e.z) f.z = e.z + cut * e.ldz;
+  if (e.xs) f.xs = e.xs + cut;
+  return planned<ES, P_RC, Q_RC>(who, p, Q, K, tail, f, slabs, st);
+}
+
+template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
   if constexpr (!P_RC && !Q_RC)
     if (P.R <= 64 && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
@@ -867,11 +908,8 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   size_t room = ws && ws_bytes > 512 ? ws_bytes - 256 : 0;
   if (K > 0 && (!e.res || e.ldr < (1l << 20)) && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
     Mat p = P, q = Q;
-    if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st)) {
-      const Plan plan = plan_product(P.R, Q.R, dd_ceil_div(K, ROWB / ES), room);
-      if (plan.shape == 0) return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
-      return tiled<ES, P_RC, Q_RC, 128, 128, 2, 4>(who, p, q, K, plan.splits, e, (float*)at, st);
-    }
+    if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st))
+      return rounds<ES, P_RC, Q_RC>(who, p, q, K, e, (float*)at, room, st);
   }
   const int bk = ROWB / ES;
   const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));
