@@ -120,6 +120,13 @@ struct Args {
   }
 };
 
+// What is written is none of these operands, whose elements other workgroups read later.  (Views of one buffer
+// that overlap in another way look like the columns of one product, side by side, and are not told apart.)
+void apart(const void* out, const char* what, std::initializer_list<const void*> operands) {
+  for (const void* p : operands)
+    if (out && p == out) refuse("%s is one of the other operands", what);
+}
+
 template <typename F>
 void call(const char* name, F&& f) {
   int rc;
@@ -162,6 +169,7 @@ void rms_norm_fwd(const Args& a) {
   if ((y.type == DD_E4M3) != a.given(6)) refuse("scale goes with an e4m3 y, and only with it");
   const float eps = a.real(7);
   if (rows == 0) return;
+  apart(y.p, "y", {x.p, r.p, s.p});
   call("dd_rms_norm_fwd", [&] {
     return dd_rms_norm_fwd_(x.p, x.ld, x.type, r.p, r.ld, rt, s.p, s.ld, gamma, y.p, y.ld, y.type, rstd, scale, (int)rows, (int)C,
                             eps, a.stream);
@@ -176,6 +184,8 @@ void rms_norm_bwd(const Args& a) {
              dr = a.view(6, "dres", rows, C, s.mask(), true);
   const float *rstd = (const float*)a.flat(2, "rstd", rows, F32, false), *gamma = (const float*)a.flat(3, "gamma", C, F32, false);
   float* dgamma = (float*)a.flat(5, "dgamma", C);
+  apart(ds.p, "ds", {dy.p, s.p});
+  apart(dgamma, "dgamma", {gamma, rstd});
   const int accumulate = (int)a.number(7);
   float* ws = (float*)a.number(8);
   const size_t bytes = (size_t)a.number(9);
@@ -209,6 +219,8 @@ void linear_fwd(const Args& a) {
   float* ws = (float*)a.number(9);
   const size_t bytes = (size_t)a.number(10);
   if (M == 0) return;
+  apart(y.p, "y", {x.p, w.p, z.p, bias});
+  apart(z.p, "z", {x.p, w.p, r.p});
   call("dd_linear_fwd", [&] {
     return dd_linear_fwd_(x.p, x.ld, w.p, w.ld, x.type, xs, wsc, bias, act, r.p, r.ld, y.p, y.ld, y.type, z.p, z.ld, (int)M,
                           (int)N, (int)K, ws, bytes, a.stream);
@@ -230,6 +242,9 @@ void linear_bwd(const Args& a) {
   const int accumulate = (int)a.number(9);
   float* ws = (float*)a.number(10);
   const size_t bytes = (size_t)a.number(11);
+  apart(dz.p == dy.p ? nullptr : dz.p, "dz", {x.p, w.p});
+  apart(dx.p, "dx", {dy.p, dz.p, x.p, w.p, dw.p, db});   // (x: dw reads it behind dx)
+  apart(dw.p, "dw", {dy.p, dz.p, x.p, w.p, db});
   if (act != DD_ACT_NONE || db)
     call("dd_linear_act_bwd", [&] {
       return dd_linear_act_bwd_(dy.p, dy.ld, z.p, z.ld, act, dz.p, dz.ld, db, bias_type, accumulate, (int)M, (int)N, ws, bytes, a.stream);
@@ -280,6 +295,7 @@ void gated_scan_fwd(const Args& a) {
   const View h = a.view(2, "h", s.rows, s.D, s.u.mask());
   const float* h0 = (const float*)a.flat(6, "h0", s.B * s.D);
   float* hT = (float*)a.flat(7, "hT", s.B * s.D);
+  apart(h.p, "h", {s.u.p, s.c.p, s.i.p, h0, hT});
   float* ws = (float*)a.number(10);
   const size_t bytes = (size_t)a.number(11);
   call("dd_gated_scan_fwd", [&] {
@@ -297,6 +313,10 @@ void gated_scan_bwd(const Args& a) {
   if (a.given(7) != a.given(8)) refuse("di goes with i, and only with it");
   const float *h0 = (const float*)a.flat(10, "h0", s.B * s.D), *dhT = (const float*)a.flat(11, "dhT", s.B * s.D);
   float* dh0 = (float*)a.flat(12, "dh0", s.B * s.D);
+  apart(du.p, "du", {dh.p, s.u.p, s.c.p, s.i.p, h.p, dc.p, di.p});
+  apart(dc.p, "dc", {dh.p, s.u.p, s.c.p, s.i.p, h.p, di.p});
+  apart(di.p, "di", {dh.p, s.u.p, s.c.p, s.i.p, h.p});
+  apart(dh0, "dh0", {h0});
   float* ws = (float*)a.number(15);
   const size_t bytes = (size_t)a.number(16);
   call("dd_gated_scan_bwd", [&] {

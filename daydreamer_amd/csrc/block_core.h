@@ -6,27 +6,10 @@
 
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // largest finite e4m3 value
 constexpr float E4M3_MAX = 448.0f;
-
-inline int dtype_size(int t) { return t == DD_F32 ? 4 : t == DD_BF16 ? 2 : 1; }
-
-// Is every row of the [*, cols] view (p, ld) aligned to `bytes`?
-inline bool rows_aligned(const void* p, long ld, int type, int bytes) {
-  return p == nullptr || ((uintptr_t)p % bytes == 0 && (ld * dtype_size(type)) % bytes == 0);
-}
-
-// The first and one-past-the-last byte of a [rows, cols] view; do two of them overlap?
-struct Span { uintptr_t lo, hi; };
-inline Span span_of(const void* p, long rows, long ld, long cols, int type) {
-  if (p == nullptr || rows <= 0 || cols <= 0) return {0, 0};
-  return {(uintptr_t)p, (uintptr_t)p + (uintptr_t)(((rows - 1) * ld + cols) * dtype_size(type))};
-}
-inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
 
 // V consecutive elements as floats, and back.  The accesses are as wide as V allows whatever the address:
 // global memory takes 16-byte accesses at any alignment of the element, so that rows of 1542 bf16 need

@@ -96,10 +96,10 @@ __device__ __forceinline__ unsigned restarts(const ScanArgs& p, long b, int o0, 
   return (unsigned)__ballot(r);
 }
 
-// The pairs (a, b) of a run of up to STEPS steps in scan order, identity past n, zero a at restarts.
-// Forward b = gate phi(c); backward b = a dh.  z, q as in gates (backward keeps them).
+// A run of up to STEPS steps in scan order (the last one repeated past n), restarts aside: z, q as in gates and
+// b = gate phi(c) (forward) or dh (backward).
 template <typename E, int VC, bool GATE, bool BWD>
-__device__ __forceinline__ void run_pairs(const ScanArgs& p, long b, int o0, int n, unsigned cut, int d, float z[STEPS][VC],
+__device__ __forceinline__ void run_pairs(const ScanArgs& p, long b, int o0, int n, int d, float z[STEPS][VC],
                                           float q[STEPS][VC], float bb[STEPS][VC]) {
   constexpr bool LOW = sizeof(E) == 2;
   float u[STEPS][VC], c[STEPS][VC], i[STEPS][VC];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_pairs(ScanArgs p) {
     const int o0 = k * p.span + wave * len + s;
     float z[STEPS][VC], q[STEPS][VC], bb[STEPS][VC], a2[VC], b2[VC];
     const unsigned cut = restarts<BWD>(p, b, o0, STEPS, lane);
-    run_pairs<E, VC, GATE, BWD>(p, b, o0, STEPS, cut, d, z, q, bb);
+    run_pairs<E, VC, GATE, BWD>(p, b, o0, STEPS, d, z, q, bb);
     run_total<VC, BWD>(STEPS, cut, q, bb, a2, b2);
 #pragma unroll
     for (int j = 0; j < VC; ++j) compose(A[j], Bv[j], a2[j], b2[j]);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_fwd(ScanArgs p) {
 #pragma unroll
     for (int j = 0; j < VC; ++j) { A[j] = 1.f; Bv[j] = 0.f; }
     if (n > 0) {
-      run_pairs<E, VC, GATE, false>(p, b, o0, n, cut, d, z, q, bb);
+      run_pairs<E, VC, GATE, false>(p, b, o0, n, d, z, q, bb);
       run_total<VC, false>(n, cut, q, bb, A, Bv);
     }
     exchange<VC>(sh[buf], wave, waves, lane, A, Bv, x, in);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
 #pragma unroll
           for (int j = 0; j < VC; ++j) hp[s][j] = s == n - 1 ? first[j] : hp[s][j];
       }
-      run_pairs<E, VC, GATE, true>(p, b, o0, n, cut, d, z, q, dh);
+      run_pairs<E, VC, GATE, true>(p, b, o0, n, d, z, q, dh);
       run_total<VC, true>(n, cut, q, dh, A, Bv);
     }
     exchange<VC>(sh[buf], wave, waves, lane, A, Bv, x, in);

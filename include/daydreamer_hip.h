@@ -250,7 +250,8 @@ int dd_gru_cell_bwd(const float* dhn, long lddn, const float* z3, long ldz,
  * residual stream, a product with its epilogue, the gated scan.  The counterparts on the RSSM path
  * are dd_ln_act_fwd (nets.py:585-602), dd_gemm_f32 (nets.py:573) and dd_gru_cell_fwd
  * (nets.py:149-160).  Storage types are given per operand; arithmetic, sums and states are fp32.
- * `void*` operands are row-major views [rows, cols] with a leading dimension in ELEMENTS. */
+ * `void*` operands are row-major views [rows, cols] with a leading dimension in ELEMENTS, at any alignment
+ * of the element.  What is written overlaps no other operand, except where a line below says so. */
 #define DD_F32 0
 #define DD_BF16 1
 #define DD_E4M3 2   /* OCP float8 e4m3 (no infinities, largest value 448) */
@@ -269,7 +270,7 @@ int dd_rms_norm_fwd(const void* x, long ldx, int x_type, const void* res, long l
                     float* rstd, float* scale, int rows, int C, float eps, void* stream);
 /* ds = dres + d y / d s applied to dy: the gradient of x AND of res (dres, ds in res_type; dres may be
  * NULL, ds may be dres itself).  dgamma (NULL ok) = or += (accumulate) sum over rows; partial sums of
- * up to 1024 workgroups in ws (rows * C or 1024 * C floats, whichever is less), added in a fixed order. */
+ * up to 1536 workgroups in ws (rows * C or 1536 * C floats, whichever is less), added in a fixed order. */
 int dd_rms_norm_bwd(const void* dy, long ldy, int y_type, const void* s, long lds, int res_type,
                     const float* rstd, const float* gamma, const void* dres, long ldr, void* ds, long ldd,
                     float* dgamma, int accumulate, int rows, int C, float* ws, size_t ws_bytes, void* stream);

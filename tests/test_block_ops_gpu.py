@@ -142,6 +142,24 @@ def test_norm_rows_do_not_mix(hip):
   assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[4, 1541])) and bool((y[6] == 0).all())
 
 
+@pytest.mark.parametrize('C', [1024, 1542, 4099, 16389])
+@pytest.mark.parametrize('rt', [F32, BF16])
+def test_norm_in_place_at_any_width(hip, C, rt):
+  """s over res and ds over dres give what separate outputs give: no wave of a row reads what another wrote."""
+  rows = 37
+  x, r, dy, dres = (rnd(rows, C, seed=k, dtype=t).cuda() for k, t in [(1, BF16), (2, rt), (3, BF16), (4, rt)])
+  g = (1 + rnd(C, seed=5, scale=0.1)).cuda()
+  y, y2, s, ds = (torch.zeros(rows, C, device='cuda', dtype=t) for t in (BF16, BF16, rt, rt))
+  rstd, rstd2 = torch.zeros(rows, device='cuda'), torch.zeros(rows, device='cuda')
+  hip.rms_norm_fwd(x, g, y, rstd=rstd, res=r, s=s)
+  stream = r.clone()
+  hip.rms_norm_fwd(x, g, y2, rstd=rstd2, res=stream, s=stream)
+  assert torch.equal(stream, s) and torch.equal(y2, y) and torch.equal(rstd2, rstd)
+  hip.rms_norm_bwd(dy, s, rstd, g, ds, None, dres)
+  hip.rms_norm_bwd(dy, s, rstd, g, dres, None, dres)
+  assert torch.equal(dres, ds)
+
+
 # ---- product --------------------------------------------------------------------------------------
 
 LINEAR_SHAPES = [(1300, 301, 1031), (20, 70, 1031), (50, 40, 4100), (1300, 1030, 520), (2500, 520, 1542), (130, 2048, 1544), (5000, 1024, 72), (257, 129, 8200), (1, 1, 1), (1, 64, 512), (3, 5, 7), (8, 2048, 1024), (17, 130, 40), (33, 96, 1542), (64, 64, 64), (65, 65, 65),
@@ -232,6 +250,62 @@ def test_linear_residual_in_place_and_rows_do_not_mix(hip):
   hip.linear_fwd(x, w, y2, res=r)
   keep = [i for i in range(70) if i not in (3, 40)]
   assert torch.equal(y2[keep], y[keep]) and bool(torch.isnan(y2[3]).all()) and not bool(torch.isfinite(y2[40]).any())
+
+
+@pytest.mark.parametrize('act,yt', [('gelu', BF16), ('silu', F32)])
+@pytest.mark.parametrize('M,N,K', [(3001, 1541, 453), (10001, 2049, 517), (33001, 260, 1542)])
+def test_linear_many_tiles(hip, ref, M, N, K, act, yt):
+  """Products of more than one round of tiles, whose last rows may run in another launch and tile shape."""
+  test_linear(hip, ref, M, N, K, act, yt)
+
+
+@pytest.mark.parametrize('M,N,K', [(3001, 453, 1541), (517, 7751, 2050)])
+def test_linear_gradients_many_tiles(hip, ref, M, N, K):
+  test_linear_gradients(hip, ref, M, N, K, 'silu', F32)
+
+
+def test_linear_e4m3_many_tiles(hip, ref):
+  test_linear_e4m3(hip, ref, 16501, 1030, 1040, 'silu')
+
+
+@pytest.mark.parametrize('M', [3, 70, 300])
+@pytest.mark.parametrize('act', ['elu', 'silu', 'gelu'])
+def test_activations_at_extremes(hip, ref, M, act):
+  """Arguments from the smallest to the largest, and NaN, in every variant of the epilogue (few rows, tiles, and
+  a contraction of one element)."""
+  N = 24
+  z = torch.tensor([0.0, 1e-30, -1e-30, 0.25, -0.25, -0.3125, 5.0, -5.0, 20.0, -20.0, 88.0, -88.0, 1e4, -1e4, 3e38, -3e38]).to(BF16)
+  w = torch.cat([z, z[:8]])[:, None].cuda()
+  x = torch.ones(M, 1, device='cuda', dtype=BF16)
+  y = torch.zeros(M, N, device='cuda')
+  hip.linear_fwd(x, w, y, act=act)
+  zz = w.cpu().double().t().expand(M, N)
+  want = ref._act(zz, act)[0]
+  within(y, want, 16 * U * zz.abs(), act)
+  x[1] = float('nan')
+  hip.linear_fwd(x, w, y, act=act)
+  assert bool(torch.isnan(y[1]).all()) and bool(torch.isfinite(y[0]).all()) and bool(torch.isfinite(y[2]).all())
+
+
+@pytest.mark.parametrize('ld', [(1 << 20) - 6, (1 << 23) + 2])
+def test_linear_rows_far_apart(hip, ld):
+  """Operands and outputs whose rows are megabytes apart (offsets past 2^31 elements and 2^32 bytes), in the tiled
+  and in the general kernel: the results of compact ones."""
+  M, N, K = (5000 if ld < 1 << 22 else 300), 40, 64
+  far = [torch.empty(M, ld, device='cuda', dtype=BF16) for _ in range(2)]
+  assert far[0].numel() > 1 << 31
+  x, w, r = rnd(M, K, seed=1, dtype=BF16), rnd(N, K, seed=2, dtype=BF16), rnd(M, N, seed=3, dtype=BF16)
+  xs, ys, zs, rs = far[0][:, 5:5 + K], far[1][:, 3:3 + N], far[1][:, 100:100 + N], far[0][:, 200:200 + N]
+  xs.copy_(x), rs.copy_(r)
+  hip.linear_fwd(xs, w.cuda(), ys, res=rs, z=zs)
+  want = x.double() @ w.double().t()
+  err = dot_error(x, w, K)
+  within(zs, want, err, 'z')
+  within(ys, want + r.double(), err + 2 * U * (want.abs() + r.double().abs()), 'y')
+  dx, dw = far[1][:, 300:300 + K], torch.zeros(N, K, device='cuda')
+  hip.linear_bwd(rs, xs, w.cuda(), dx=dx, dw=dw)
+  within(dx, r.double() @ w.double(), dot_error(r, w.t(), N), 'dx')
+  within(dw, r.double().t() @ x.double(), dot_error(r.t(), x.t(), M), 'dw')
 
 
 def test_linear_ragged_columns_hold_anything(hip):
@@ -424,6 +498,29 @@ def test_scan_saturated_gates(hip, ref):
     within(h, want, 256 * U * 4.0, f'gate {v}')
 
 
+def test_norm_and_scan_rows_far_apart(hip):
+  """Offsets past 2^31 elements and 2^32 bytes: bit for bit the results of compact operands."""
+  ld, R, C, T = (1 << 20) + 6, 4200, 40, 2100
+  far = [torch.empty(R, ld, device='cuda', dtype=BF16) for _ in range(2)]
+  assert far[0].numel() > 1 << 31
+  near = [rnd(R, C, seed=k, dtype=BF16).cuda() for k in range(4)]
+  src = [far[0][:, 50 * k + 1:50 * k + 1 + C] for k in range(4)]
+  for a, b in zip(src, near):
+    a.copy_(b)
+  dst = [far[1][:, 50 * k + 1:50 * k + 1 + C] for k in range(4)]
+  out = [torch.empty(R, C, device='cuda', dtype=BF16) for _ in range(4)]
+  g = torch.ones(C, device='cuda')
+  rstd = [torch.empty(R, device='cuda') for _ in range(2)]
+  for (x, r, dy, dr), (y, s, ds, _), inv in ((src, dst, rstd[0]), (near, out, rstd[1])):
+    hip.rms_norm_fwd(x, g, y, rstd=inv, res=r, s=s)
+    hip.rms_norm_bwd(dy, s, inv, g, ds, None, dr)
+  assert torch.equal(rstd[0], rstd[1]) and all(torch.equal(a, b) for a, b in zip(dst[:3], out[:3]))
+  for (u, c, i, dh), (h, du, dc, di) in ((src, dst), (near, out)):
+    hip.gated_scan_fwd(u, c, h, T, i=i)
+    hip.gated_scan_bwd(dh, u, c, h, du, dc, T, i=i, di=di)
+  assert all(torch.equal(a, b) for a, b in zip(dst, out))
+
+
 # ---- together -------------------------------------------------------------------------------------
 
 
@@ -547,6 +644,43 @@ def test_block_replays_from_a_graph(hip):
   assert lib.dd_graph_destroy(ex) == 0
 
 
+def test_two_graphs_replay_at_once(hip):
+  """Two captured blocks (a split scan and split products among their launches) with a HipOps, that is a
+  workspace, each, replayed at the same time on two streams with eager work between: the eager results."""
+  from daydreamer_amd import graphs, hipops
+  B, T, C, D = 1, 2000, 128, 64
+  lib, runs = hip.lib, []
+  for n in range(2):
+    ops = hipops.HipOps('cuda:0')
+    blk = Block(ops, B, T, C, D, seed=7 * n)
+    x, res, dout = rnd(B * T, C, seed=2 + n, dtype=BF16).cuda(), rnd(B * T, C, seed=3 + n).cuda(), rnd(B * T, C, seed=4 + n, dtype=BF16).cuda()
+    first = restarts(B, T, 0.01, n).cuda()
+    blk.forward(x, res, first)
+    blk.backward(dout, first)
+    torch.cuda.synchronize()
+    st, ex, nodes = graphs.stream('cuda:0', f'block-test-{n}'), ctypes.c_void_p(), ctypes.c_int()
+    with torch.cuda.stream(st):
+      assert lib.dd_graph_capture_begin(st.cuda_stream) == 0
+      blk.forward(x, res, first)
+      blk.backward(dout, first)
+      assert lib.dd_graph_capture_end(st.cuda_stream, ctypes.byref(ex), ctypes.byref(nodes)) == 0, lib.dd_last_error()
+    runs.append((blk, x, res, dout, first, st, ex, Block(hip, B, T, C, D, seed=7 * n)))
+  for k in range(3):
+    for n, (blk, x, res, dout, first, st, ex, eager) in enumerate(runs):
+      x.copy_(rnd(B * T, C, seed=50 + 2 * k + n, dtype=BF16))
+      eager.forward(x, res, first)
+      eager.backward(dout, first)
+    torch.cuda.synchronize()
+    for run in runs:
+      assert lib.dd_graph_launch(run[6], run[5].cuda_stream) == 0
+    torch.cuda.synchronize()
+    for blk, eager in ((run[0], run[7]) for run in runs):
+      for a, b in [(blk.out, eager.out), (blk.hT, eager.hT), (blk.dstream, eager.dstream)] + [(blk.grads[m], eager.grads[m]) for m in blk.grads]:
+        assert torch.equal(a, b), k
+  for run in runs:
+    assert lib.dd_graph_destroy(run[6]) == 0
+
+
 def test_block_on_another_stream(hip):
   """The operators run on the stream that is current, in its order."""
   B, T, C, D = 2, 50, 128, 64
@@ -608,3 +742,48 @@ def test_binding_refusals(hip):
     with pytest.raises((AssertionError, RuntimeError, KeyError)):
       call()
       pytest.fail(f'call {k} was not refused')
+
+
+def test_outputs_are_no_other_operands(hip):
+  """Written over an operand that other workgroups still read, a result would depend on their order: refused."""
+  x, w, y = torch.zeros(16, 16, device='cuda', dtype=BF16), torch.zeros(16, 16, device='cuda', dtype=BF16), torch.zeros(16, 16, device='cuda', dtype=BF16)
+  a, b, g, r = torch.zeros(16, 16, device='cuda', dtype=BF16), torch.zeros(16, 16, device='cuda', dtype=BF16), torch.ones(16, device='cuda'), torch.ones(16, device='cuda')
+  s0 = torch.zeros(4, 16, device='cuda')
+  calls = [
+      lambda: hip.linear_fwd(x, w, x),
+      lambda: hip.linear_fwd(x, w, w),
+      lambda: hip.linear_fwd(x, w, y, z=y),
+      lambda: hip.linear_fwd(x, w, y, res=a, z=a),
+      lambda: hip.linear_bwd(y, x, w, dx=x),
+      lambda: hip.linear_bwd(y, x, w, dx=y),
+      lambda: hip.linear_bwd(y, x, w, dw=w),
+      lambda: hip.linear_bwd(y, x, w, act='silu', z=a, dz=x),
+      lambda: hip.rms_norm_fwd(x, g, x),
+      lambda: hip.rms_norm_bwd(y, x, r, g, x),
+      lambda: hip.gated_scan_fwd(x, w, x, 4),
+      lambda: hip.gated_scan_fwd(x, w, w, 4),
+      lambda: hip.gated_scan_bwd(y, x, w, a, y, b, 4),
+      lambda: hip.gated_scan_bwd(y, x, w, a, b, b, 4),
+      lambda: hip.gated_scan_bwd(y, x, w, a, b, a, 4),
+      lambda: hip.gated_scan_bwd(y, x, w, a, b, torch.zeros_like(b), 4, h0=s0, dh0=s0),
+  ]
+  for k, call in enumerate(calls):
+    with pytest.raises(AssertionError):
+      call()
+      pytest.fail(f'call {k} was not refused')
+
+
+def test_calls_without_rows(hip):
+  """No rows: nothing is read, gradients of parameters are zero, or unchanged where they accumulate."""
+  e = lambda n, t=BF16: torch.zeros(0, n, device='cuda', dtype=t)  # noqa: E731
+  w, g, none = torch.ones(8, 16, device='cuda', dtype=BF16), torch.ones(16, device='cuda'), torch.zeros(0, device='cuda')
+  hip.linear_fwd(e(16), w, e(8))
+  hip.rms_norm_fwd(e(16), g, e(16), rstd=none)
+  hip.quant_rows(e(16), e(16, FP8), none)
+  hip.gated_scan_fwd(e(16), e(16), e(16), 4)
+  for keep in (False, True):
+    dw, db, dg = torch.full((8, 16), 3.0, device='cuda'), torch.full((8,), 3.0, device='cuda'), torch.full((16,), 3.0, device='cuda')
+    hip.linear_bwd(e(8), e(16), w, dx=e(16), dw=dw, dbias=db, accumulate=keep)
+    hip.rms_norm_bwd(e(16), e(16), none, g, e(16), dg, accumulate=keep)
+    want = 3.0 if keep else 0.0
+    assert all(bool((t == want).all()) for t in (dw, db, dg))
