@@ -93,18 +93,24 @@ __device__ __forceinline__ void finish_ragged(const Epi& e, long m, long n, long
 struct Mat { const void* p; long ld; int R; };
 typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(1)));   // 16 bytes at any address
 
-// The first n (fewer than a chunk's) elements at p, zeros behind.
+// The first n (at least one, fewer than a chunk's) elements at p, zeros behind: 8 + 4 + 2 + 1 bytes, in flight
+// together.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <int ES>
 __device__ __forceinline__ i32x4 partial_chunk(const char* p, int n) {
-  unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16 / ES; ++j)
-    if (j < n) {
-      if constexpr (ES == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
-      else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
-    }
-  return i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+  n = __builtin_amdgcn_readfirstlane(n) * ES;   // (the same for all rows)
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+  typedef unsigned u32 __attribute__((aligned(1)));
+  typedef unsigned short u16 __attribute__((aligned(1)));
+  u32x2 a = {0, 0};
+  unsigned b = 0, c = 0, d = 0;
+  if (n & 8) a = *reinterpret_cast<const u32x2*>(p);
+  if (n & 4) b = *reinterpret_cast<const u32*>(p + (n & 8));
+  if (n & 2) c = *reinterpret_cast<const u16*>(p + (n & 12));
+  if (ES == 1 && n & 1) d = *reinterpret_cast<const unsigned char*>(p + (n & 14));
+  c |= d << 8 * (n & 2);
+  const i32x4 low = n & 4 ? i32x4{(int)b, (int)c, 0, 0} : i32x4{(int)c, 0, 0, 0};
+  return n & 8 ? i32x4{(int)a.x, (int)a.y, low.x, low.y} : low;
 }
 
 constexpr int ROWB = 128;         // bytes of the contraction per tile row
@@ -124,7 +130,7 @@ __device__ __forceinline__ void stage(const Mat& a, long r0, long k0, int K, cha
       if (r0 + r < a.R) {
         const char* p = (const char*)a.p + ((r0 + r) * a.ld + k0 + kc) * ES;
         if (k0 + kc + PER <= K) __builtin_memcpy(&v, p, 16);
-        else v = partial_chunk<ES>(p, (int)(K - k0 - kc));
+        else if (k0 + kc < K) v = partial_chunk<ES>(p, K % PER);
       }
       *reinterpret_cast<i32x4*>(sh + r * LROW + kc * ES) = v;
     } else {
@@ -212,14 +218,17 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
   }
 }
 
-// Rows -> rows of whole 16-byte chunks, zeros behind; units of T (4 bytes
-// where the rows are aligned for it), `ldo` and `ldi` in units, 32 KB of a row per workgroup and pass.
-template <typename T>
-__global__ void __launch_bounds__(256) k_linear_pack(const T* in, long ldi, int cols, T* out, int ldo) {
-  in += (long)blockIdx.x * ldi;
-  out += (long)blockIdx.x * ldo;
-#pragma unroll 4
-  for (int c = threadIdx.x; c < ldo; c += 256) out[c] = c < cols ? in[c] : (T)0;
+// Rows -> rows of whole 16-byte chunks, zeros behind; a chunk per thread.
+template <int ES>
+__global__ void __launch_bounds__(256) k_linear_pack(const char* in, long ldb, int cols, char* out, unsigned chunks, unsigned total) {
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, row = i / chunks;
+  if (i >= total) return;
+  const int c = (int)(i - row * chunks) * (16 / ES);
+  const char* from = in + row * ldb + (long)c * ES;
+  i32x4 v;
+  if (c + 16 / ES <= cols) v = __builtin_bit_cast(i32x4, *reinterpret_cast<const u32x4u*>(from));
+  else v = partial_chunk<ES>(from, cols % (16 / ES));
+  *reinterpret_cast<i32x4*>(out + i * 16l) = v;
 }
 
 // ---- tiled kernel --------------------------------------------------------------------------------
@@ -491,16 +500,24 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
   float* out = reinterpret_cast<float*>(mine);
   // 16-byte chunk c of row r, permuted by the row so that the writes of 16 rows fall on different banks
   auto at = [&](int r, int c) { return out + r * W + ((c ^ (r & (W / 4 - 1))) << 2); };
-  const int nc = (lane % LPR) * 8;
+  // The lane's 8 columns end where the row ends and overlap its neighbour's (the same values twice) rather than being
+  // cut: element by element they took longer than the product (111 x 2391 x 577 with a residual: 25 us against 13).
+  // Fewer than 8 columns of the wave's: none is full.
+  const int cols = (int)min((long)W, Q.R - (n0 + wn));
+  int nc = (lane % LPR) * 8;
+  const bool shifted = cols >= 8 && nc < cols && nc + 8 > cols;
+  if (shifted) nc = cols - 8;
+  const bool full = nc + 8 <= cols;
   const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
-  const bool full = n + 8 <= Q.R;
   const int es = e.ytype == DD_F32 ? 4 : 2, burst = e.ytype == DD_F32 ? HALVES / 2 : HALVES;
   auto fetch = [&](int i) {   // the residual's rows 16 i .. 16 (i + burst) - 1 of the wave
-    const int rows = (int)min((long)burst * 16, P.R - (m0 + wm + 16 * i)), cols = (int)min((long)W, Q.R - (n0 + wn));
+    const int rows = (int)min((long)burst * 16, P.R - (m0 + wm + 16 * i));
     const unsigned ldb = (unsigned)(e.ldr * es);
     const char* base = (const char*)e.res + ((m0 + wm + 16 * i) * e.ldr + n0 + wn) * es;
+    // an odd row's last bf16 is half of a 4-byte unit: read whole, except at the end of the matrix (below)
+    const unsigned width = cols * es + (m0 + wm + 16 * i + rows < P.R ? cols * es & 2 : 0);
     const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu,
-                      rows > 0 && cols > 0 ? (rows - 1) * ldb + cols * es : 0u, 0x00020000u};
+                      rows > 0 && cols > 0 ? (rows - 1) * ldb + width : 0u, 0x00020000u};
     const unsigned to = lds + wave * (OUT + RES) + OUT, step = 1024 / (W * es) * ldb,
                    v = es == 4 ? lane / (W / 4) * ldb + lane % (W / 4) * 16 : lane / (W / 8) * ldb + lane % (W / 8) * 16;
 #pragma unroll 1
@@ -513,26 +530,37 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
     constexpr int PER = ROWS / 16;   // sixteens of an accumulator block
     // (a bit, not i / PER == k: the compiler would index the accumulators by i, in memory)
     const unsigned which = 1u << i / PER;
+    int l = lane, c = nc;
+    asm volatile("" : "+v"(c));   // these addresses are computed here, not kept across the loop
+    if constexpr (BM * BN <= 16384 || ES == 1) asm volatile("" : "+v"(l));   // (nor these, where registers are short)
+    const int lr = l / LPR;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int k = 0; k < MT; ++k)
-      if (which >> k & 1 && (PER == 1 || (lane % 32) / 16 == i % PER))
+      if (which >> k & 1 && (PER == 1 || (l % 32) / 16 == i % PER))
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int g = 0; g < PER * PER; ++g) {   // 16 x 16: one run of four columns, 32 x 32: four, 8 apart
             const f32x4 t = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
-            *reinterpret_cast<f32x4*>(at(lane % 16, (ROWS * j + 8 * g) / 4 + lane / ROWS)) = t;
+            *reinterpret_cast<f32x4*>(at(l % 16, (ROWS * j + 8 * g) / 4 + l / ROWS)) = t;
           }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int k = 0; k < RI; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(at(lr + RPI * k, nc / 4 + h));
+        const f32x4 t = *reinterpret_cast<const f32x4*>(at(lr + RPI * k, lane % LPR * 2 + h));
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[k][4 * h + j] = t[j];
       }
+    if (cols % 8 != 0 && cols >= 8 && cols < W) {   // (wave-uniform)
+      if (shifted)
+#pragma unroll
+        for (int k = 0; k < RI; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = at(lr + RPI * k, (c + j) / 4)[(c + j) & 3];
+    }
   };
   if (slabs) {
     float* slab = slabs + ((long)split * P.R + mrow) * Q.R + n;
@@ -548,7 +576,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (n + j < Q.R) to[j] = v[k][j];
+            if (nc + j < cols) to[j] = v[k][j];
         }
       }
     }
@@ -562,6 +590,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
     for (int k = 0; k < (WROWS + 63) / 64; ++k) xs[k] = e.xs[min(m0 + wm + 64 * k + lane, (long)P.R - 1)];
   }
   const int left = (int)min((long)WROWS, P.R - mrow);   // rows from the lane's first one on
+  const float corner = shifted && e.res && es == 2 ? (float)((const __bf16*)e.res)[min(mrow + left - 1, (long)P.R - 1) * e.ldr + n + 7] : 0.f;
 #pragma unroll 1
   for (int i = 0; i < HALVES; ++i) {
     if (e.res && i % burst == 0) fetch(i);
@@ -607,6 +636,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
           float t[8];
           if (e.ytype == DD_F32) load_f32<8>((const float*)r + RPI * k * W, t);
           else load_bf16<8>((const __bf16*)r + RPI * k * W, t);
+          if (shifted && es == 2 && 16 * i + RPI * k == left - 1) t[7] = corner;
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[k][j] += t[j];
         }
@@ -638,16 +668,15 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
           store_bf16<8>(to, v[k]);
         }
       }
-    } else {
-#pragma unroll 1
-      for (int k = 0; k < RI; ++k)
-        if (16 * i + RPI * k < left)
-#pragma unroll 1
-          for (int j = 0; n + j < Q.R; ++j) {
-            float t[1] = {at(lr + RPI * k, (nc + j) / 4)[j & 3]};
-            finish<1>(e, mrow + 16 * i + RPI * k, n + j, t);
-          }
     }
+    if (cols > 0 && cols < 8)
+      for (int k = lane; k < 16 * 8; k += 64) {
+        const int r = k / 8, j = k % 8;
+        const long m = m0 + wm + 16 * i + r;
+        if (j >= cols || m >= P.R) continue;
+        float t[1] = {at(r, j / 4)[j & 3]};
+        finish<1>(e, m, n0 + wn + j, t);
+      }
     // (the reads of this burst are complete before the next one overwrites it)
     if (e.res && (i + 1) % burst == 0) {
       __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -743,14 +772,17 @@ __global__ void __launch_bounds__(64 * WV) k_linear_few(Mat P, Mat Q, int K, Epi
   }
 }
 
-// Sum of the partial results of a split contraction, slabs ascending, and the epilogue: eight columns of a
-// row per thread, element by element where the row ends inside them.
+// Sum of the partial results of a split contraction, slabs ascending, and the epilogue: V columns of a row per
+// thread, eight slabs' loads in flight.  Eight columns where that leaves every CU threads; one where the
+// output is small or its rows ragged (64 x 71 of 60 slabs 6 us, of 16 by eight columns 11).
 template <int V>
-__device__ __forceinline__ void sum_and_finish(const float* slabs, int S, long M, long N, long m, long n, const Epi& e) {
-  const long at = m * N + n;
+__global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, unsigned chunks, Epi e) {
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, r = i / chunks;
+  const long m = r, n = (long)(i - r * chunks) * V, at = m * N + n;
+  if (m >= M) return;
   float v[V], t[V];
   load_f32<V>(slabs + at, v);
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 1; s < S; ++s) {
     load_f32<V>(slabs + s * M * N + at, t);
 #pragma unroll
@@ -758,16 +790,13 @@ __device__ __forceinline__ void sum_and_finish(const float* slabs, int S, long M
   }
   finish<V>(e, m, n, v);
 }
-__global__ void __launch_bounds__(256) k_linear_finish(const float* slabs, int S, long M, long N, int chunks, Epi e) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, m = i / chunks, n = i % chunks * 8;
-  if (m >= M) return;
-  if (n + 8 <= N) return sum_and_finish<8>(slabs, S, M, N, m, n, e);
-#pragma unroll 1
-  for (long j = n; j < N; ++j) sum_and_finish<1>(slabs, S, M, N, m, j, e);
-}
-inline void sum_slabs(const float* slabs, int S, long M, long N, const Epi& e, hipStream_t st) {
-  const int chunks = dd_ceil_div(N, 8);
-  k_linear_finish<<<(unsigned)((M * chunks + 255) / 256), 256, 0, st>>>(slabs, S, M, N, chunks, e);
+inline int sum_slabs(const char* who, const float* slabs, int S, long M, long N, const Epi& e, hipStream_t st) {
+  DD_REQUIRE(M * N < (1l << 32) - 256, "dd_linear: a split product of 2^32 outputs");
+  const unsigned per = N % 8 == 0 && M * N >= 8 * 65536 ? 8 : 1, grid = (unsigned)((M * N / per + 255) / 256);
+  if (per == 8) k_linear_finish<8><<<grid, 256, 0, st>>>(slabs, S, M, N, (unsigned)(N / 8), e);
+  else k_linear_finish<1><<<grid, 256, 0, st>>>(slabs, S, M, N, (unsigned)N, e);
+  DD_CHECK_LAUNCH(who);
+  return 0;
 }
 
 // Splits of a contraction: none where the tiles alone fill the chip.
@@ -799,7 +828,7 @@ inline Plan plan_product(long M, long N, int ksteps, size_t slab_room, int shape
   for (int i = 0; i < shapes; ++i) {
     const TileShape& t = SHAPES[i];
     const long tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
-    for (int s = 1; s <= 16 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
+    for (int s = 1; s <= 64 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
       if (s > 1 && sizeof(float) * (size_t)(M * N) * s > slab_room) break;
       const long wgs = tiles * s, full = wgs / t.slots, left = wgs % t.slots;
       const float steps = (float)((ksteps + s - 1) / s);
@@ -821,11 +850,7 @@ int tiled(const char* who, Mat P, Mat Q, int K, int splits, const Epi& e, float*
   k_linear_tile<ES, P_RC, Q_RC, BM, BN, WM, WN><<<(unsigned)((long)tm * tn * parts), 64 * WM * WN, 0, st>>>(
       P, Q, K, kspan, tm, tn, parts > 1 ? slabs : nullptr, e);
   DD_CHECK_LAUNCH(who);
-  if (parts > 1) {
-    sum_slabs(slabs, parts, P.R, Q.R, e, st);
-    DD_CHECK_LAUNCH(who);
-  }
-  return 0;
+  return parts > 1 ? sum_slabs(who, slabs, parts, P.R, Q.R, e, st) : 0;
 }
 
 // The operand with rows that the tiled kernel can read, copied into the workspace unless it has them
@@ -836,14 +861,8 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
   const long rows = rc ? K : a.R;
   const int cols = rc ? a.R : K, chunks = dd_ceil_div(cols, 16 / ES);
   const size_t bytes = ((size_t)rows * chunks * 16 + 255) / 256 * 256;
-  if (bytes > room) return false;
-  const unsigned grid = (unsigned)rows;
-  if ((uintptr_t)a.p % 4 == 0 && a.ld * ES % 4 == 0 && cols * ES % 4 == 0)
-    k_linear_pack<unsigned><<<grid, 256, 0, st>>>((const unsigned*)a.p, a.ld * ES / 4, cols * ES / 4, (unsigned*)ws, chunks * 4);
-  else if (ES == 2)
-    k_linear_pack<unsigned short><<<grid, 256, 0, st>>>((const unsigned short*)a.p, a.ld, cols, (unsigned short*)ws, chunks * 8);
-  else
-    k_linear_pack<unsigned char><<<grid, 256, 0, st>>>((const unsigned char*)a.p, a.ld, cols, (unsigned char*)ws, chunks * 16);
+  if (bytes > room || rows * chunks >= (1l << 32) - 256) return false;
+  k_linear_pack<ES><<<(unsigned)((rows * chunks + 255) / 256), 256, 0, st>>>((const char*)a.p, a.ld * ES, cols, ws, chunks, (unsigned)(rows * chunks));
   a.p = ws;
   a.ld = chunks * (16 / ES);
   ws += bytes;
@@ -919,21 +938,18 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
   k_linear_any<ES, P_RC, Q_RC><<<dim3(tiles.x, tiles.y, parts), 256, 0, st>>>(P, Q, K, kspan, parts > 1 ? ws : nullptr, e);
   DD_CHECK_LAUNCH(who);
-  if (parts > 1) {
-    sum_slabs(ws, parts, P.R, Q.R, e, st);
-    DD_CHECK_LAUNCH(who);
-  }
-  return 0;
+  return parts > 1 ? sum_slabs(who, ws, parts, P.R, Q.R, e, st) : 0;
 }
 
 // dz = dy act'(z), and the workgroup's share of dbias; without an activation dz IS dy and only the column
-// sums are taken.  HBM-bound: 512 columns per workgroup (1 KB of a row in one wave's access), four waves on
-// different rows, four rows requested at a time; the columns of a ragged row's end one by one.
+// sums are taken.  HBM-bound: a wave takes 512 columns of a row at a time (1 KB), or several rows of narrower
+// matrices (`lanes` of it per row: 30237 x 64: 6 us against 14 with whole waves), four waves on different rows, four rows
+// requested at a time; the columns of a ragged row's end one by one.
 template <int V, int ACT>
 __device__ __forceinline__ void act_rows(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz, long c,
-                                         long m0, long m1, float sum[V]) {
+                                         long m0, long m1, int step, float sum[V]) {
 #pragma unroll 4
-  for (long m = m0; m < m1; m += 4) {
+  for (long m = m0; m < m1; m += step) {
     float d[V], t[V];
     load_bf16<V>(dy + m * ldy + c, d);
     if constexpr (ACT != DD_ACT_NONE) {
@@ -949,25 +965,28 @@ __device__ __forceinline__ void act_rows(const __bf16* dy, long ldy, const __bf1
 }
 template <int ACT>
 __global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz,
-                                                 float* parts, int M, int N, int rows_per) {
-  __shared__ float sh[4][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long c = ((long)blockIdx.x * 64 + lane) * 8;
-  const long m0 = (long)blockIdx.y * rows_per + wave, m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
+                                                 float* parts, int M, int N, int rows_per, int lanes) {
+  __shared__ float sh[4 * 512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, apart = 64 / lanes;   // rows of a wave
+  const long c = ((long)blockIdx.x * lanes + lane % lanes) * 8;
+  const long m0 = (long)blockIdx.y * rows_per + wave * apart + lane / lanes, m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
   float sum[8] = {};
-  if (c + 8 <= N) act_rows<8, ACT>(dy, ldy, z, ldz, dz, lddz, c, m0, m1, sum);
+  if (c + 8 <= N) act_rows<8, ACT>(dy, ldy, z, ldz, dz, lddz, c, m0, m1, 4 * apart, sum);
   else
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c + j < N) act_rows<1, ACT>(dy, ldy, z, ldz, dz, lddz, c + j, m0, m1, sum + j);
+      if (c + j < N) act_rows<1, ACT>(dy, ldy, z, ldz, dz, lddz, c + j, m0, m1, 4 * apart, sum + j);
   if (!parts) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sh[wave][lane * 8 + j] = sum[j];
+  for (int j = 0; j < 8; ++j) sh[threadIdx.x * 8 + j] = sum[j];
   __syncthreads();
-#pragma unroll
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const long col = (long)blockIdx.x * 512 + i;
-    if (col < N) parts[(long)blockIdx.y * N + col] = sh[0][i] + sh[1][i] + sh[2][i] + sh[3][i];
+  for (int i = threadIdx.x; i < 8 * lanes; i += 256) {   // waves and their rows in order
+    const long col = (long)blockIdx.x * lanes * 8 + i;
+    if (col >= N) continue;
+    float t = sh[i];
+#pragma unroll 4
+    for (int r = 1; r < 4 * apart; ++r) t += sh[r * lanes * 8 + i];
+    parts[(long)blockIdx.y * N + col] = t;
   }
 }
 
@@ -1032,9 +1051,11 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
   DD_REQUIRE(M == 0 || (dy && ldy >= N), "dd_linear_act_bwd: dy is null or its leading dimension is below N");
   DD_REQUIRE(M == 0 || !act_on || (z && dz && ldz >= N && lddz >= N), "dd_linear_act_bwd: an activation needs z and dz");
   const hipStream_t st = (hipStream_t)stream;
-  // 1024 workgroups, at least four rows each
-  const int cols = dd_ceil_div(N, 512);
-  const int rows_per = max(4, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
+  // 1024 workgroups, at least a row each for every row of lanes
+  int lanes = 64;
+  while (lanes > 1 && N <= 4 * lanes) lanes /= 2;
+  const int cols = dd_ceil_div(N, 8 * lanes);
+  const int rows_per = max(256 / lanes, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
   DD_REQUIRE(n <= 65535, "dd_linear_act_bwd: too many rows");
   DD_REQUIRE(!dbias || ws_bytes / sizeof(float) >= (size_t)n * N, "dd_linear_act_bwd: the workspace is too small");
   if (M > 0) {
@@ -1042,7 +1063,7 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
 #define DD_ACT_BWD(A_)                                                                                          \
   case A_:                                                                                                      \
     k_act_bwd<A_><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz,       \
-                                        dbias ? ws : nullptr, M, N, rows_per);                                  \
+                                        dbias ? ws : nullptr, M, N, rows_per, lanes);                                  \
     break;
     switch (act) { DD_ACT_BWD(DD_ACT_NONE) DD_ACT_BWD(DD_ACT_ELU) DD_ACT_BWD(DD_ACT_SILU) DD_ACT_BWD(DD_ACT_GELU) }
 #undef DD_ACT_BWD
