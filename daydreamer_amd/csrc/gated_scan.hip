@@ -44,6 +44,7 @@ struct ScanArgs {
   float2* pairs;                    // [B][splits][D] of a split time axis
   int B, T, D, groups, splits, span;
   float shift; int tanh_c;
+  int shared_lines;                 // rows are not aligned to cache lines
 };
 
 template <typename E, int VC>
@@ -151,14 +152,28 @@ __device__ __forceinline__ void run_total(int n, unsigned cut, const float q[STE
   }
 }
 
+// This workgroup's sequence, channels and split.  Rows that are not aligned to cache lines: neighbouring channels
+// of the same steps share lines, so they are given to one XCD (consecutive workgroups go to the eight in turn)
+// one after the other and meet in its L2; else the splits of the same channels come first (1 x 24368 x 2367 fp32
+// 774 us backward the second way, 598 the first; 2 x 16385 x 512 144 and 151).
+struct Work { int g, k; long b; };
+__device__ __forceinline__ Work work_of(const ScanArgs& p, int splits) {
+  unsigned id = blockIdx.x;
+  if (!p.shared_lines) return {(int)(id / splits % p.groups), (int)(id % splits), (long)(id / splits / p.groups)};
+  const unsigned q = gridDim.x / 8, r = gridDim.x % 8, xcd = id % 8;
+  id = xcd * q + min(xcd, r) + id / 8;
+  return {(int)(id % p.groups), (int)(id / p.groups % splits), (long)(id / p.groups / splits)};
+}
+
 // First launch of a split time axis: the pairs of all splits but the last (in scan order), and in
 // slot 0 the initial state as a restart, so that a state updated in place is read before it is written.
 template <typename E, int VC, bool GATE, bool BWD>
 __global__ void __launch_bounds__(64 * WAVES) k_scan_pairs(ScanArgs p) {
   __shared__ float2 sh[WAVES][64 * VC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int k = blockIdx.x % (p.splits - 1), g = (blockIdx.x / (p.splits - 1)) % p.groups;
-  const long b = blockIdx.x / (p.splits - 1) / p.groups;
+  const Work w = work_of(p, p.splits - 1);
+  const int k = w.k, g = w.g;
+  const long b = w.b;
   const int d = min((g * 64 + lane) * VC, p.D - VC);
   const bool live = (g * 64 + lane) * VC < p.D;
   const int len = p.span / WAVES;   // this wave's steps, in scan order: a multiple of STEPS; the last split is not here
@@ -180,28 +195,40 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_pairs(ScanArgs p) {
   if (wave == 0 && live)
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      for (int w = 1; w < WAVES; ++w) compose(A[j], Bv[j], sh[w][lane * VC + j].x, sh[w][lane * VC + j].y);
+      for (int o = 1; o < WAVES; ++o) compose(A[j], Bv[j], sh[o][lane * VC + j].x, sh[o][lane * VC + j].y);
       float2* out = p.pairs + b * p.splits * p.D + d + j;
       out[(long)(k + 1) * p.D] = make_float2(A[j], Bv[j]);
       if (k == 0) out[0] = make_float2(0.f, p.x0 ? p.x0[b * p.D + d + j] : 0.f);
     }
 }
 
-// State at the start of split k of (b, d): the initial one, or the composed pairs of what precedes it.
+// State at the start of split k of (b, d): the initial one, or the composed pairs of what precedes it, an equal
+// run of them per wave (64 of them one after the other took a wave 6 us).
 template <int VC>
-__device__ __forceinline__ void start_state(const ScanArgs& p, long b, int k, int d, float x[VC]) {
+__device__ __forceinline__ void start_state(const ScanArgs& p, long b, int k, int d, float2 (*sh)[64 * VC], int wave, int waves,
+                                            int lane, float x[VC]) {
 #pragma unroll
   for (int j = 0; j < VC; ++j) x[j] = 0.f;
   if (p.splits == 1) {
     if (p.x0) load_f32<VC>(p.x0 + b * p.D + d, x);
     return;
   }
+  float A[VC], B[VC];
+#pragma unroll
+  for (int j = 0; j < VC; ++j) { A[j] = 1.f; B[j] = 0.f; }
+  const int per = (k + waves) / waves, from = wave * per, to = min(k + 1, from + per);
 #pragma unroll 8
-  for (int s = 0; s <= k; ++s) {
+  for (int s = from; s < to; ++s) {
     const float2* q = p.pairs + (b * p.splits + s) * p.D + d;
 #pragma unroll
-    for (int j = 0; j < VC; ++j) x[j] = apply(q[j].x, q[j].y, x[j]);
+    for (int j = 0; j < VC; ++j) compose(A[j], B[j], q[j].x, q[j].y);
   }
+#pragma unroll
+  for (int j = 0; j < VC; ++j) sh[wave][lane * VC + j] = make_float2(A[j], B[j]);
+  __syncthreads();
+  for (int w = 0; w < waves; ++w)
+#pragma unroll
+    for (int j = 0; j < VC; ++j) x[j] = apply(sh[w][lane * VC + j].x, sh[w][lane * VC + j].y, x[j]);
 }
 
 // A wave's pair into LDS; returns the state that reaches this wave and moves `x` past all waves.
@@ -229,13 +256,14 @@ template <typename E, int VC, bool GATE>
 __global__ void __launch_bounds__(64 * WAVES) k_scan_fwd(ScanArgs p) {
   __shared__ float2 sh[2][WAVES][64 * VC];   // two buffers: one barrier per exchange
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int k = blockIdx.x % p.splits, g = (blockIdx.x / p.splits) % p.groups;
-  const long b = blockIdx.x / p.splits / p.groups;
+  const Work w = work_of(p, p.splits);
+  const int k = w.k, g = w.g;
+  const long b = w.b;
   const int d = min((g * 64 + lane) * VC, p.D - VC);   // lanes past the last channel repeat it, and store nothing
   const bool live = (g * 64 + lane) * VC < p.D;
   const int end = min(p.T, (k + 1) * p.span);
   float x[VC];
-  start_state<VC>(p, b, k, d, x);
+  start_state<VC>(p, b, k, d, sh[1], wave, waves, lane, x);   // (the first exchange takes sh[0])
   int buf = 0;
   for (int base = k * p.span; base < end; base += waves * STEPS, buf ^= 1) {
     const int o0 = base + wave * STEPS, n = min(STEPS, end - o0);   // n <= 0: a wave behind the end
@@ -264,13 +292,14 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
   constexpr bool LOW = sizeof(E) == 2;
   __shared__ float2 sh[2][WAVES][64 * VC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int k = blockIdx.x % p.splits, g = (blockIdx.x / p.splits) % p.groups;
-  const long b = blockIdx.x / p.splits / p.groups;
+  const Work w = work_of(p, p.splits);
+  const int k = w.k, g = w.g;
+  const long b = w.b;
   const int d = min((g * 64 + lane) * VC, p.D - VC);
   const bool live = (g * 64 + lane) * VC < p.D;
   const int end = min(p.T, (k + 1) * p.span);   // in scan order: o = T - 1 - t
   float x[VC];
-  start_state<VC>(p, b, k, d, x);
+  start_state<VC>(p, b, k, d, sh[1], wave, waves, lane, x);   // (the first exchange takes sh[0])
   int buf = 0;
   for (int base = k * p.span; base < end; base += waves * STEPS, buf ^= 1) {
     const int o0 = base + wave * STEPS, n = min(STEPS, end - o0);
@@ -333,14 +362,15 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
 }
 
 // Splits of the time axis: none where the channels alone give every CU a workgroup; else enough for
-// four workgroups per CU, each at least two exchanges of all waves long.
+// four workgroups per CU, each at least one exchange of all waves long (two: 3 x 966 x 2240 forward 37 us against
+// 28; from 256 steps on: 162 take 9 us in one launch and 12 in two).
 inline void plan(ScanArgs& p) {
   constexpr int PASS = WAVES * STEPS;
   const long wgs = (long)p.B * p.groups;
   p.splits = 1;
   p.span = p.T;
   if (wgs < 256 && p.T >= 4 * PASS) {
-    const long want = min((1024 + wgs - 1) / wgs, (long)p.T / (2 * PASS));
+    const long want = min((1024 + wgs - 1) / wgs, (long)p.T / PASS);
     p.span = dd_ceil_div(dd_ceil_div(p.T, want), PASS) * PASS;
     p.splits = dd_ceil_div(p.T, p.span);
     if (p.splits == 1) p.span = p.T;
@@ -367,14 +397,27 @@ int launch(ScanArgs& p, float* ws, size_t ws_bytes, hipStream_t stream) {
   return 0;
 }
 
-// bf16: two channels per lane (256 bytes of a row per wave) where that leaves every CU a workgroup, or the time
-// axis is split anyway (50 x 50 x 1024 backward: 11 us against 16 with one; 4 x 4096 x 1024 forward 48 against 53).
+// Two channels per lane.  bf16 (256 bytes of a row per wave): where that leaves every CU a workgroup, or the time axis
+// is split anyway (50 x 50 x 1024 backward: 11 us against 16 with one; 4 x 4096 x 1024 forward 48 against 53).
+// fp32: long scans of rows that are not aligned to cache lines, a smaller part of which is then shared (1 x 24368
+// x 2367 backward 510 us against 598; aligned rows 2 x 16385 x 512 lose 2%, 29 x 78 x 3392 a fifth).
 template <bool BWD>
 int dispatch(ScanArgs& p, int type, float* ws, size_t ws_bytes, hipStream_t st) {
 #define DD_SCAN(E_, VC_) \
   return p.i ? launch<E_, VC_, true, BWD>(p, ws, ws_bytes, st) : launch<E_, VC_, false, BWD>(p, ws, ws_bytes, st)
-  if (type == DD_F32) DD_SCAN(float, 1);
-  if (p.D % 2 == 0 && ((long)p.B * dd_ceil_div(p.D, 128) >= 256 || p.T >= 4 * WAVES * STEPS)) DD_SCAN(__bf16, 2);
+  const long es = type == DD_F32 ? 4 : 2;
+  auto aligned = [&](const void* q, long ld) { return !q || ((uintptr_t)q % 128 == 0 && (ld * es) % 128 == 0); };
+  p.shared_lines = !(aligned(p.u, p.ldu) && aligned(p.c, p.ldc) && aligned(p.i, p.ldi) && aligned(p.h, p.ldh) &&
+                     aligned(p.dh, p.lddh) && aligned(p.du, p.lddu) && aligned(p.dc, p.lddc) && aligned(p.di, p.lddi));
+  // (an odd row's last lane takes its neighbour's second channel as well; a group of that lane alone would write
+  // another workgroup's channel, which a state updated in place must not see)
+  const bool pairs = p.D > 1 && p.D % 128 != 1;
+  const long wgs = (long)p.B * dd_ceil_div(p.D, 128);
+  if (type == DD_F32) {
+    if (pairs && p.shared_lines && wgs * dd_ceil_div(p.T, WAVES * STEPS) >= 2048) DD_SCAN(float, 2);
+    DD_SCAN(float, 1);
+  }
+  if (p.D % 2 == 0 && (wgs >= 256 || p.T >= 4 * WAVES * STEPS)) DD_SCAN(__bf16, 2);
   DD_SCAN(__bf16, 1);
 #undef DD_SCAN
 }

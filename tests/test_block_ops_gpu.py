@@ -397,6 +397,14 @@ def test_scan(hip, ref, B, T, D, gate, cand, dt):
   hs.whole(), d.whole()
 
 
+@pytest.mark.parametrize('B,T,D', [(300, 256, 131), (100, 704, 131), (100, 704, 129)])
+@pytest.mark.parametrize('gate,cand', [(False, 'tanh'), (True, None)])
+def test_scan_of_many_unaligned_rows(hip, ref, B, T, D, gate, cand):
+  """Rows that share cache lines with their neighbours, enough of them for two fp32 channels per lane, the last of
+  which overlap where a row is odd; whole and split."""
+  test_scan(hip, ref, B, T, D, gate, cand, F32)
+
+
 def test_scan_defaults(hip, ref):
   """No restarts, no initial state, no final one."""
   u, c = rnd(60, 32, seed=1), rnd(60, 32, seed=2)
