@@ -393,6 +393,7 @@ template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
   typedef Inst<ES> I;
   constexpr int NW = WM * WN, MT = BM / WM / I::ROWS, NT = BN / WN / I::ROWS, UP = BM * ROWB, UQ = BN * ROWB;
+  static_assert(BM % (WM * I::ROWS) == 0 && BN % (WN * I::ROWS) == 0, "the waves' instructions cover the tile");
   constexpr int STEPS = 2, BK = ROWB / ES, LDS = 3 * UP + 2 * UQ;
   __shared__ __attribute__((aligned(1024))) char sh[LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -873,13 +874,16 @@ bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
 template <int ES, bool P_RC, bool Q_RC>
 int planned(const char* who, const Mat& P, const Mat& Q, int K, const Plan& plan, const Epi& e, float* slabs, hipStream_t st) {
   if constexpr (!P_RC)
-    if (plan.shape == 2) return tiled<ES, P_RC, Q_RC, 192, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
+    if (plan.shape == 2) {   // (48 rows a wave are three of the 16 x 16 instruction's, but no whole number of 32)
+      if constexpr (ES == 2) return tiled<ES, P_RC, Q_RC, 192, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
+      else return tiled<ES, P_RC, Q_RC, 192, 128, 2, 4>(who, P, Q, K, plan.splits, e, slabs, st);
+    }
   if (plan.shape == 1) return tiled<ES, P_RC, Q_RC, 128, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
   return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, P, Q, K, plan.splits, e, slabs, st);
 }
 // The tiled products.  Where the last round of tiles would leave most of the chip idle, whole rounds take
 // the first rows and a launch of its own, with a plan of its own, the rest (37500 x 1024 x 2048, 2.3 rounds:
-// bf16 166 -> 161, e4m3 102 -> 94 us; its dx 150 -> 138).
+// 166 -> 161 us; its dx 150 -> 138).
 template <int ES, bool P_RC, bool Q_RC>
 int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, size_t room, hipStream_t st) {
   const int ksteps = dd_ceil_div(K, ROWB / ES), shapes = P_RC ? 2 : 3;

@@ -264,8 +264,9 @@ def test_linear_gradients_many_tiles(hip, ref, M, N, K):
   test_linear_gradients(hip, ref, M, N, K, 'silu', F32)
 
 
-def test_linear_e4m3_many_tiles(hip, ref):
-  test_linear_e4m3(hip, ref, 16501, 1030, 1040, 'silu')
+@pytest.mark.parametrize('M,N,K', [(3001, 1541, 903), (2500, 2048, 1536), (16501, 1030, 1040)])
+def test_linear_e4m3_many_tiles(hip, ref, M, N, K):
+  test_linear_e4m3(hip, ref, M, N, K, 'silu')
 
 
 @pytest.mark.parametrize('M', [3, 70, 300])
