@@ -218,19 +218,6 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
   }
 }
 
-// Rows -> rows of whole 16-byte chunks, zeros behind; a chunk per thread.
-template <int ES>
-__global__ void __launch_bounds__(256) k_linear_pack(const char* in, long ldb, int cols, char* out, unsigned chunks, unsigned total) {
-  const unsigned i = blockIdx.x * 256 + threadIdx.x, row = i / chunks;
-  if (i >= total) return;
-  const int c = (int)(i - row * chunks) * (16 / ES);
-  const char* from = in + row * ldb + (long)c * ES;
-  i32x4 v;
-  if (c + 16 / ES <= cols) v = __builtin_bit_cast(i32x4, *reinterpret_cast<const u32x4u*>(from));
-  else v = partial_chunk<ES>(from, cols % (16 / ES));
-  *reinterpret_cast<i32x4*>(out + i * 16l) = v;
-}
-
 // ---- tiled kernel --------------------------------------------------------------------------------
 //
 // BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
@@ -264,18 +251,21 @@ struct TileCopy {
   const char* base;      // tile's first byte of the next step
   long step;             // bytes from a step to the next
   unsigned size;         // bytes from base to the end of the tile's last row (KC) or of a whole step (RC)
-  unsigned ldb, cols;    // RC: bytes of a row, of the tile's part of it and what is behind
+  unsigned ldb, cols;    // RC: bytes of a row, of the tile's part of it and what is behind (in the contraction's last row)
   int voff[N];
   // KC: contraction elements in front of the lane's chunk (a single wave: in even and odd blocks of 8 rows;
   // an even number of waves: a wave's blocks are all even or all odd)
   int col[1 + NW % 2];
   // the tile at (r0, k0); `apart`: steps of 128 bytes (KC) from one copy to the next
-  __device__ __forceinline__ void init(const Mat& a, long r0, long k0, int K, int wave, int lane, int apart = 1) {
+  // ends: the last step is the operand's last.  (A copy takes whole 4-byte units up to the range's end: the last
+  // element of an odd RC row is read with the next row's first, and in the last row it is left to mend_corner.)
+  __device__ __forceinline__ void init(const Mat& a, long r0, long k0, int K, int wave, int lane, bool ends = true, int apart = 1) {
     base = (const char*)a.p + (RC ? k0 * a.ld + r0 : r0 * a.ld + k0) * ES;
     step = RC ? BK * a.ld * ES : ROWB * apart;
     ldb = (unsigned)(a.ld * ES);
-    cols = (unsigned)((a.R - r0) * ES + 3) & ~3u;   // (an odd length was packed: zeros behind)
-    size = RC ? (BK - 1) * ldb + cols : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
+    cols = (unsigned)((a.R - r0) * ES);
+    if (!ends) cols += cols & 2;
+    size = RC ? (BK - 1) * ldb + cols + (cols & 2) : (unsigned)min((long)R_, a.R - r0) * ldb - ldb + (unsigned)(K - k0) * ES;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = (i * NW + wave) * 64 + lane;
@@ -293,7 +283,7 @@ struct TileCopy {
   // The copies of the next step into LDS offset `lds`; rest: contraction elements left (none: zeros).
   __device__ __forceinline__ u32x4 begin(int rest, int wave) {
     unsigned bytes = rest > 0 ? size : 0u;
-    if (RC && rest < BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
+    if (RC && rest <= BK) bytes = rest > 0 ? (unsigned)(rest - 1) * ldb + cols : 0u;
     const u32x4 rs = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffffu, bytes, 0x00020000u};
     if (!RC && rest > 0 && rest < BK)     // the last step of a ragged contraction: chunks that are not whole are
 #pragma unroll                            // moved out of the descriptor's range (mend_tail writes the one that is cut)
@@ -322,6 +312,13 @@ __device__ __forceinline__ void mend_tail(const Mat& a, long r0, int K, int k0, 
     if (r0 + r < a.R) v = partial_chunk<ES>((const char*)a.p + ((r0 + r) * a.ld + k0 + c * PER) * ES, n);
     *reinterpret_cast<i32x4*>(tile + r * ROWB + ((c ^ ((r >> 1) & 7)) << 4)) = v;
   }
+}
+// The last element of an RC operand of odd row length, row k of the tile of the last step.
+template <int R_>
+__device__ __forceinline__ void mend_corner(const Mat& a, long r0, int K, int k, char* tile) {
+  const int r = (int)(a.R - 1 - r0);
+  const unsigned short v = reinterpret_cast<const unsigned short*>(a.p)[(K - 1) * a.ld + a.R - 1];
+  *reinterpret_cast<unsigned short*>(tile + k * (R_ * 2) + (((r >> 3) ^ rc_swizzle(k)) << 4) + (r & 7) * 2) = v;
 }
 // Every copy of this wave but the LATER newest has landed, and then every wave's; reads issued before are
 // complete.
@@ -413,8 +410,8 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
 
   TileCopy<ES, P_RC, BM, NW> cp;
   TileCopy<ES, Q_RC, BN, NW> cq;
-  cp.init(P, m0, kb, K, wave, lane);
-  cq.init(Q, n0, kb, K, wave, lane);
+  cp.init(P, m0, kb, K, wave, lane, kend == K);
+  cq.init(Q, n0, kb, K, wave, lane, kend == K);
   const unsigned lds = (unsigned)(uintptr_t)(DD_LDS char*)sh;
   typename I::Acc acc[MT][NT] = {};
   int rest_p = kend - (int)kb, rest_q = rest_p;   // of the step that is copied next
@@ -435,12 +432,15 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
   // next one the copies of Q (step t + 2) and P (t + 3) are issued - a few behind each row of instructions: in
   // one go they would hold the waves up while the address unit works through them.  Operands are read one
   // group ahead, across the barrier too, so that the matrix unit has work while the waves meet.
-  // (a contraction that ends inside a chunk: its last step's tiles are mended once they have landed)
-  const bool cut = kend == K && K % (16 / ES) != 0 && !(P_RC && Q_RC);
+  // (a contraction that ends inside a chunk, an odd RC row: the last step's tiles are mended once they have landed)
+  const bool odd_p = P_RC && P.R % 2 != 0 && m0 + BM >= P.R, odd_q = Q_RC && Q.R % 2 != 0 && n0 + BN >= Q.R;
+  const bool part = K % (16 / ES) != 0, cut = kend == K && ((part && !(P_RC && Q_RC)) || odd_p || odd_q);
   auto mend = [&](int at_p, int at_q) {
     const int k0 = (int)kb + (steps - 1) * BK;
-    if constexpr (!P_RC) mend_tail<ES, BM>(P, m0, K, k0, sh + at_p, threadIdx.x, NW * 64);
-    if constexpr (!Q_RC) mend_tail<ES, BN>(Q, n0, K, k0, sh + at_q, threadIdx.x, NW * 64);
+    if constexpr (!P_RC) { if (part) mend_tail<ES, BM>(P, m0, K, k0, sh + at_p, threadIdx.x, NW * 64); }
+    else if (odd_p && threadIdx.x == 0) mend_corner<BM>(P, m0, K, K - 1 - k0, sh + at_p);
+    if constexpr (!Q_RC) { if (part) mend_tail<ES, BN>(Q, n0, K, k0, sh + at_q, threadIdx.x, NW * 64); }
+    else if (odd_q && threadIdx.x == 0) mend_corner<BN>(Q, n0, K, K - 1 - k0, sh + at_q);
     sync_copies();
   };
   int p0 = 0, p1 = UP, p2 = 2 * UP, q0 = 3 * UP, q1 = 3 * UP + UQ;
@@ -707,8 +707,8 @@ __global__ void __launch_bounds__(64 * WV) k_linear_few(Mat P, Mat Q, int K, Epi
   TileCopy<ES, false, 16, 1> cq;
   TileCopy<ES, false, 16 * MB, 1> cp;
   int rest = K - wave * BK;
-  cq.init(Q, n0, (long)wave * BK, K, 0, lane, WV);
-  cp.init(P, 0, (long)wave * BK, K, 0, lane, WV);
+  cq.init(Q, n0, (long)wave * BK, K, 0, lane, true, WV);
+  cp.init(P, 0, (long)wave * BK, K, 0, lane, true, WV);
   auto copy = [&](int buf) {
     cq.issue(lds + buf * TURN, 0, rest);
     cp.issue(lds + buf * TURN + 16 * ROWB, 0, rest);
@@ -808,11 +808,8 @@ inline int pick_splits(long tiles, int ktiles, size_t slab_bytes, size_t ws_byte
   return (int)max(s, 1l);
 }
 
-// Can the tiled kernel's copies read this operand?  Offsets within a tile stay below 2^31; a copy takes whole
-// 4-byte units up to the operand's last byte, so RC rows (which nothing mends) have an even length.
-inline bool tileable(const Mat& a, bool rc, int es) {
-  return (!rc || a.R % 2 == 0) && (long)(rc ? 64 : 256) * a.ld * es < (1l << 30);
-}
+// Can the tiled kernel's copies read this operand?  Offsets within a tile stay below 2^31.
+inline bool tileable(const Mat& a, bool rc, int es) { return (long)(rc ? 64 : 256) * a.ld * es < (1l << 30); }
 
 // The tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and the
 // rest of a tile (start, epilogue) take then, in microseconds (fitted to bf16 products of 2500 to 37500 rows).
@@ -852,23 +849,6 @@ int tiled(const char* who, Mat P, Mat Q, int K, int splits, const Epi& e, float*
       P, Q, K, kspan, tm, tn, parts > 1 ? slabs : nullptr, e);
   DD_CHECK_LAUNCH(who);
   return parts > 1 ? sum_slabs(who, slabs, parts, P.R, Q.R, e, st) : 0;
-}
-
-// The operand with rows that the tiled kernel can read, copied into the workspace unless it has them
-// already; false: no room.
-template <int ES>
-bool pack(Mat& a, bool rc, int K, char*& ws, size_t& room, hipStream_t st) {
-  if (tileable(a, rc, ES)) return true;
-  const long rows = rc ? K : a.R;
-  const int cols = rc ? a.R : K, chunks = dd_ceil_div(cols, 16 / ES);
-  const size_t bytes = ((size_t)rows * chunks * 16 + 255) / 256 * 256;
-  if (bytes > room || rows * chunks >= (1l << 32) - 256) return false;
-  k_linear_pack<ES><<<(unsigned)((rows * chunks + 255) / 256), 256, 0, st>>>((const char*)a.p, a.ld * ES, cols, ws, chunks, (unsigned)(rows * chunks));
-  a.p = ws;
-  a.ld = chunks * (16 / ES);
-  ws += bytes;
-  room -= bytes;
-  return true;
 }
 
 template <int ES, bool P_RC, bool Q_RC>
@@ -925,20 +905,17 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
       DD_CHECK_LAUNCH(who);
       return 0;
     }
-  // The tiled kernel, on packed copies of transposed operands of odd length where the product is large enough
-  // to pay for them (about 6 us an operand at 2500 x 1541, against 100 us for the general kernel).
-  char* at = (char*)(((uintptr_t)ws + 255) / 256 * 256);
-  size_t room = ws && ws_bytes > 512 ? ws_bytes - 256 : 0;
-  if (K > 0 && (!e.res || e.ldr < (1l << 20)) && ((tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES)) || (double)P.R * Q.R * K >= 134217728.0)) {
-    Mat p = P, q = Q;
-    if (pack<ES>(p, P_RC, K, at, room, st) && pack<ES>(q, Q_RC, K, at, room, st))
-      return rounds<ES, P_RC, Q_RC>(who, p, q, K, e, (float*)at, room, st);
-  }
+  const size_t room = ws ? ws_bytes : 0;
+  // Below 2^22 multiplications over a short contraction the general kernel's small tiles start and end sooner
+  // (128 x 128 x 128 4.2 us against 5.4, 8 x 64 x 72 dw 4.4 against 5.1; 70 x 64 x 1000 8.5 either way).
+  const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * ES < 8 * ROWB;
+  if (!small && K > 0 && tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES) && (!e.res || e.ldr < (1l << 20)))
+    return rounds<ES, P_RC, Q_RC>(who, P, Q, K, e, ws, room, st);
   const int bk = ROWB / ES;
   const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));
   DD_REQUIRE(tiles.y <= 65535, "dd_linear: more than 4194240 output columns");
   const int ktiles = dd_ceil_div(K, bk);
-  const int S = pick_splits((long)tiles.x * tiles.y, ktiles, sizeof(float) * (size_t)P.R * Q.R, ws ? ws_bytes : 0);
+  const int S = pick_splits((long)tiles.x * tiles.y, ktiles, sizeof(float) * (size_t)P.R * Q.R, room);
   const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
   k_linear_any<ES, P_RC, Q_RC><<<dim3(tiles.x, tiles.y, parts), 256, 0, st>>>(P, Q, K, kspan, parts > 1 ? ws : nullptr, e);
   DD_CHECK_LAUNCH(who);
@@ -948,41 +925,63 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
 // dz = dy act'(z), and the workgroup's share of dbias; without an activation dz IS dy and only the column
 // sums are taken.  HBM-bound: a wave takes 512 columns of a row at a time (1 KB), or several rows of narrower
 // matrices (`lanes` of it per row: 30237 x 64: 6 us against 14 with whole waves), four waves on different rows, four rows
-// requested at a time; the columns of a ragged row's end one by one.
+// requested at a time.  Up to 256 rows a workgroup takes all rows of
+// 64 columns and stores the sums itself, one launch less (110 x 2752 gelu 4.6 us against 6.8; 500 x 741 10 against
+// 8.5).
+// Columns c .. c + V - 1 of rows m0, m0 + step, ...; `seen` of them are counted by another lane.
 template <int V, int ACT>
 __device__ __forceinline__ void act_rows(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz, long c,
-                                         long m0, long m1, int step, float sum[V]) {
-#pragma unroll 4
-  for (long m = m0; m < m1; m += step) {
-    float d[V], t[V];
-    load_bf16<V>(dy + m * ldy + c, d);
-    if constexpr (ACT != DD_ACT_NONE) {
-      load_bf16<V>(z + m * ldz + c, t);
+                                         long m0, long m1, int step, int seen, float sum[V]) {
+  constexpr int ROWS = 4;   // loaded together (dz may be dy or z: a store in between would hold the next loads up)
+  for (long m = m0; m < m1; m += ROWS * step) {
+    float d[ROWS][V], t[ROWS][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] *= act_slope<ACT>(t[j]);
-      // bf16: the two products that read dz take bf16 operands
-      store_bf16<V>(dz + m * lddz + c, d);
+    for (int r = 0; r < ROWS; ++r) {
+      const long row = m + r * step < m1 ? m + r * step : m;
+      load_bf16<V>(dy + row * ldy + c, d[r]);
+      if constexpr (ACT != DD_ACT_NONE) load_bf16<V>(z + row * ldz + c, t[r]);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] += d[j];
+    for (int r = 0; r < ROWS; ++r) {
+      if (m + r * step >= m1) break;
+      if constexpr (ACT != DD_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[r][j] *= act_slope<ACT>(t[r][j]);
+        // bf16: the two products that read dz take bf16 operands
+        store_bf16<V>(dz + (m + r * step) * lddz + c, d[r]);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += j < seen ? 0.f : d[r][j];
+    }
   }
 }
 template <int ACT>
 __global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, const __bf16* z, long ldz, __bf16* dz, long lddz,
-                                                 float* parts, int M, int N, int rows_per, int lanes) {
+                                                 float* parts, int M, int N, int rows_per, int lanes, void* dbias, int type,
+                                                 int accumulate) {
   __shared__ float sh[4 * 512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, apart = 64 / lanes;   // rows of a wave
   const long c = ((long)blockIdx.x * lanes + lane % lanes) * 8;
   const long m0 = (long)blockIdx.y * rows_per + wave * apart + lane / lanes, m1 = min((long)M, (blockIdx.y + 1l) * rows_per);
   float sum[8] = {};
-  if (c + 8 <= N) act_rows<8, ACT>(dy, ldy, z, ldz, dz, lddz, c, m0, m1, 4 * apart, sum);
-  else
+  // A ragged row's last columns are those of a full vector that overlaps the lane before, in the same wave (another
+  // workgroup might have written dz over dy there); only a wave's first lane takes them one by one.
+  const int seen = c < N && c + 8 > N && lane % lanes != 0 ? (int)(c + 8 - N) : 0;
+  if (c + 8 - seen <= N && c < N) {
+    act_rows<8, ACT>(dy, ldy, z, ldz, dz, lddz, c - seen, m0, m1, 4 * apart, seen, sum);
+  } else {
+#pragma unroll 1
+    for (int j = 0; c + j < N; ++j) {
+      float t[1] = {0.f};
+      act_rows<1, ACT>(dy, ldy, z, ldz, dz, lddz, c + j, m0, m1, 4 * apart, 0, t);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < N) act_rows<1, ACT>(dy, ldy, z, ldz, dz, lddz, c + j, m0, m1, 4 * apart, sum + j);
-  if (!parts) return;
+      for (int k = 0; k < 8; ++k) sum[k] = k == j ? t[0] : sum[k];
+    }
+  }
+  if (!parts && !dbias) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sh[threadIdx.x * 8 + j] = sum[j];
+  for (int j = 0; j < 8; ++j)   // (8 - seen sums, from the lane's own first column)
+    if (j >= seen) sh[threadIdx.x * 8 + j - seen] = sum[j];
   __syncthreads();
   for (int i = threadIdx.x; i < 8 * lanes; i += 256) {   // waves and their rows in order
     const long col = (long)blockIdx.x * lanes * 8 + i;
@@ -990,7 +989,9 @@ __global__ void __launch_bounds__(256) k_act_bwd(const __bf16* dy, long ldy, con
     float t = sh[i];
 #pragma unroll 4
     for (int r = 1; r < 4 * apart; ++r) t += sh[r * lanes * 8 + i];
-    parts[(long)blockIdx.y * N + col] = t;
+    if (parts) parts[(long)blockIdx.y * N + col] = t;
+    else if (type == DD_F32) { float* p = (float*)dbias + col; *p = accumulate ? *p + t : t; }
+    else { __bf16* p = (__bf16*)dbias + col; *p = (__bf16)(accumulate ? (float)*p + t : t); }
   }
 }
 
@@ -1056,10 +1057,11 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
   DD_REQUIRE(M == 0 || !act_on || (z && dz && ldz >= N && lddz >= N), "dd_linear_act_bwd: an activation needs z and dz");
   const hipStream_t st = (hipStream_t)stream;
   // 1024 workgroups, at least a row each for every row of lanes
-  int lanes = 64;
+  const bool whole = M <= 256;
+  int lanes = whole ? 8 : 64;
   while (lanes > 1 && N <= 4 * lanes) lanes /= 2;
   const int cols = dd_ceil_div(N, 8 * lanes);
-  const int rows_per = max(256 / lanes, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
+  const int rows_per = whole ? max(M, 1) : max(256 / lanes, dd_ceil_div(M, max(1, dd_ceil_div(1024, cols)))), n = dd_ceil_div(M, rows_per);
   DD_REQUIRE(n <= 65535, "dd_linear_act_bwd: too many rows");
   DD_REQUIRE(!dbias || ws_bytes / sizeof(float) >= (size_t)n * N, "dd_linear_act_bwd: the workspace is too small");
   if (M > 0) {
@@ -1067,13 +1069,14 @@ extern "C" int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long l
 #define DD_ACT_BWD(A_)                                                                                          \
   case A_:                                                                                                      \
     k_act_bwd<A_><<<grid, 256, 0, st>>>((const __bf16*)dy, ldy, (const __bf16*)z, ldz, (__bf16*)dz, lddz,       \
-                                        dbias ? ws : nullptr, M, N, rows_per, lanes);                                  \
+                                        dbias && !whole ? ws : nullptr, M, N, rows_per, lanes, dbias, bias_type,    \
+                                        accumulate);                                                                \
     break;
     switch (act) { DD_ACT_BWD(DD_ACT_NONE) DD_ACT_BWD(DD_ACT_ELU) DD_ACT_BWD(DD_ACT_SILU) DD_ACT_BWD(DD_ACT_GELU) }
 #undef DD_ACT_BWD
     DD_CHECK_LAUNCH("dd_linear_act_bwd");
   }
-  if (dbias) {
+  if (dbias && !(whole && M > 0)) {
     k_part_sum<<<dd_ceil_div(N, 32), 1024, 0, st>>>(ws, n, N, dbias, bias_type, accumulate);
     DD_CHECK_LAUNCH("dd_linear_act_bwd(dbias)");
   }
