@@ -386,6 +386,9 @@ __device__ __forceinline__ f32x16 mma(i32x8 q, i32x8 p, f32x16 c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(q, p, c, 0, 0, 0, 127, 0, 127);
 }
 
+// The largest divisor of n that is at most m.
+constexpr int whole_part(int n, int m) { return m <= 0 ? 0 : m >= n ? n : n % m == 0 ? m : whole_part(n, m - 1); }
+
 template <int ES, bool P_RC, bool Q_RC, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linear_tile(Mat P, Mat Q, int K, int kspan, int tm, int tn, float* slabs, Epi e) {
   typedef Inst<ES> I;
@@ -489,14 +492,17 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
 
   // Sixteen rows at a time through the wave's own LDS (Q was the instruction's first operand: a lane holds four
   // consecutive columns of one row); LPR lanes finish a row, 8 columns each, RI rows per lane.  The residual's
-  // tile - the part of it that these lanes finish - comes into the wave's LDS in one burst (fp32: in two), as
-  // the tiles did: requested sixteen rows at a time it cost a memory latency each (37500 x 2048 x 1024 with a
-  // residual: 222 us).  Only the writes to LDS know which accumulators they take; the rest of the
+  // tile - the part of it that these lanes finish - comes into the wave's LDS in bursts as large as that is, like the
+  // tiles before it: requested sixteen rows at a time it cost a memory latency each (37500 x 2048 x 1024 with a
+  // residual 222 us against 184).  Only the writes to LDS know which accumulators they take; the rest of the
   // loop stays rolled, because copies of three activations would not fit the instruction cache.
   constexpr int W = BN / WN, LPR = W / 8, RPI = 64 / LPR, RI = 16 / RPI, ROWS = I::ROWS, WROWS = BM / WM, HALVES = WROWS / 16;
-  constexpr int OUT = 16 * W * 4, RES = LDS / NW - OUT;   // bytes of a wave
+  // Rows of an exchange, an accumulator block's where the wave's LDS holds them beside the residual; bytes of the two;
+  // sixteens of rows in a burst of the residual (a divisor of the wave's, so that bursts end with the rows).
+  constexpr int XR = LDS / NW - ROWS * W * 4 >= 4096 ? ROWS : 16, OUT = XR * W * 4, RES = LDS / NW - OUT;
+  constexpr int BURST2 = whole_part(HALVES, RES / (16 * W * 2)), BURST4 = whole_part(HALVES, RES / (16 * W * 4));
   static_assert(RI * RPI == 16, "sixteen rows are whole rows of every lane");
-  static_assert(RES >= WROWS * W * 2, "the residual's LDS");
+  static_assert(BURST4 > 0, "the residual's LDS");
   char* mine = sh + wave * (OUT + RES);
   float* out = reinterpret_cast<float*>(mine);
   // 16-byte chunk c of row r, permuted by the row so that the writes of 16 rows fall on different banks
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
   if (shifted) nc = cols - 8;
   const bool full = nc + 8 <= cols;
   const long n = n0 + wn + nc, mrow = m0 + wm + lane / LPR;
-  const int es = e.ytype == DD_F32 ? 4 : 2, burst = e.ytype == DD_F32 ? HALVES / 2 : HALVES;
+  const int es = e.ytype == DD_F32 ? 4 : 2, burst = e.ytype == DD_F32 ? BURST4 : BURST2;
   auto fetch = [&](int i) {   // the residual's rows 16 i .. 16 (i + burst) - 1 of the wave
     const int rows = (int)min((long)burst * 16, P.R - (m0 + wm + 16 * i));
     const unsigned ldb = (unsigned)(e.ldr * es);
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
     const unsigned to = lds + wave * (OUT + RES) + OUT, step = 1024 / (W * es) * ldb,
                    v = es == 4 ? lane / (W / 4) * ldb + lane % (W / 4) * 16 : lane / (W / 8) * ldb + lane % (W / 8) * 16;
 #pragma unroll 1
-    for (int k = 0; k < WROWS * W * 2 / 1024; ++k) copy16(rs, to + k * 1024, (int)(v + k * step));
+    for (int k = 0; k < burst * 16 * W * es / 1024; ++k) copy16(rs, to + k * 1024, (int)(v + k * step));
   };
   // the sums of sixteen rows: lane's RI rows of 8 columns
   const int lr = lane / LPR;
@@ -533,18 +539,18 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
     const unsigned which = 1u << i / PER;
     int l = lane, c = nc;
     asm volatile("" : "+v"(c));   // these addresses are computed here, not kept across the loop
-    if constexpr (BM * BN <= 16384 || ES == 1) asm volatile("" : "+v"(l));   // (nor these, where registers are short)
-    const int lr = l / LPR;
+    if constexpr (BM * BN <= 16384) asm volatile("" : "+v"(l));   // (nor these: 128 registers)
+    const int lr = l / LPR + (XR == 32 ? i % 2 * 16 : 0);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int k = 0; k < MT; ++k)
-      if (which >> k & 1 && (PER == 1 || (l % 32) / 16 == i % PER))
+      if (which >> k & 1 && (XR == 32 ? i % 2 == 0 : PER == 1 || (l % 32) / 16 == i % PER))
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int g = 0; g < PER * PER; ++g) {   // 16 x 16: one run of four columns, 32 x 32: four, 8 apart
             const f32x4 t = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
-            *reinterpret_cast<f32x4*>(at(l % 16, (ROWS * j + 8 * g) / 4 + l / ROWS)) = t;
+            *reinterpret_cast<f32x4*>(at(l % XR, (ROWS * j + 8 * g) / 4 + l / ROWS)) = t;
           }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -675,7 +681,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
         const int r = k / 8, j = k % 8;
         const long m = m0 + wm + 16 * i + r;
         if (j >= cols || m >= P.R) continue;
-        float t[1] = {at(r, j / 4)[j & 3]};
+        float t[1] = {at(r + (XR == 32 ? i % 2 * 16 : 0), j / 4)[j & 3]};
         finish<1>(e, m, n0 + wn + j, t);
       }
     // (the reads of this burst are complete before the next one overwrites it)
@@ -811,20 +817,26 @@ inline int pick_splits(long tiles, int ktiles, size_t slab_bytes, size_t ws_byte
 // Can the tiled kernel's copies read this operand?  Offsets within a tile stay below 2^31.
 inline bool tileable(const Mat& a, bool rc, int es) { return (long)(rc ? 64 : 256) * a.ld * es < (1l << 30); }
 
-// The tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes and the
-// rest of a tile (start, epilogue) take then, in microseconds (fitted to bf16 products of 2500 to 37500 rows).
+// The tile shapes: how many tiles run at once on the chip, and what a step of 128 contraction bytes, the
+// rest of a tile (start, epilogue), an activation and one more tensor in the epilogue (residual, pre-activation) take
+// then, in microseconds (fitted to products of 2500 to 37500 rows).
 // 256 x 256 is the fastest per output (1430 against 1140 TFLOP/s of 128 x 128, 8192^3); the small ones fill the
 // chip with fewer rows and waste less in a last round (2500 x 2048 x 1536: 192 x 128 22, 128 x 128 26, 256 x 256
 // 36 us; 2500 x 1024 x 1024: 13.5, 12.4, 21).  192 rows are for P by rows: the transposing reads' swizzle
 // wants a power of two.
-struct TileShape { int rows, cols, slots; float step, rest; };
-constexpr TileShape SHAPES[] = {{256, 256, 256, 1.38f, 10.f}, {128, 128, 512, 0.96f, 4.5f}, {192, 128, 256, 0.62f, 6.5f}};
+struct TileShape { int rows, cols, slots; float step, rest, act, tensor; };
+constexpr TileShape SHAPES[] = {
+    {256, 256, 256, 1.38f, 10.f, 4.5f, 5.5f}, {128, 128, 512, 0.96f, 4.5f, 1.2f, 1.5f}, {192, 128, 256, 0.62f, 6.5f, 1.5f, 2.5f}};
 
+inline float epilogue_cost(const TileShape& t, const Epi& e) {
+  return (e.act != DD_ACT_NONE ? t.act : 0.f) + ((e.res != nullptr) + (e.z != nullptr)) * t.tensor;
+}
 struct Plan { int shape, splits; float us; };
-inline Plan plan_product(long M, long N, int ksteps, size_t slab_room, int shapes) {
+inline Plan plan_product(long M, long N, int ksteps, size_t slab_room, int shapes, const Epi& e) {
   Plan best{0, 1, 1e30f};
   for (int i = 0; i < shapes; ++i) {
-    const TileShape& t = SHAPES[i];
+    TileShape t = SHAPES[i];
+    t.rest += epilogue_cost(t, e);
     const long tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
     for (int s = 1; s <= 64 && s <= max(1, ksteps / 4); s = s < 4 ? s + 1 : s * 2) {
       if (s > 1 && sizeof(float) * (size_t)(M * N) * s > slab_room) break;
@@ -867,7 +879,7 @@ int planned(const char* who, const Mat& P, const Mat& Q, int K, const Plan& plan
 template <int ES, bool P_RC, bool Q_RC>
 int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, size_t room, hipStream_t st) {
   const int ksteps = dd_ceil_div(K, ROWB / ES), shapes = P_RC ? 2 : 3;
-  Plan all = plan_product(P.R, Q.R, ksteps, room, shapes), head{}, tail{};
+  Plan all = plan_product(P.R, Q.R, ksteps, room, shapes, e), head{}, tail{};
   long cut = 0;
   float best = 0.95f * all.us;
   for (int i = 0; i < shapes; ++i) {
@@ -875,8 +887,8 @@ int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, siz
     const long tm = dd_ceil_div(P.R, t.rows), tn = dd_ceil_div(Q.R, t.cols), full = tm * tn / t.slots;
     const long rows = full * t.slots / tn * t.rows;   // of whole rounds
     if (full == 0 || rows == 0 || rows >= P.R) continue;
-    const Plan rest = plan_product(P.R - rows, Q.R, ksteps, room, shapes);
-    const float us = full * (t.step * ksteps + t.rest) + rest.us + 2.f;
+    const Plan rest = plan_product(P.R - rows, Q.R, ksteps, room, shapes, e);
+    const float us = full * (t.step * ksteps + t.rest + epilogue_cost(t, e)) + rest.us + 2.f;
     if (us < best) { best = us; cut = rows; head = {i, 1, us}; tail = rest; }
   }
   if (cut == 0) return planned<ES, P_RC, Q_RC>(who, P, Q, K, all, e, slabs, st);
