@@ -282,14 +282,15 @@ int dd_quant_rows(const void* x, long ldx, int x_type, void* q, long ldq, float*
 /* y[m][n] = act(z[m][n]) + res[m][n],  z = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n].
  * x [M,K] and w [N,K] both bf16, or both e4m3 with their scales; bias, scales fp32; y bf16 or fp32, res
  * in y's type; z (bf16, NULL ok) is stored for the backward pass.  bias, res NULL ok; res may be y
- * itself (same view).  ws: partial sums of a split contraction. */
+ * itself (same view).  ws: partial sums of a split contraction, as many as fit. */
 int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
                   const float* w_scale, const float* bias, int act, const void* res, long ldr, void* y, long ldy,
                   int y_type, void* z, long ldz, int M, int N, int K, float* ws, size_t ws_bytes, void* stream);
 /* Gradients of the bf16 product (the gradient of res is dy).  dd_linear_act_bwd: dz = dy act'(z) (bf16;
  * dz may be dy or z itself; with DD_ACT_NONE z and dz are unused, dz IS dy) and dbias [N] (NULL ok);
  * dd_linear_bwd_data: dx [M,K] = dz w; dd_linear_bwd_weight: dw [N,K] = or += (accumulate) dz^T x.
- * Sums are split and added in a fixed order: equal calls give equal bits. */
+ * Sums are split and added in a fixed order: equal calls give equal bits.  ws: up to 1024 * N floats for dbias;
+ * partial sums of split contractions, as many as fit. */
 int dd_linear_act_bwd(const void* dy, long ldy, const void* z, long ldz, int act, void* dz, long lddz,
                       void* dbias, int bias_type, int accumulate, int M, int N, float* ws, size_t ws_bytes,
                       void* stream);
