@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM * BN > 16384 ? 2 : 4) k_linea
 
 // ---- few rows: single steps of serving -----------------------------------------------------------
 //
-// At most 64 rows, so the weights are read once and that read is the time.  A workgroup owns 16 weight
+// At most 128 rows, so the weights are read once and that read is the time.  A workgroup owns 16 weight
 // rows; its waves take turns along the contraction, 128 bytes of every row at a time, each with two LDS
 // buffers of its own: no barrier, the next turn's copies are in flight while 16 x 16 instructions work on
 // this one's.  At the end the waves add up in LDS: one launch, no partial sums in memory.  (Operands straight
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(64 * WV) k_linear_few(Mat P, Mat Q, int K, Epi
   copy(1);
   for (int t = 0; t < turns; ++t) {
     char* a = mine + (t & 1) * TURN;
-    __builtin_amdgcn_s_waitcnt(0x0f70 | COPIES);   // all but the next turn's copies have landed
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (COPIES & 15) | (COPIES >> 4) << 14);   // vmcnt: all but the next turn's copies have landed
     asm volatile("" ::: "memory");
     const int k0 = (wave + t * WV) * BK;
     if (K % (16 / ES) != 0 && k0 + BK > K) {        // the contraction ends inside a chunk
@@ -908,19 +908,21 @@ int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, siz
 
 template <int ES, bool P_RC, bool Q_RC>
 int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+  // Below 2^22 multiplications over a short contraction the general kernel's small tiles start and end sooner
+  // (128 x 128 x 128 4.2 us against 5.4, 8 x 64 x 72 dw 4.4 against 5.1; 70 x 64 x 1000 8.5 either way).
+  const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * ES < 8 * ROWB;
+  // 65 to 128 rows: 110 x 2391 x 577 8.4 us against 10.4 on tiles, 128 x 4096 x 1024 7.9 against 11.4.
   if constexpr (!P_RC && !Q_RC)
-    if (P.R <= 64 && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
+    if ((P.R <= 64 || (P.R <= 128 && !small)) && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
       const unsigned grid = dd_ceil_div(Q.R, 16);
       if (P.R <= 16) k_linear_few<ES, 1, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
       else if (P.R <= 32) k_linear_few<ES, 2, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
-      else k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
+      else if (P.R <= 64) k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
+      else k_linear_few<ES, 8, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
       DD_CHECK_LAUNCH(who);
       return 0;
     }
   const size_t room = ws ? ws_bytes : 0;
-  // Below 2^22 multiplications over a short contraction the general kernel's small tiles start and end sooner
-  // (128 x 128 x 128 4.2 us against 5.4, 8 x 64 x 72 dw 4.4 against 5.1; 70 x 64 x 1000 8.5 either way).
-  const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * ES < 8 * ROWB;
   if (!small && K > 0 && tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES) && (!e.res || e.ldr < (1l << 20)))
     return rounds<ES, P_RC, Q_RC>(who, P, Q, K, e, ws, room, st);
   const int bk = ROWB / ES;

@@ -264,6 +264,13 @@ def test_linear_gradients_many_tiles(hip, ref, M, N, K):
   test_linear_gradients(hip, ref, M, N, K, 'silu', F32)
 
 
+@pytest.mark.parametrize('act,yt', [(None, F32), ('gelu', BF16)])
+@pytest.mark.parametrize('M,N,K', [(65, 700, 1000), (97, 333, 1031), (128, 520, 4104), (111, 2391, 577)])
+def test_linear_a_hundred_rows(hip, ref, M, N, K, act, yt):
+  test_linear(hip, ref, M, N, K, act, yt)
+  test_linear_e4m3(hip, ref, M, N, K, act)
+
+
 @pytest.mark.parametrize('M,N,K', [(3001, 1541, 903), (2500, 2048, 1536), (16501, 1030, 1040)])
 def test_linear_e4m3_many_tiles(hip, ref, M, N, K):
   test_linear_e4m3(hip, ref, M, N, K, 'silu')
