@@ -4,8 +4,7 @@
 //   y = act(z) + res,  z[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz
 //
-// bf16 (16 x 16-bit products per matrix instruction step) or e4m3 (twice the rate, half the bytes);
-// sums in fp32.  All three products are P Q^T with different storage orders: an operand is
+// Operands bf16 or e4m3 (twice the rate, half the bytes), sums in fp32.  All three products are P Q^T with different storage orders: an operand is
 // contraction-contiguous (KC) or row-contiguous (RC).
 #include "block_core.h"
 #include <type_traits>
@@ -220,10 +219,9 @@ __global__ void __launch_bounds__(256) k_linear_any(Mat P, Mat Q, int K, int ksp
 
 // ---- tiled kernel --------------------------------------------------------------------------------
 //
-// BM x BN outputs per workgroup, WM x WN waves of 32 x 32 instruction tiles, 128 bytes of the
-// contraction per step.  A step's tiles come from global memory straight into LDS (16 bytes per lane,
-// no registers in between), two steps ahead for P (three tiles of it), one for Q (two): 160 KB at
-// 256 x 256, the whole LDS, 80 KB and two workgroups per CU at 128 x 128.
+// BM x BN outputs per workgroup, WM x WN waves, 128 bytes of the contraction per step.  A step's tiles come
+// from global memory straight into LDS (16 bytes per lane, no registers in between), two steps ahead for P (three tiles of it), one for Q (two): 160 KB at
+// 256 x 256, the whole LDS, 104 at 192 x 128, 80 and two workgroups per CU at 128 x 128.
 // Reads past an operand's end give zeros (buffer descriptor) - no bounds checks in the loop; rows may
 // start at any address.
 //
@@ -239,7 +237,8 @@ __device__ __forceinline__ int rc_swizzle(int k) { return ((k & 3) << 2) ^ ((k >
 
 // 16 bytes per lane from a buffer descriptor's range to LDS, lane after lane from offset `lds`; zeros past the range.
 // Written as assembly so that the compiler does not wait for a copy in flight at every LDS read that it cannot
-// tell apart from the copy's target; the waits that are needed are written out.
+// tell apart from the copy's target; the waits that are needed are written out.  (m0 is reserved: the
+// compiler keeps nothing in it.)
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy16(const u32x4& rs, unsigned lds, int voff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(rs) : "memory");
