@@ -4,7 +4,9 @@
 //   y = act(z) + res,  z[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz
 //
-// Operands bf16 or e4m3 (twice the rate, half the bytes), sums in fp32.  All three products are P Q^T with different storage orders: an operand is
+// Operands bf16 or e4m3 (twice the rate, half the bytes), sums in fp32.  The 8-bit instruction adds eight consecutive
+// products aligned at the largest and cuts what is below 2^-13 of it, then goes on in fp32: taken for its
+// rate, because the operands themselves are rounded to 2^-4.  All three products are P Q^T with different storage orders: an operand is
 // contraction-contiguous (KC) or row-contiguous (RC).
 #include "block_core.h"
 #include <type_traits>
@@ -910,10 +912,14 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
   // Below 2^22 multiplications over a short contraction the general kernel's small tiles start and end sooner
   // (128 x 128 x 128 4.2 us against 5.4, 8 x 64 x 72 dw 4.4 against 5.1; 70 x 64 x 1000 8.5 either way).
   const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * ES < 8 * ROWB;
-  // 65 to 128 rows: 110 x 2391 x 577 8.4 us against 10.4 on tiles, 128 x 4096 x 1024 7.9 against 11.4.
-  if constexpr (!P_RC && !Q_RC)
-    if ((P.R <= 64 || (P.R <= 128 && !small)) && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
-      const unsigned grid = dd_ceil_div(Q.R, 16);
+  // Few rows, as long as the weights' 16-row workgroups are a round or two of the chip: each reads all of x, and tiles
+  // read it less often (8 x 16384 x 1024 7.3 us against 12.5 on tiles, 8 x 32768 x 1024 14.6 against 14.2; 64 x 8192
+  // x 1024 7.6 and 11.5, 64 x 16384 x 1024 13.5 and 13.2; 128 x 4096 x 1024 7.7 and 11.5, 128 x 8192 x 1024 14.0 and 11.5;
+  // long rows and 16 of x at most: the weights' read is all there is, 8 x 65536 x 4096 91 and 123).
+  if constexpr (!P_RC && !Q_RC) {
+    const unsigned grid = dd_ceil_div(Q.R, 16);
+    const unsigned most = P.R <= 16 ? ((long)K * ES >= 8192 ? 1u << 30 : 1024) : P.R <= 64 ? 512 : P.R <= 128 && !small ? 256 : 0;
+    if (grid <= most && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
       if (P.R <= 16) k_linear_few<ES, 1, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
       else if (P.R <= 32) k_linear_few<ES, 2, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
       else if (P.R <= 64) k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
@@ -921,6 +927,7 @@ int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_
       DD_CHECK_LAUNCH(who);
       return 0;
     }
+  }
   const size_t room = ws ? ws_bytes : 0;
   if (!small && K > 0 && tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES) && (!e.res || e.ldr < (1l << 20)))
     return rounds<ES, P_RC, Q_RC>(who, P, Q, K, e, ws, room, st);

@@ -280,7 +280,8 @@ int dd_quant_rows(const void* x, long ldx, int x_type, void* q, long ldq, float*
                   void* stream);
 
 /* y[m][n] = act(z[m][n]) + res[m][n],  z = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n].
- * x [M,K] and w [N,K] both bf16, or both e4m3 with their scales; bias, scales fp32; y bf16 or fp32, res
+ * x [M,K] and w [N,K] both bf16, or both e4m3 with their scales (of eight consecutive e4m3 products, what is below
+ * 2^-13 of the largest is cut off; sums are fp32); bias, scales fp32; y bf16 or fp32, res
  * in y's type; z (bf16, NULL ok) is stored for the backward pass.  bias, res NULL ok; res may be y
  * itself (same view).  ws: partial sums of a split contraction, as many as fit. */
 int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
