@@ -8,7 +8,7 @@
 // derivative of what the forward pass computed; all arithmetic is fp32.
 //
 // Bound: HBM.  A row's elements stay in registers from their load to the last store - each input is
-// read once, each output written once - so a row belongs to one wave (C <= 1024), four (<= 4096) or
+// read once, each output written once - so a row belongs to a wave or a part of one (C <= 1024), four (<= 4096) or
 // sixteen (<= 32768), 8 or 16 elements per lane (32 past 16384) in vectors of eight: with 32 in a lane of
 // fewer waves too few fit a CU (backward, 20001 x 1542: 101 us).  The last vector of a ragged row
 // ends at the row's end and so overlaps the one before it: both lanes hold and store the same values there,
@@ -81,27 +81,34 @@ __device__ __forceinline__ void store_row(void* base, int type, long off, int l,
   }
 }
 
-// Sum (MAX: maximum) over the lanes of a row: one wave, or the whole workgroup.
+// Sum (MAX: maximum) over the lanes of a row: a part of a wave, one wave, or the whole workgroup.
 template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, int wpr, float* red) {
+__device__ __forceinline__ float row_reduce(float v, int per, float* red) {
+  if (per < 64) {
+    for (int d = per / 2; d > 0; d /= 2) {
+      const float o = __shfl_xor(v, d);
+      v = MAX ? fmaxf(v, o) : v + o;
+    }
+    return v;
+  }
   v = MAX ? wave_max(v) : wave_sum(v);
-  if (wpr == 1) return v;
+  if (per == 64) return v;
   // What this wave read is in registers before another wave stores it (s over res: vectors overlap).
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();   // the previous reduction's values have been read
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float t = red[0];
-  for (int w = 1; w < wpr; ++w) t = MAX ? fmaxf(t, red[w]) : t + red[w];
+  for (int w = 1; w < per / 64; ++w) t = MAX ? fmaxf(t, red[w]) : t + red[w];
   return t;
 }
 
 template <int NC, bool NORM, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int wpr) {
+__global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int per) {
   __shared__ float red[16];
-  const int per = 64 * wpr, l = threadIdx.x % per;
+  const int l = threadIdx.x % per;
   const long row = (long)blockIdx.x * (blockDim.x / per) + threadIdx.x / per;
-  if (row >= a.rows) return;   // whole waves; with wpr > 1 a workgroup holds one row and never leaves
+  if (row >= a.rows) return;   // all lanes of a row; a row of several waves has its workgroup for itself
   float v[NC][8], t[NC][8];
   load_row<NC>(a.x, a.xt, row * a.ldx, l, per, a.C, v);
   if (a.r) {
@@ -125,7 +132,7 @@ __global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int wpr) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += j >= dup ? v[i][j] * v[i][j] : 0.f;
     }
-    const float rstd = 1.0f / sqrtf(row_reduce<false>(ss, wpr, red) / (float)a.C + a.eps);
+    const float rstd = 1.0f / sqrtf(row_reduce<false>(ss, per, red) / (float)a.C + a.eps);
     if (a.s) store_row<NC>(a.s, a.rt, row * a.lds, l, per, a.C, v);
     if (a.rstd && l == 0) a.rstd[row] = rstd;
 #pragma unroll
@@ -139,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int wpr) {
     for (int i = 0; i < NC; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
-    m = row_reduce<true>(m, wpr, red);
+    m = row_reduce<true>(m, per, red);
     // a row of zeros (or of values whose reciprocal would overflow) is stored as zeros with scale 1
     const bool some = m >= 1e-30f;
     const float inv = some ? E4M3_MAX / m : 1.0f;
@@ -168,9 +175,9 @@ struct RmsBwdArgs {
 // A workgroup strides over the rows; every lane keeps its columns' share of dgamma in registers, the
 // four waves of a workgroup are added in LDS, one partial row per workgroup goes to the workspace.
 template <int NC, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 4 : NC == 1 ? 6 : 4) k_rms_bwd(RmsBwdArgs a, int wpr) {
-  extern __shared__ float sh[];   // 16 reduction slots | (wpr == 1) [4][C] partial sums
-  const int per = 64 * wpr, l = threadIdx.x % per, rpb = blockDim.x / per, slot = threadIdx.x / per;
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 4 : NC == 1 ? 6 : 4) k_rms_bwd(RmsBwdArgs a, int per) {
+  extern __shared__ float sh[];   // 16 reduction slots | (a wave or less per row) [rows][C] partial sums
+  const int l = threadIdx.x % per, rpb = blockDim.x / per, slot = threadIdx.x / per;
   float g[NC][8], pg[NC][8] = {};
   load_row<NC>(a.gamma, DD_F32, 0, l, per, a.C, g);
   for (long row = (long)blockIdx.x * rpb + slot; row < a.rows; row += (long)gridDim.x * rpb) {
@@ -191,7 +198,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 4 : NC == 1 ? 6 : 4
         s1 += j >= dup ? dy[i][j] * n[i][j] : 0.f;
       }
     }
-    s1 = row_reduce<false>(s1, wpr, sh) / (float)a.C;
+    s1 = row_reduce<false>(s1, per, sh) / (float)a.C;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 4 : NC == 1 ? 6 : 4
   }
   if (!a.parts) return;
   float* out = a.parts + (long)blockIdx.x * a.C;
-  if (wpr > 1) {
+  if (per > 64) {
     store_row<NC>(out, DD_F32, 0, l, per, a.C, pg);
     return;
   }
@@ -234,14 +241,22 @@ inline Shape row_shape(int C, bool forward) {
   return best;
 }
 
+// Lanes of a row: all of its waves', or the power of two that holds a narrow row, several of which share a wave
+// then (31849 x 64: forward 14.8 us with a wave each, 6.2 so; backward 17.1 and 11.3).
+inline int row_lanes(const Shape& sh, int C) {
+  int per = 64 * sh.wpr;
+  while (per > 8 && C <= 4 * per) per /= 2;
+  return per;
+}
+
 template <bool NORM>
 int launch_fwd(const RmsArgs& a, hipStream_t st) {
   const Shape sh = row_shape(a.C, true);
   DD_REQUIRE(sh.wpr > 0, "dd_rms_norm_fwd / dd_quant_rows: more than 32768 columns");
-  const int threads = sh.wpr == 16 ? 1024 : 256, rpb = threads / (64 * sh.wpr);
+  const int threads = sh.wpr == 16 ? 1024 : 256, per = row_lanes(sh, a.C), rpb = threads / per;
   const dim3 grid(dd_ceil_div(a.rows, rpb));
 #define DD_RMS_FWD(N_, T_) \
-  if (sh.nc == N_ && threads == T_) { k_rms_fwd<N_, NORM, T_><<<grid, T_, 0, st>>>(a, sh.wpr); }
+  if (sh.nc == N_ && threads == T_) { k_rms_fwd<N_, NORM, T_><<<grid, T_, 0, st>>>(a, per); }
   DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(3, 256) DD_RMS_FWD(4, 256) DD_RMS_FWD(1, 1024) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
 #undef DD_RMS_FWD
   DD_CHECK_LAUNCH(NORM ? "dd_rms_norm_fwd" : "dd_quant_rows");
@@ -289,16 +304,16 @@ extern "C" int dd_rms_norm_bwd(const void* dy, long ldy, int y_type, const void*
   DD_REQUIRE(rows == 0 || (ldy >= C && lds >= C && ldd >= C && (!dres || ldr >= C)), "dd_rms_norm_bwd: a leading dimension below C");
   const Shape sh = row_shape(C, false);
   DD_REQUIRE(sh.wpr > 0, "dd_rms_norm_bwd: more than 32768 columns");
-  const int threads = sh.wpr == 16 ? 1024 : 256, rpb = threads / (64 * sh.wpr);
+  const int threads = sh.wpr == 16 ? 1024 : 256, per = row_lanes(sh, C), rpb = threads / per;
   // as many workgroups as are resident at once (more leave a ragged last round: 20001 x 1542 with 768, 1024,
   // 1536 workgroups 90, 76, 63 us; 20000 x 1024, two vectors a lane, 59, 60, 66)
   const int grid = min(dd_ceil_div(rows, rpb), threads == 1024 ? 256 : sh.nc == 1 ? 1536 : 768);
   DD_REQUIRE(!dgamma || ws_bytes / sizeof(float) >= (size_t)grid * C, "dd_rms_norm_bwd: the workspace is too small");
   if (grid > 0) {
     const RmsBwdArgs a{dy, ldy, y_type, s, lds, res_type, dres, ldr, ds, ldd, rstd, gamma, dgamma ? ws : nullptr, rows, C};
-    const size_t lds_bytes = (16 + (sh.wpr == 1 && dgamma ? (size_t)rpb * C : 0)) * sizeof(float);
+    const size_t lds_bytes = (16 + (per <= 64 && dgamma ? (size_t)rpb * C : 0)) * sizeof(float);
 #define DD_RMS_BWD(N_, T_) \
-  if (sh.nc == N_ && threads == T_) { k_rms_bwd<N_, T_><<<grid, T_, lds_bytes, st>>>(a, sh.wpr); }
+  if (sh.nc == N_ && threads == T_) { k_rms_bwd<N_, T_><<<grid, T_, lds_bytes, st>>>(a, per); }
     DD_RMS_BWD(1, 256) DD_RMS_BWD(2, 256) DD_RMS_BWD(1, 1024) DD_RMS_BWD(2, 1024) DD_RMS_BWD(4, 1024)
 #undef DD_RMS_BWD
     DD_CHECK_LAUNCH("dd_rms_norm_bwd");

@@ -57,7 +57,8 @@ def within(out, want, tol, what=''):
 
 # ---- norm -----------------------------------------------------------------------------------------
 
-NORM_SHAPES = [(4, 8), (3, 9), (700, 1542), (2, 515), (3, 1025), (2, 4097), (1, 16390), (1, 1), (3, 7), (8, 64), (5, 1542), (130, 1024), (257, 512), (6, 2050), (2, 8192), (3, 9001), (1, 32768)]
+NORM_SHAPES = [(4, 8), (3, 9), (700, 1542), (2, 515), (3, 1025), (2, 4097), (1, 16390), (1, 1), (3, 7), (8, 64), (5, 1542), (130, 1024), (257, 512), (6, 2050), (2, 8192), (3, 9001), (1, 32768),
+               (1000, 64), (3333, 100), (77, 200), (130, 17), (61, 256)]
 
 
 @pytest.mark.parametrize('rows,C', NORM_SHAPES)
@@ -91,7 +92,7 @@ def test_norm(hip, ref, rows, C, xt, rt):
     t.whole()
 
 
-@pytest.mark.parametrize('rows,C', [(1, 5), (9, 64), (33, 1024), (4, 1542), (2, 12000)])
+@pytest.mark.parametrize('rows,C', [(1, 5), (9, 64), (33, 1024), (4, 1542), (2, 12000), (300, 100), (77, 33)])
 @pytest.mark.parametrize('norm', [True, False])
 def test_rows_to_e4m3(hip, ref, rows, C, norm):
   x, r, g = rnd(rows, C, seed=7, dtype=BF16), rnd(rows, C, seed=8), 1 + rnd(C, seed=9, scale=0.1)
@@ -142,7 +143,7 @@ def test_norm_rows_do_not_mix(hip):
   assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[4, 1541])) and bool((y[6] == 0).all())
 
 
-@pytest.mark.parametrize('C', [1024, 1542, 4099, 16389])
+@pytest.mark.parametrize('C', [33, 100, 1024, 1542, 4099, 16389])
 @pytest.mark.parametrize('rt', [F32, BF16])
 def test_norm_in_place_at_any_width(hip, C, rt):
   """s over res and ds over dres give what separate outputs give: no wave of a row reads what another wrote."""
