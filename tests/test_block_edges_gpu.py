@@ -1,0 +1,96 @@
+"""Operators of the residual recurrent block at the edges of their ranges, on the GPU: relative precision where values
+are small or gates are all but shut, in-place forms, what surrounds a view, and every variant a size can select.
+
+Tolerances as in test_block_ops_gpu.py: u = 2^-24, half a step of the stored type, and the named roundings between.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, BF16, FP8 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+HALF = {F32: U, BF16: 2.0 ** -8}
+
+
+def rnd(*shape, seed=0, scale=1.0, dtype=F32):
+  g = torch.Generator().manual_seed(seed)
+  return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def close(out, want, rel, what):
+  """|out - want| <= (rel + half a step of out's type) |want|, elementwise."""
+  o, w = out.detach().cpu().double(), want.double()
+  lim = (rel + HALF[out.dtype] * (1 + rel)) * w.abs() + 1e-37
+  over = (o - w).abs() > lim
+  if bool(over.any()) or not bool(torch.isfinite(o).all()):
+    i = int((over | ~torch.isfinite(o)).reshape(-1).nonzero()[0])
+    raise AssertionError(f'{what}: {int(over.sum())} of {over.numel()} off, first at {i}: {float(o.reshape(-1)[i])} '
+                         f'for {float(w.reshape(-1)[i])}')
+
+
+# ---- scan: relative precision ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_a_decay_that_is_all_but_shut(hip, dt):
+  """The decay sigmoid(-v) and what is multiplied with it, to a few u of themselves however far v is out."""
+  v = torch.cat([torch.arange(-30, 31, dtype=F32) * 0.5, torch.tensor([17.0, 20.0, 24.0, 40.0, 80.0, -40.0, -80.0])])
+  D = v.numel()
+  u, c = v[None].to(dt), torch.zeros(1, D, dtype=dt)
+  h, hT, h0 = torch.zeros(1, D, device='cuda', dtype=dt), torch.zeros(1, D, device='cuda'), torch.ones(1, D, device='cuda')
+  hip.gated_scan_fwd(u.cuda(), c.cuda(), h, 1, h0=h0, hT=hT, shift=-1.0, cand=None)
+  x = u.double() - 1.0
+  a = torch.sigmoid(-x)
+  # the exponent of e^-v is off by (1.5 |v| + 2) u in all (its rounding, the constant's), and sum, reciprocal,
+  # product and exponential by 8 u
+  rel = (1.5 * x.abs() + 10) * U
+  close(hT, a, rel, 'hT')
+  close(h, a, rel, 'h')
+  du, dc, dh0 = (torch.zeros(1, D, device='cuda', dtype=t) for t in (dt, dt, F32))
+  hip.gated_scan_bwd(torch.ones(1, D, device='cuda', dtype=dt), u.cuda(), c.cuda(), h, du, dc, 1, h0=h0, dh0=dh0, shift=-1.0, cand=None)
+  close(dh0, a, rel, 'dh0')
+  close(du, -a * torch.sigmoid(x), 2 * rel + 4 * U, 'du')
+  close(dc, torch.sigmoid(x), rel, 'dc')
+
+
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_small_candidates(hip, dt, gate):
+  """tanh of small and large candidates, to its own size: in h, and in du (no state) or di (with an input gate)."""
+  m = torch.cat([2.0 ** -torch.arange(0, 40, dtype=F32), 0.0625 * (1 + torch.tensor([-2.0, -1.0, 0.0, 1.0, 2.0]) / 128),
+                 torch.tensor([0.28125, 0.30078125, 0.3125, 2.0, 5.0, 12.0, 50.0])])
+  c = torch.cat([m, -m])[None].to(dt)
+  D = c.shape[1]
+  u, i = torch.full((1, D), 0.5, dtype=dt), torch.full((1, D), 0.25, dtype=dt)
+  kw = dict(i=i.cuda()) if gate else {}
+  h, hT = torch.zeros(1, D, device='cuda', dtype=dt), torch.zeros(1, D, device='cuda')
+  hip.gated_scan_fwd(u.cuda(), c.cuda(), h, 1, hT=hT, shift=0.0, **kw)
+  g = torch.sigmoid(i.double() if gate else u.double())
+  want = g * torch.tanh(c.double())
+  # tanh's exponential form: 1 - 2 r from 1/16 on (bf16), r to 4 u, so 64 u of itself there; (1 - e) / (1 + e) from 0.3 on
+  # (fp32) to 9 u; the gate 8 u
+  rel = (80 if dt == BF16 else 24) * U
+  close(hT, want, rel, 'hT')
+  close(h, want, rel, 'h')
+  du, dc, di = (torch.zeros(1, D, device='cuda', dtype=dt) for _ in range(3))
+  kb = dict(di=di, **kw) if gate else {}
+  hip.gated_scan_bwd(torch.ones(1, D, device='cuda', dtype=dt), u.cuda(), c.cuda(), h, du, dc, 1, shift=0.0, **kb)
+  close(di if gate else du, torch.tanh(c.double()) * g * (1 - g), rel + 16 * U, 'di' if gate else 'du')
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_long_memories(hip, dt):
+  """Two thousand steps of nearly shut and nearly open gates: what survives of the initial state, to its own size."""
+  T, D = 2000, 8
+  v = torch.tensor([-9.0, -8.0, -7.5, -7.0, -6.5, -6.0, -5.5, 14.0])
+  u, c = v.expand(T, D).contiguous().to(dt), torch.zeros(T, D, dtype=dt)
+  h, hT = torch.zeros(T, D, device='cuda', dtype=dt), torch.zeros(1, D, device='cuda')
+  steps = 2000
+  u[1:, 7] = -12.0
+  hip.gated_scan_fwd(u.cuda(), c.cuda(), h, T, h0=torch.ones(1, D, device='cuda'), hT=hT, shift=0.0, cand=None)
+  want = torch.sigmoid(-u.double()).log().sum(0, keepdim=True).exp()
+  # a factor is off by u |v| (1 - a) through the exponent of e^-v, which (1 - a) makes less than u, and 3 u through sum,
+  # reciprocal and product; as much again for the multiplications
+  close(hT, want, steps * 6 * U, 'hT')
