@@ -89,6 +89,17 @@ __device__ __forceinline__ float phi_of(float c, int tanh_c) {
     return tanh_f(c);
   }
 }
+// ... and its slope 1 - phi^2 = 4 e r^2, e = e^-2|c|, r = 1 / (1 + e), not by a difference either.
+template <bool BRIEF>
+__device__ __forceinline__ void phi_slope(float c, int tanh_c, float& phi, float& slope) {
+  phi = c;
+  slope = 1.f;
+  if (!tanh_c) return;
+  const float e = fast_exp(-2.0f * fabsf(c)), r = fast_rcp(1.0f + e), er = e * r;
+  slope = 4.0f * r * er;
+  if constexpr (BRIEF) phi = fabsf(c) < 0.0625f ? c * fma_(c * c, -1.f / 3, 1.f) : copysignf(fma_(-2.0f, er, 1.0f), c);
+  else phi = tanh_f(c);
+}
 __device__ __forceinline__ float sigmoid1(float x) { return fast_rcp(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f)); }
 
 // Bit s: step o0 + s (in scan order, of `n`) of sequence b starts anew.  One load for the wave's run.
@@ -339,14 +350,16 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
       for (int j = 0; j < VC; ++j) {
         const float gr = dh[s][j] + in[j];             // d loss / d h[t]
         in[j] = restart ? 0.f : q[s][j] * gr;
-        const float phi = phi_of<BRIEF>(c[s][j], p.tanh_c);
-        const float slope = p.tanh_c ? fma_(-phi, phi, 1.f) : 1.f;
+        float phi, slope;
+        phi_slope<BRIEF>(c[s][j], p.tanh_c, phi, slope);
         const float before = restart ? 0.f : hp[s][j];
         const float gz = gr * z[s][j];
         if constexpr (GATE) {
-          const float w = sigmoid1(gi[s][j]), gw = gr * w;
+          float w, w1;
+          gates(gi[s][j], 0.f, w, w1);
+          const float gw = gr * w;
           du[j] = -gz * q[s][j] * before;
-          di[j] = gw * phi * (1.f - w);
+          di[j] = gw * phi * w1;
           dc[j] = gw * slope;
         } else {
           du[j] = gz * q[s][j] * (phi - before);

@@ -94,3 +94,25 @@ def test_long_memories(hip, dt):
   # a factor is off by u |v| (1 - a) through the exponent of e^-v, which (1 - a) makes less than u, and 3 u through sum,
   # reciprocal and product; as much again for the multiplications
   close(hT, want, steps * 6 * U, 'hT')
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_slopes_of_saturated_candidates_and_gates(hip, dt):
+  """dc where tanh is all but flat and di where the input gate is all but open or shut: to their own size."""
+  m = torch.arange(1, 33, dtype=F32)
+  c = torch.cat([m, -m])[None].to(dt)
+  D = c.shape[1]
+  i = (1.25 * torch.cat([m, -m]))[None].to(dt)
+  u = torch.zeros(1, D, dtype=dt)
+  one = torch.ones(1, D, device='cuda', dtype=dt)
+  du, dc, di = (torch.zeros(1, D, device='cuda', dtype=dt) for _ in range(3))
+  hip.gated_scan_bwd(one, u.cuda(), c.cuda(), one, du, dc, 1, i=i.cuda(), di=di, shift=0.0)
+  x, g = c.double(), i.double()
+  w = torch.sigmoid(g)
+  slope = 4 * torch.exp(-2 * x.abs()) / (1 + torch.exp(-2 * x.abs())) ** 2
+  # the exponent 2 |c| of e is off by 3 |c| u (its rounding and the constant's), |i|'s by 1.5 |i| u; e, 1 + e and its
+  # reciprocal twice, products: 16 u
+  close(dc, w * slope, (3 * x.abs() + 1.5 * g.abs() + 24) * U, 'dc')
+  close(di, torch.tanh(x) * w * torch.sigmoid(-g), (3 * g.abs() + 32) * U + (80 if dt == BF16 else 24) * U, 'di')
+  hip.gated_scan_bwd(one, u.cuda(), c.cuda(), one, du, dc, 1, shift=0.0)
+  close(dc, 0.5 * slope, (3 * x.abs() + 24) * U, 'dc without an input gate')
