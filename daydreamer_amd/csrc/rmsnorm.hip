@@ -147,15 +147,15 @@ __global__ void __launch_bounds__(THREADS) k_rms_fwd(RmsArgs a, int per) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
     m = row_reduce<true>(m, per, red);
-    // a row of zeros (or of values whose reciprocal would overflow) is stored as zeros with scale 1
-    const bool some = m >= 1e-30f;
-    const float inv = some ? E4M3_MAX / m : 1.0f;
-    if (l == 0) a.scale[row] = some ? m / E4M3_MAX : 1.0f;
+    // a row of zeros is stored as zeros with scale 1; one so small that 448 / m would overflow is brought up by an exact
+    // power of two first (its scale may be subnormal, and is rounded as those are)
+    const float up = m < 0x1p-100f ? 0x1p64f : 1.0f, inv = m > 0.f ? E4M3_MAX / (m * up) : 1.0f;
+    if (l == 0) a.scale[row] = m > 0.f ? m / E4M3_MAX : 1.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = v[i][j] * inv;   // at most 448 but for the roundings; a NaN stays one
+        const float t = v[i][j] * up * inv;   // at most 448 but for the roundings; a NaN stays one
         v[i][j] = t > E4M3_MAX ? E4M3_MAX : t < -E4M3_MAX ? -E4M3_MAX : t;
       }
   }

@@ -263,7 +263,7 @@ int dd_gru_cell_bwd(const float* dhn, long lddn, const float* z3, long ldz,
 /* s = round(x + res) in res_type;  y = s / sqrt(mean(s^2) + eps) * gamma, from s as it is stored.
  * res may be NULL (s = x, stored only if s is given); s may be res or x itself (same view).  With
  * y_type DD_E4M3 a row of y is divided by scale[row] = max|y| / 448 and rounded (nearest even); a row
- * whose largest magnitude is below 1e-30 becomes zeros with scale 1.  rstd [rows] may be NULL.
+ * of zeros has scale 1.  rstd [rows] may be NULL.
  * C <= 32768; x, res fp32 or bf16. */
 int dd_rms_norm_fwd(const void* x, long ldx, int x_type, const void* res, long ldr, int res_type,
                     void* s, long lds, const float* gamma, void* y, long ldy, int y_type,

@@ -312,7 +312,7 @@ class RefOps:
   def quant_rows(self, x, q, scale):
     x = x.double()
     most = x.abs().amax(1, keepdim=True)
-    some = most >= 1e-30
+    some = most > 0
     q.copy_(self._e4m3(torch.where(some, x * (448.0 / torch.where(some, most, torch.ones_like(most))), x)))
     scale.copy_(torch.where(some, most / 448.0, torch.ones_like(most))[:, 0])
 

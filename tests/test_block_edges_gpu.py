@@ -116,3 +116,28 @@ def test_slopes_of_saturated_candidates_and_gates(hip, dt):
   close(di, torch.tanh(x) * w * torch.sigmoid(-g), (3 * g.abs() + 32) * U + (80 if dt == BF16 else 24) * U, 'di')
   hip.gated_scan_bwd(one, u.cuda(), c.cuda(), one, du, dc, 1, shift=0.0)
   close(dc, 0.5 * slope, (3 * x.abs() + 24) * U, 'dc without an input gate')
+
+
+# ---- rows in 8 bits -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+@pytest.mark.parametrize('C', [5, 64, 1030, 9001])
+def test_small_rows_to_e4m3(hip, dt, C):
+  """Rows down to the smallest numbers are scaled as any other row is; a row of zeros is zeros with scale 1."""
+  sizes = torch.tensor([1.0, 1e-20, 1e-29, 1e-31, 1e-35, 2e-36, 1e-36, 1e-38, 1e-40, 1e-42, 0.0])
+  x = rnd(1, C, seed=1).double().clamp(-3, 3)
+  x[0, 0] = 3.5
+  x = (x * sizes.double()[:, None]).to(dt)
+  q, scale = torch.zeros(len(sizes), C, device='cuda', dtype=FP8), torch.zeros(len(sizes), device='cuda')
+  hip.quant_rows(x.cuda(), q, scale)
+  most = x.double().abs().amax(1)
+  want = torch.where(most > 0, most / 448, torch.ones_like(most))
+  # half a step of fp32, a subnormal one below the smallest normal number
+  assert bool(((scale.cpu().double() - want).abs() <= 2 * U * want + 2.0 ** -150).all())
+  got = q.cpu().float().double()
+  # in units of the exact scale: half a step of e4m3 (2^-4 of the value, 2^-10 below its smallest normal), and 4 u of 448
+  # through the reciprocal's and the products' roundings
+  v = x.double() / want[:, None]
+  assert bool(((got - v).abs() <= 2.0 ** -4 * v.abs() + 2.0 ** -10 + 4 * U * 448).all())
+  assert bool((got.abs().amax(1)[most > 0] == 448).all()) and bool((got[most == 0] == 0).all())
