@@ -42,11 +42,36 @@ const char* names(unsigned types) {
   }
 }
 
+// Memory of a view: rows of `width` bytes, `step` bytes from one to the next.
+struct Span {
+  long at = 0, step = 0, width = 0, rows = 0;
+  long end() const { return at + (rows - 1) * step + width; }
+};
+inline long floor_div(long a, long b) { return a / b - (a % b != 0 && (a < 0) != (b < 0)); }
+// Is there a k in [lo, hi] with low < at + k step < high (all exclusive)?
+inline bool any_between(long at, long step, long lo, long hi, long low, long high) {
+  if (step == 0) return low < at && at < high;
+  return std::max(lo, floor_div(low - at, step) + 1) <= std::min(hi, floor_div(high - at - 1, step));
+}
+inline bool overlap(const Span& a, const Span& b) {
+  if (a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0 || a.end() <= b.at || b.end() <= a.at) return false;
+  // rows k of a and j of b share bytes if b.at + j step - a.width < a.at + k step < b.at + j step + b.width
+  if (a.step == b.step) return any_between(a.at, a.step, 1 - b.rows, a.rows - 1, b.at - a.width, b.at + b.width);
+  const Span &few = a.rows < b.rows ? a : b, &many = a.rows < b.rows ? b : a;
+  for (long j = 0; j < few.rows; ++j) {
+    const long at = few.at + j * few.step;
+    if (any_between(many.at, many.step, 0, many.rows - 1, at - many.width, at + few.width)) return true;
+  }
+  return false;
+}
+
 struct View {
   void* p = nullptr;
   long ld = 0;
   int type = DD_F32;
+  Span m;
   unsigned mask() const { return 1u << type; }
+  operator Span() const { return m; }
 };
 
 const at::Tensor& tensor(PyObject* o, const char* what, int device, unsigned types, int& type) {
@@ -99,6 +124,8 @@ struct Args {
     v.p = t.data_ptr();
     v.ld = rows > 1 ? t.stride(0) : std::max<long>(cols, t.stride(0));
     if (v.ld < cols) refuse("%s: rows overlap", what);
+    const long es = t.element_size();
+    v.m = {(long)(uintptr_t)v.p, rows > 1 ? v.ld * es : 0, cols * es, v.p ? rows : 0};
     return v;
   }
   // n contiguous values
@@ -120,11 +147,18 @@ struct Args {
   }
 };
 
-// What is written is none of these operands, whose elements other workgroups read later.  (Views of one buffer
-// that overlap in another way look like the columns of one product, side by side, and are not told apart.)
-void apart(const void* out, const char* what, std::initializer_list<const void*> operands) {
-  for (const void* p : operands)
-    if (out && p == out) refuse("%s is one of the other operands", what);
+// Contiguous values as a span; NULL: nothing.
+Span line(const void* p, long n, int es = 4) { return {(long)(uintptr_t)p, 0, n * es, p ? 1 : 0}; }
+
+// What is written shares no memory with these operands, whose elements other workgroups read or write.
+void apart(const Span& out, const char* what, std::initializer_list<Span> operands) {
+  for (const Span& o : operands)
+    if (overlap(out, o)) refuse("%s shares memory with another operand", what);
+}
+// ... except with this one if it is the same view: every element is read by the lane, or behind the wait, that writes it.
+void apart_or_same(const View& out, const char* what, const View& in) {
+  const bool same = out.p == in.p && out.type == in.type && out.m.step == in.m.step && out.m.rows == in.m.rows;
+  if (!same && overlap(out, in)) refuse("%s shares memory with an operand that it may be, but is another view of it", what);
 }
 
 template <typename F>
@@ -169,7 +203,13 @@ void rms_norm_fwd(const Args& a) {
   if ((y.type == DD_E4M3) != a.given(6)) refuse("scale goes with an e4m3 y, and only with it");
   const float eps = a.real(7);
   if (rows == 0) return;
-  apart(y.p, "y", {x.p, r.p, s.p});
+  const Span g = line(gamma, C), inv = line(rstd, rows), sc = line(scale, rows);
+  apart(y, "y", {x, r, s, g, inv, sc});
+  apart(s, "s", {g, inv, sc});
+  apart_or_same(s, "s", x);
+  apart_or_same(s, "s", r);
+  apart(inv, "rstd", {x, r, g, sc});
+  apart(sc, "scale", {x, r, g});
   call("dd_rms_norm_fwd", [&] {
     return dd_rms_norm_fwd_(x.p, x.ld, x.type, r.p, r.ld, rt, s.p, s.ld, gamma, y.p, y.ld, y.type, rstd, scale, (int)rows, (int)C,
                             eps, a.stream);
@@ -184,8 +224,10 @@ void rms_norm_bwd(const Args& a) {
              dr = a.view(6, "dres", rows, C, s.mask(), true);
   const float *rstd = (const float*)a.flat(2, "rstd", rows, F32, false), *gamma = (const float*)a.flat(3, "gamma", C, F32, false);
   float* dgamma = (float*)a.flat(5, "dgamma", C);
-  apart(ds.p, "ds", {dy.p, s.p});
-  apart(dgamma, "dgamma", {gamma, rstd});
+  const Span g = line(gamma, C), dg = line(dgamma, C), inv = line(rstd, rows);
+  apart(ds, "ds", {dy, s, g, inv, dg});
+  apart_or_same(ds, "ds", dr);
+  apart(dg, "dgamma", {dy, s, g, inv, dr});
   const int accumulate = (int)a.number(7);
   float* ws = (float*)a.number(8);
   const size_t bytes = (size_t)a.number(9);
@@ -201,6 +243,8 @@ void quant_rows(const Args& a) {
   a.shape(0, "x", rows, C);
   const View x = a.view(0, "x", rows, C, REAL), q = a.view(1, "q", rows, C, E4M3);
   float* scale = (float*)a.flat(2, "scale", rows, F32, false);
+  apart(q, "q", {x, line(scale, rows)});
+  apart(line(scale, rows), "scale", {x});
   call("dd_quant_rows", [&] { return dd_quant_rows_(x.p, x.ld, x.type, q.p, q.ld, scale, (int)rows, (int)C, a.stream); });
 }
 
@@ -219,8 +263,10 @@ void linear_fwd(const Args& a) {
   float* ws = (float*)a.number(9);
   const size_t bytes = (size_t)a.number(10);
   if (M == 0) return;
-  apart(y.p, "y", {x.p, w.p, z.p, bias});
-  apart(z.p, "z", {x.p, w.p, r.p});
+  const Span b = line(bias, N), sx = line(xs, M), sw = line(wsc, N);
+  apart(y, "y", {x, w, z, b, sx, sw});
+  apart_or_same(y, "y", r);
+  apart(z, "z", {x, w, r, b, sx, sw});
   call("dd_linear_fwd", [&] {
     return dd_linear_fwd_(x.p, x.ld, w.p, w.ld, x.type, xs, wsc, bias, act, r.p, r.ld, y.p, y.ld, y.type, z.p, z.ld, (int)M,
                           (int)N, (int)K, ws, bytes, a.stream);
@@ -242,9 +288,15 @@ void linear_bwd(const Args& a) {
   const int accumulate = (int)a.number(9);
   float* ws = (float*)a.number(10);
   const size_t bytes = (size_t)a.number(11);
-  apart(dz.p == dy.p ? nullptr : dz.p, "dz", {x.p, w.p});
-  apart(dx.p, "dx", {dy.p, dz.p, x.p, w.p, dw.p, db});   // (x: dw reads it behind dx)
-  apart(dw.p, "dw", {dy.p, dz.p, x.p, w.p, db});
+  const Span b = line(db, N, bias_type == DD_F32 ? 4 : 2);
+  if (act != DD_ACT_NONE) {
+    apart(dz, "dz", {x, w});
+    apart_or_same(dz, "dz", dy);
+    apart_or_same(dz, "dz", z);
+  }
+  apart(dx, "dx", {dy, dz, x, w, dw, b});   // (x: dw reads it behind dx)
+  apart(dw, "dw", {dy, dz, x, w, b});
+  apart(b, "dbias", {dy, dz, x, w, z});
   if (act != DD_ACT_NONE || db)
     call("dd_linear_act_bwd", [&] {
       return dd_linear_act_bwd_(dy.p, dy.ld, z.p, z.ld, act, dz.p, dz.ld, db, bias_type, accumulate, (int)M, (int)N, ws, bytes, a.stream);
@@ -264,6 +316,7 @@ struct Scan {
   long rows, D, T, B, fstride = 0;
   View u, c, i;
   const float* first = nullptr;
+  Span restarts;
   float shift;
   int tanh;
   Scan(const Args& a, int at_u, int at_c, int at_i, int at_T, int at_first, int at_shift, int at_cand) {
@@ -280,6 +333,7 @@ struct Scan {
       if (t.dim() != 1 || t.size(0) != rows) refuse("first is not [%ld]", rows);
       first = (const float*)t.data_ptr();
       fstride = rows > 1 ? t.stride(0) : 1;
+      restarts = {(long)(uintptr_t)first, fstride * 4, 4, fstride ? rows : 1};
     }
     shift = a.real(at_shift);
     PyObject* cand = a.a[at_cand];
@@ -295,7 +349,10 @@ void gated_scan_fwd(const Args& a) {
   const View h = a.view(2, "h", s.rows, s.D, s.u.mask());
   const float* h0 = (const float*)a.flat(6, "h0", s.B * s.D);
   float* hT = (float*)a.flat(7, "hT", s.B * s.D);
-  apart(h.p, "h", {s.u.p, s.c.p, s.i.p, h0, hT});
+  const Span from = line(h0, s.B * s.D), to = line(hT, s.B * s.D);
+  apart(h, "h", {s.u, s.c, s.i, s.restarts, from, to});
+  apart(to, "hT", {s.u, s.c, s.i, s.restarts});
+  if (hT != h0) apart(to, "hT", {from});
   float* ws = (float*)a.number(10);
   const size_t bytes = (size_t)a.number(11);
   call("dd_gated_scan_fwd", [&] {
@@ -313,10 +370,12 @@ void gated_scan_bwd(const Args& a) {
   if (a.given(7) != a.given(8)) refuse("di goes with i, and only with it");
   const float *h0 = (const float*)a.flat(10, "h0", s.B * s.D), *dhT = (const float*)a.flat(11, "dhT", s.B * s.D);
   float* dh0 = (float*)a.flat(12, "dh0", s.B * s.D);
-  apart(du.p, "du", {dh.p, s.u.p, s.c.p, s.i.p, h.p, dc.p, di.p});
-  apart(dc.p, "dc", {dh.p, s.u.p, s.c.p, s.i.p, h.p, di.p});
-  apart(di.p, "di", {dh.p, s.u.p, s.c.p, s.i.p, h.p});
-  apart(dh0, "dh0", {h0});
+  const Span from = line(h0, s.B * s.D), end = line(dhT, s.B * s.D), start = line(dh0, s.B * s.D);
+  apart(du, "du", {dh, s.u, s.c, s.i, h, s.restarts, from, end, start, dc, di});
+  apart(dc, "dc", {dh, s.u, s.c, s.i, h, s.restarts, from, end, start, di});
+  apart(di, "di", {dh, s.u, s.c, s.i, h, s.restarts, from, end, start});
+  apart(start, "dh0", {dh, s.u, s.c, s.i, h, s.restarts, from});
+  if (dh0 != dhT) apart(start, "dh0", {end});
   float* ws = (float*)a.number(15);
   const size_t bytes = (size_t)a.number(16);
   call("dd_gated_scan_bwd", [&] {
@@ -338,11 +397,22 @@ PyObject* bind(PyObject*, PyObject* handle) {
   Py_RETURN_NONE;
 }
 
+// overlap(at, step, width, rows, at, step, width, rows), in bytes: do two views share memory?
+PyObject* share(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  long v[8];
+  if (n != 8) { PyErr_SetString(PyExc_TypeError, "overlap: 8 numbers are needed"); return nullptr; }
+  for (int k = 0; k < 8; ++k) {
+    v[k] = PyLong_AsLong(a[k]);
+    if (v[k] == -1 && PyErr_Occurred()) return nullptr;
+  }
+  return PyBool_FromLong(overlap({v[0], v[1], v[2], v[3]}, {v[4], v[5], v[6], v[7]}));
+}
+
 #define DD_METHOD(name, n) {#name, (PyCFunction)(void*)entry<n, name>, METH_FASTCALL, nullptr}
 PyMethodDef METHODS[] = {
     DD_METHOD(rms_norm_fwd, 8), DD_METHOD(rms_norm_bwd, 10), DD_METHOD(quant_rows, 3), DD_METHOD(linear_fwd, 11),
     DD_METHOD(linear_bwd, 12), DD_METHOD(gated_scan_fwd, 12), DD_METHOD(gated_scan_bwd, 17),
-    {"bind", bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    {"overlap", (PyCFunction)(void*)share, METH_FASTCALL, nullptr}, {"bind", bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_block", nullptr, -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,40 @@
+"""Host logic of the residual recurrent block on the CPU: what the binding takes for shared memory, and which kernel a
+product of a size takes."""
+
+import random
+
+import pytest
+
+from daydreamer_amd import hipops
+
+
+def touched(at, step, width, rows):
+  return {at + k * step + j for k in range(rows) for j in range(width)}
+
+
+def test_views_that_share_memory():
+  """Against sets of bytes: columns of one buffer side by side, rows in between, another stride, single rows, nothing."""
+  hipops.load_library()
+  from daydreamer_amd import _block
+  rng = random.Random(0)
+  seen = {True: 0, False: 0}
+  for _ in range(20000):
+    views = []
+    for _ in range(2):
+      width, rows = rng.randint(0, 6), rng.randint(0, 5)
+      step = rng.choice([8, 8, 8, 16, 24, 11, width])
+      step = 0 if rows <= 1 else max(step, width)
+      views.append((rng.randint(1000, 1060), step, width, rows))
+    a, b = views
+    want = bool(touched(*a) & touched(*b))
+    assert _block.overlap(*a, *b) == want == _block.overlap(*b, *a), (a, b)
+    seen[want] += 1
+  assert min(seen.values()) > 2000
+  for a, b, want in [((0, 4096, 64, 1 << 30), (64, 4096, 64, 1 << 30), False),       # side by side
+                     ((0, 4096, 65, 1 << 30), (64, 4096, 64, 1 << 30), True),
+                     ((0, 4096, 64, 1 << 30), (4096 * (1 << 30), 4096, 64, 1 << 30), False),   # one behind the other
+                     ((0, 4096, 64, 1 << 30), (4096 * ((1 << 30) - 1) + 63, 0, 1, 1), True),
+                     ((0, 4096, 64, 1 << 30), (4096 * ((1 << 30) - 1) + 64, 0, 1, 1), False)]:
+    assert _block.overlap(*a, *b) is want
+  with pytest.raises(TypeError):
+    _block.overlap(1, 2, 3)

@@ -141,3 +141,51 @@ def test_small_rows_to_e4m3(hip, dt, C):
   v = x.double() / want[:, None]
   assert bool(((got - v).abs() <= 2.0 ** -4 * v.abs() + 2.0 ** -10 + 4 * U * 448).all())
   assert bool((got.abs().amax(1)[most > 0] == 448).all()) and bool((got[most == 0] == 0).all())
+
+
+# ---- operands that share memory -------------------------------------------------------------------
+
+
+def test_shared_memory_is_refused(hip):
+  """Another view of an operand that may be the output itself, parts of an operand, and vectors inside a matrix."""
+  buf = torch.zeros(64, 64, device='cuda', dtype=BF16)
+  big = torch.zeros(64, 64, device='cuda')
+  x, w = torch.zeros(16, 16, device='cuda', dtype=BF16), torch.zeros(16, 16, device='cuda', dtype=BF16)
+  y, v, g = (torch.zeros(16, 16, device='cuda', dtype=BF16) for _ in range(3))
+  one, ones = torch.ones(16, device='cuda'), torch.ones(16, device='cuda')
+  flat = buf.reshape(-1)[:256].view(16, 16)                          # rows of 16 next to each other
+  a, b = buf[:16, :16], buf[1:17, :16]                               # rows 64 apart, one row further
+  state = big.reshape(-1)[:64].view(4, 16)
+  calls = [
+      lambda: hip.linear_fwd(x, w, flat, res=a),                     # the same address, another stride
+      lambda: hip.linear_fwd(x, w, a, res=b),                        # one row further
+      lambda: hip.linear_fwd(x, w, a, z=buf[:16, 8:24]),             # half of its columns
+      lambda: hip.linear_fwd(x, w, big[:16, :16], bias=big[3, 4:20]),
+      lambda: hip.linear_fwd(flat, w, a),
+      lambda: hip.linear_bwd(a, x, w, act='silu', z=v, dz=b),
+      lambda: hip.linear_bwd(a, x, w, act='silu', z=b, dz=b[:, :16], dx=buf[2:18, :16]),
+      lambda: hip.linear_bwd(x, x, w, dw=g, act='silu', z=v, dz=x),  # dw reads x behind dz
+      lambda: hip.linear_bwd(y, x, w, dx=a, dw=b),
+      lambda: hip.linear_bwd(y, x, w, dbias=y[0]),
+      lambda: hip.rms_norm_fwd(x, one, y, res=a, s=flat),
+      lambda: hip.rms_norm_fwd(x, one, y, res=a, s=b),
+      lambda: hip.rms_norm_fwd(a, one, y, s=flat),
+      lambda: hip.rms_norm_fwd(x, big[0, :16], y, res=big[:16, :16], s=big[:16, :16]),
+      lambda: hip.rms_norm_fwd(x, one, y, rstd=one),
+      lambda: hip.rms_norm_bwd(y, x, one, ones, a, dres=b),
+      lambda: hip.rms_norm_bwd(y, x, one, ones, v, dgamma=one),
+      lambda: hip.quant_rows(buf[:16, :16], buf.view(FP8)[:16, :16], one),
+      lambda: hip.gated_scan_fwd(x, w, y, 4, h0=state, hT=big.reshape(-1)[16:80].view(4, 16)),
+      lambda: hip.gated_scan_fwd(big[:16, :16], big[16:32, :16], big[32:48, :16], 4, first=big[40:56, 3]),
+      lambda: hip.gated_scan_fwd(x, w, a, 4, i=b),
+      lambda: hip.gated_scan_bwd(y, x, w, v, a, b, 4),
+      lambda: hip.gated_scan_bwd(y, x, w, v, a, g, 4, dhT=state, dh0=big.reshape(-1)[16:80].view(4, 16)),
+  ]
+  for k, call in enumerate(calls):
+    with pytest.raises(AssertionError):
+      call()
+      pytest.fail(f'call {k} was not refused')
+  # side by side, and rows in between: no memory is shared
+  hip.linear_fwd(buf[:16, :16], w, buf[:16, 16:32], res=buf[:16, 32:48], z=buf[16:32, :16])
+  hip.linear_fwd(buf[0:32:2, :16], w, buf[1:32:2, :16])
+  hip.gated_scan_fwd(buf[:16, :16], buf[:16, 16:32], buf[:16, 32:48], 4)
