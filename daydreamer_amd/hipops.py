@@ -131,6 +131,17 @@ EXPORTS = sorted(list(_SIGS) + ['dd_version', 'dd_last_error'])
 ABI_VERSION = 12   # include/daydreamer_hip.h DD_ABI_VERSION
 
 
+class _Missing:
+  """Stands for daydreamer_amd/_block.so where it is not built or not loadable: its first use says so."""
+
+  def __init__(self, why):
+    self.why = why
+
+  def __getattr__(self, name):
+    raise RuntimeError(f'daydreamer_amd/_block.so not found or not loadable ({self.why}): build it with '
+                       f'__graft_entry__.build() (make -C daydreamer_amd/csrc).')
+
+
 def load_library():
   """Load the shared library and declare prototypes.  Raises if missing."""
   global _lib
@@ -151,12 +162,11 @@ def load_library():
     raise RuntimeError(f'{_LIB_PATH} has ABI version {lib.dd_version()}, this binding needs '
                        f'{ABI_VERSION}: rebuild it (make -C daydreamer_amd/csrc)')
   global _block
-  try:   # native binding of the residual recurrent block (csrc/block_bind.cpp)
+  try:   # native binding of the residual recurrent block (csrc/block_bind.cpp); nothing else needs it
     from . import _block
+    _block.bind(lib._handle)
   except ImportError as e:
-    raise RuntimeError(f'daydreamer_amd/_block.so not found or not loadable ({e}): build it with '
-                       f'__graft_entry__.build() (make -C daydreamer_amd/csrc).') from e
-  _block.bind(lib._handle)
+    _block = _Missing(str(e))
   _lib = lib
   return lib
 

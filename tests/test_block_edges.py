@@ -2,6 +2,8 @@
 product of a size takes."""
 
 import random
+import subprocess
+import sys
 
 import pytest
 
@@ -38,3 +40,23 @@ def test_views_that_share_memory():
     assert _block.overlap(*a, *b) is want
   with pytest.raises(TypeError):
     _block.overlap(1, 2, 3)
+
+
+def test_the_library_loads_without_the_native_binding():
+  """Without _block.so everything but the block's methods works; those say what is missing."""
+  code = """
+import sys
+sys.modules['daydreamer_amd._block'] = None     # what an import of a missing module finds
+from daydreamer_amd import hipops
+lib = hipops.load_library()
+assert lib.dd_version() == hipops.ABI_VERSION and hipops.load_library() is lib
+ops = object.__new__(hipops.HipOps)
+ops._index, ops._ws_ptr, ops.ws_bytes = 0, 0, 0
+try:
+  ops.quant_rows(None, None, None)
+except RuntimeError as e:
+  assert '_block.so not found' in str(e) and 'build()' in str(e), e
+else:
+  raise SystemExit('not refused')
+"""
+  subprocess.run([sys.executable, '-c', code], check=True, timeout=120)
