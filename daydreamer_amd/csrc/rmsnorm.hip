@@ -257,7 +257,7 @@ int launch_fwd(const RmsArgs& a, hipStream_t st) {
   const dim3 grid(dd_ceil_div(a.rows, rpb));
 #define DD_RMS_FWD(N_, T_) \
   if (sh.nc == N_ && threads == T_) { k_rms_fwd<N_, NORM, T_><<<grid, T_, 0, st>>>(a, per); }
-  DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(3, 256) DD_RMS_FWD(4, 256) DD_RMS_FWD(1, 1024) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
+  DD_RMS_FWD(1, 256) DD_RMS_FWD(2, 256) DD_RMS_FWD(3, 256) DD_RMS_FWD(4, 256) DD_RMS_FWD(2, 1024) DD_RMS_FWD(4, 1024)
 #undef DD_RMS_FWD
   DD_CHECK_LAUNCH(NORM ? "dd_rms_norm_fwd" : "dd_quant_rows");
   return 0;
