@@ -874,15 +874,21 @@ int planned(const char* who, const Mat& P, const Mat& Q, int K, const Plan& plan
   if (plan.shape == 1) return tiled<ES, P_RC, Q_RC, 128, 128, 4, 2>(who, P, Q, K, plan.splits, e, slabs, st);
   return tiled<ES, P_RC, Q_RC, 256, 256, 2, 4>(who, P, Q, K, plan.splits, e, slabs, st);
 }
-// The tiled products.  Where the last round of tiles would leave most of the chip idle, whole rounds take
-// the first rows and a launch of its own, with a plan of its own, the rest (37500 x 1024 x 2048, 2.3 rounds:
-// 166 -> 161 us; its dx 150 -> 138).
-template <int ES, bool P_RC, bool Q_RC>
-int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, size_t room, hipStream_t st) {
-  const int ksteps = dd_ceil_div(K, ROWB / ES), shapes = P_RC ? 2 : 3;
-  Plan all = plan_product(P.R, Q.R, ksteps, room, shapes, e), head{}, tail{};
-  long cut = 0;
-  float best = 0.95f * all.us;
+// Which kernels a product takes, all of it host logic: the launches follow it, and dd_linear_plan tells it.
+struct Choice {
+  enum Kernel { FEW, TILES, GENERAL } kernel;
+  int few;           // FEW: sixteens of rows in the accumulators
+  long cut;          // TILES: rows of a first launch (0: one launch does all)
+  Plan head, rest;   // its plan, the other rows'
+  int splits;        // GENERAL: of the contraction
+};
+
+// Tiles.  Where the last round of tiles would leave most of the chip idle, whole rounds take the first rows and a
+// launch of its own, with a plan of its own, the rest (37500 x 1024 x 2048, 2.3 rounds: 166 -> 161 us; its dx 150 -> 138).
+inline void choose_rounds(Choice& c, const Mat& P, const Mat& Q, int ksteps, int shapes, const Epi& e, size_t room) {
+  c.cut = 0;
+  c.rest = plan_product(P.R, Q.R, ksteps, room, shapes, e);
+  float best = 0.95f * c.rest.us;
   for (int i = 0; i < shapes; ++i) {
     const TileShape& t = SHAPES[i];
     const long tm = dd_ceil_div(P.R, t.rows), tn = dd_ceil_div(Q.R, t.cols), full = tm * tn / t.slots;
@@ -890,53 +896,69 @@ int rounds(const char* who, Mat P, Mat Q, int K, const Epi& e, float* slabs, siz
     if (full == 0 || rows == 0 || rows >= P.R) continue;
     const Plan rest = plan_product(P.R - rows, Q.R, ksteps, room, shapes, e);
     const float us = full * (t.step * ksteps + t.rest + epilogue_cost(t, e)) + rest.us + 2.f;
-    if (us < best) { best = us; cut = rows; head = {i, 1, us}; tail = rest; }
+    if (us < best) { best = us; c.cut = rows; c.head = {i, 1, us}; c.rest = rest; }
   }
-  if (cut == 0) return planned<ES, P_RC, Q_RC>(who, P, Q, K, all, e, slabs, st);
-  Mat p = P;
-  p.R = (int)cut;
-  if (const int rc = planned<ES, P_RC, Q_RC>(who, p, Q, K, head, e, slabs, st)) return rc;
-  p.p = (const char*)P.p + (P_RC ? cut : cut * P.ld) * ES;
-  p.R = P.R - (int)cut;
-  Epi f = e;
-  const long es = e.ytype == DD_F32 ? 4 : 2;
-  f.y = (char*)e.y + cut * e.ldy * es;
-  if (e.res) f.res = (const char*)e.res + cut * e.ldr * es;
-  if (e.z) f.z = e.z + cut * e.ldz;
-  if (e.xs) f.xs = e.xs + cut;
-  return planned<ES, P_RC, Q_RC>(who, p, Q, K, tail, f, slabs, st);
 }
 
-template <int ES, bool P_RC, bool Q_RC>
-int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+inline Choice choose(const Mat& P, const Mat& Q, int K, int es, bool p_rc, bool q_rc, const Epi& e, size_t room) {
+  Choice c{};
   // Below 2^22 multiplications over a short contraction the general kernel's small tiles start and end sooner
   // (128 x 128 x 128 4.2 us against 5.4, 8 x 64 x 72 dw 4.4 against 5.1; 70 x 64 x 1000 8.5 either way).
-  const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * ES < 8 * ROWB;
+  const bool small = (double)P.R * Q.R * K < 4194304.0 && (long)K * es < 8 * ROWB;
+  const bool can_tile = K > 0 && tileable(P, p_rc, es) && tileable(Q, q_rc, es);
   // Few rows, as long as the weights' 16-row workgroups are a round or two of the chip: each reads all of x, and tiles
   // read it less often (8 x 16384 x 1024 7.3 us against 12.5 on tiles, 8 x 32768 x 1024 14.6 against 14.2; 64 x 8192
   // x 1024 7.6 and 11.5, 64 x 16384 x 1024 13.5 and 13.2; 128 x 4096 x 1024 7.7 and 11.5, 128 x 8192 x 1024 14.0 and 11.5;
   // long rows and 16 of x at most: the weights' read is all there is, 8 x 65536 x 4096 91 and 123).
-  if constexpr (!P_RC && !Q_RC) {
-    const unsigned grid = dd_ceil_div(Q.R, 16);
-    const unsigned most = P.R <= 16 ? ((long)K * ES >= 8192 ? 1u << 30 : 1024) : P.R <= 64 ? 512 : P.R <= 128 && !small ? 256 : 0;
-    if (grid <= most && K > 0 && tileable(P, false, ES) && tileable(Q, false, ES)) {
-      if (P.R <= 16) k_linear_few<ES, 1, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
-      else if (P.R <= 32) k_linear_few<ES, 2, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
-      else if (P.R <= 64) k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
+  const unsigned grid = dd_ceil_div(Q.R, 16);
+  const unsigned most = P.R <= 16 ? ((long)K * es >= 8192 ? 1u << 30 : 1024) : P.R <= 64 ? 512 : P.R <= 128 && !small ? 256 : 0;
+  const int ksteps = dd_ceil_div(K, ROWB / es);
+  if (!p_rc && !q_rc && grid <= most && can_tile) {
+    c.kernel = Choice::FEW;
+    c.few = P.R <= 16 ? 1 : P.R <= 32 ? 2 : P.R <= 64 ? 4 : 8;
+  } else if (!small && can_tile && (!e.res || e.ldr < (1l << 20))) {
+    c.kernel = Choice::TILES;
+    choose_rounds(c, P, Q, ksteps, p_rc ? 2 : 3, e, room);
+  } else {
+    c.kernel = Choice::GENERAL;
+    c.splits = pick_splits((long)dd_ceil_div(P.R, 64) * dd_ceil_div(Q.R, 64), ksteps, sizeof(float) * (size_t)P.R * Q.R, room);
+  }
+  return c;
+}
+
+template <int ES, bool P_RC, bool Q_RC>
+int product(const char* who, Mat P, Mat Q, int K, const Epi& e, float* ws, size_t ws_bytes, hipStream_t st) {
+  const Choice c = choose(P, Q, K, ES, P_RC, Q_RC, e, ws ? ws_bytes : 0);
+  if (c.kernel == Choice::FEW) {
+    if constexpr (!P_RC && !Q_RC) {
+      const unsigned grid = dd_ceil_div(Q.R, 16);
+      if (c.few == 1) k_linear_few<ES, 1, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
+      else if (c.few == 2) k_linear_few<ES, 2, 8><<<grid, 512, 0, st>>>(P, Q, K, e);
+      else if (c.few == 4) k_linear_few<ES, 4, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
       else k_linear_few<ES, 8, 4><<<grid, 256, 0, st>>>(P, Q, K, e);
       DD_CHECK_LAUNCH(who);
-      return 0;
     }
+    return 0;
   }
-  const size_t room = ws ? ws_bytes : 0;
-  if (!small && K > 0 && tileable(P, P_RC, ES) && tileable(Q, Q_RC, ES) && (!e.res || e.ldr < (1l << 20)))
-    return rounds<ES, P_RC, Q_RC>(who, P, Q, K, e, ws, room, st);
-  const int bk = ROWB / ES;
+  if (c.kernel == Choice::TILES) {
+    if (c.cut == 0) return planned<ES, P_RC, Q_RC>(who, P, Q, K, c.rest, e, ws, st);
+    Mat p = P;
+    p.R = (int)c.cut;
+    if (const int rc = planned<ES, P_RC, Q_RC>(who, p, Q, K, c.head, e, ws, st)) return rc;
+    p.p = (const char*)P.p + (P_RC ? c.cut : c.cut * P.ld) * ES;
+    p.R = P.R - (int)c.cut;
+    Epi f = e;
+    const long es = e.ytype == DD_F32 ? 4 : 2;
+    f.y = (char*)e.y + c.cut * e.ldy * es;
+    if (e.res) f.res = (const char*)e.res + c.cut * e.ldr * es;
+    if (e.z) f.z = e.z + c.cut * e.ldz;
+    if (e.xs) f.xs = e.xs + c.cut;
+    return planned<ES, P_RC, Q_RC>(who, p, Q, K, c.rest, f, ws, st);
+  }
+  const int bk = ROWB / ES, ktiles = dd_ceil_div(K, bk);
   const dim3 tiles(dd_ceil_div(P.R, 64), dd_ceil_div(Q.R, 64));
   DD_REQUIRE(tiles.y <= 65535, "dd_linear: more than 4194240 output columns");
-  const int ktiles = dd_ceil_div(K, bk);
-  const int S = pick_splits((long)tiles.x * tiles.y, ktiles, sizeof(float) * (size_t)P.R * Q.R, room);
-  const int kspan = max(1, dd_ceil_div(ktiles, S)) * bk, parts = max(1, dd_ceil_div(K, kspan));
+  const int kspan = max(1, dd_ceil_div(ktiles, c.splits)) * bk, parts = max(1, dd_ceil_div(K, kspan));
   k_linear_any<ES, P_RC, Q_RC><<<dim3(tiles.x, tiles.y, parts), 256, 0, st>>>(P, Q, K, kspan, parts > 1 ? ws : nullptr, e);
   DD_CHECK_LAUNCH(who);
   return parts > 1 ? sum_slabs(who, ws, parts, P.R, Q.R, e, st) : 0;
@@ -1038,6 +1060,34 @@ extern "C" int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, i
   Epi e{y, ldy, y_type, bias, act, res, ldr, (__bf16*)z, ldz, x_scale, w_scale, 0};
   if (type == DD_BF16) return product<2, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
   return product<1, false, false>("dd_linear_fwd", P, Q, K, e, ws, ws_bytes, (hipStream_t)stream);
+}
+
+// The operands of the three products as the entry points pass them on.
+extern "C" int dd_linear_plan(int what, int type, int M, int N, int K, long ldp, long ldq, int act, long ldr, int z, size_t ws_bytes,
+                              int* plan) {
+  DD_REQUIRE(in_range(M, N, K) && M > 0, "dd_linear_plan: M, N, K > 0 (2^30 at most) are needed");
+  DD_REQUIRE(type == DD_BF16 || type == DD_E4M3, "dd_linear_plan: bf16 or e4m3");
+  DD_REQUIRE(what == 0 || ((what == 1 || what == 2) && type == DD_BF16), "dd_linear_plan: 0 forward, 1 data, 2 weight (bf16)");
+  DD_REQUIRE(act >= DD_ACT_NONE && act <= DD_ACT_GELU && plan, "dd_linear_plan: unknown activation, or no plan");
+  Epi e{};
+  if (what == 0) {
+    e.act = act;
+    e.res = ldr ? plan : nullptr;   // (looked at, not read)
+    e.ldr = ldr;
+    e.z = z ? (__bf16*)plan : nullptr;
+  }
+  const Mat P{nullptr, ldp, what == 2 ? N : M}, Q{nullptr, ldq, what == 0 ? N : K};
+  const Choice c = choose(P, Q, what == 0 ? K : what == 1 ? N : M, type == DD_BF16 ? 2 : 1, what == 2, what != 0, e, ws_bytes);
+  for (int i = 0; i < 8; ++i) plan[i] = 0;
+  plan[0] = c.kernel;
+  if (c.kernel == Choice::FEW) plan[1] = 16 * c.few;
+  if (c.kernel == Choice::GENERAL) plan[1] = c.splits;
+  if (c.kernel == Choice::TILES) {
+    const TileShape &h = SHAPES[c.head.shape], &r = SHAPES[c.rest.shape];
+    plan[1] = r.rows; plan[2] = r.cols; plan[3] = c.rest.splits;
+    if (c.cut) { plan[4] = (int)c.cut; plan[5] = h.rows; plan[6] = h.cols; plan[7] = c.head.splits; }
+  }
+  return 0;
 }
 
 extern "C" int dd_linear_bwd_data(const void* dz, long lddz, const void* w, long ldw, void* dx, long lddx, int x_type, int M,

@@ -113,6 +113,7 @@ _SIGS = {
     'dd_rms_norm_bwd': [c_p, c_l, c_i, c_p, c_l, c_i, c_p, c_p, c_p, c_l, c_p, c_l, c_p, c_i, c_i, c_i, c_p, c_z, c_p],
     'dd_quant_rows': [c_p, c_l, c_i, c_p, c_l, c_p, c_i, c_i, c_p],
     'dd_linear_fwd': [c_p, c_l, c_p, c_l, c_i, c_p, c_p, c_p, c_i, c_p, c_l, c_p, c_l, c_i, c_p, c_l, c_i, c_i, c_i, c_p, c_z, c_p],
+    'dd_linear_plan': [c_i, c_i, c_i, c_i, c_i, c_l, c_l, c_i, c_l, c_i, c_z, ctypes.POINTER(c_i)],
     'dd_linear_act_bwd': [c_p, c_l, c_p, c_l, c_i, c_p, c_l, c_p, c_i, c_i, c_i, c_i, c_p, c_z, c_p],
     'dd_linear_bwd_data': [c_p, c_l, c_p, c_l, c_p, c_l, c_i, c_i, c_i, c_i, c_p, c_z, c_p],
     'dd_linear_bwd_weight': [c_p, c_l, c_p, c_l, c_p, c_l, c_i, c_i, c_i, c_i, c_i, c_p, c_z, c_p],
@@ -128,7 +129,7 @@ _SIGS = {
 }
 
 EXPORTS = sorted(list(_SIGS) + ['dd_version', 'dd_last_error'])
-ABI_VERSION = 12   # include/daydreamer_hip.h DD_ABI_VERSION
+ABI_VERSION = 13   # include/daydreamer_hip.h DD_ABI_VERSION
 
 
 class _Missing:

@@ -37,8 +37,9 @@ extern "C" {
  * 11 (round 6): dd_gemm_f32_x, dd_imag_set_rows, dd_conv2d_s2_wgrad_ln,
  * dd_conv2d_s2_down_ln, dd_conv2d_s2_down_lnbwd, dd_stamp added.
  * 12: the residual recurrent block added: dd_rms_norm_fwd / _bwd, dd_quant_rows, dd_linear_fwd,
- * dd_linear_act_bwd / _bwd_data / _bwd_weight, dd_gated_scan_fwd / _bwd. */
-#define DD_ABI_VERSION 12
+ * dd_linear_act_bwd / _bwd_data / _bwd_weight, dd_gated_scan_fwd / _bwd.
+ * 13: dd_linear_plan added. */
+#define DD_ABI_VERSION 13
 int dd_version(void);
 const char* dd_last_error(void);
 
@@ -287,6 +288,13 @@ int dd_quant_rows(const void* x, long ldx, int x_type, void* q, long ldq, float*
 int dd_linear_fwd(const void* x, long ldx, const void* w, long ldw, int type, const float* x_scale,
                   const float* w_scale, const float* bias, int act, const void* res, long ldr, void* y, long ldy,
                   int y_type, void* z, long ldz, int M, int N, int K, float* ws, size_t ws_bytes, void* stream);
+/* Which kernels a product takes (host logic, no launch), so that a test can hold a size to the kernel that it is for.  what:
+ * 0 dd_linear_fwd (ldp, ldq: of x, w; act; ldr of the residual, 0 without one; z: is it kept), 1 dd_linear_bwd_data (of
+ * dz, w), 2 dd_linear_bwd_weight (of dz, x).  plan[8]: 0, rows of its accumulators (few rows) | 1, rows and columns of a
+ * tile, splits, and, where a first launch takes some of the rows, those, its tile and splits (tiles) | 2, splits
+ * (the general kernel). */
+int dd_linear_plan(int what, int type, int M, int N, int K, long ldp, long ldq, int act, long ldr, int z, size_t ws_bytes,
+                   int* plan);
 /* Gradients of the bf16 product (the gradient of res is dy).  dd_linear_act_bwd: dz = dy act'(z) (bf16;
  * dz may be dy or z itself; with DD_ACT_NONE z and dz are unused, dz IS dy) and dbias [N] (NULL ok);
  * dd_linear_bwd_data: dx [M,K] = dz w; dd_linear_bwd_weight: dw [N,K] = or += (accumulate) dz^T x.

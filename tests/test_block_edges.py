@@ -60,3 +60,21 @@ else:
   raise SystemExit('not refused')
 """
   subprocess.run([sys.executable, '-c', code], check=True, timeout=120)
+
+
+def test_plans_of_products():
+  """dd_linear_plan is host logic: few rows, tiles in one or two launches, the general kernel, and what it refuses."""
+  import ctypes
+  lib, plan = hipops.load_library(), (ctypes.c_int * 8)()
+
+  def ask(what, M, N, K, type=1, act=0, ldr=0, z=0, ldp=None, ws=2048 << 20):
+    k, q = K if what == 0 else N, K
+    rc = lib.dd_linear_plan(what, type, M, N, K, ldp or k, q, act, ldr, z, ws, plan)
+    return list(plan) if rc == 0 else lib.dd_last_error().decode()
+  assert ask(0, 8, 2048, 1024)[:2] == [0, 16] and ask(0, 100, 2048, 1024)[:2] == [0, 128]
+  assert ask(0, 100, 100, 100)[0] == 2 and ask(0, 100, 100, 100, ldp=1 << 24)[0] == 2
+  assert ask(0, 8192, 8192, 8192) == [1, 256, 256, 1, 0, 0, 0, 0]
+  assert ask(0, 37500, 1024, 2048, ldr=1024) == [1, 192, 128, 1, 32768, 256, 256, 1]     # whole rounds, and the rest
+  assert ask(2, 37500, 1024, 2048)[3] > 1 and ask(2, 37500, 1024, 2048, ws=0)[3] == 1   # no room, no split
+  assert 'dd_linear_plan' in ask(1, 8, 8, 8, type=2) and 'dd_linear_plan' in ask(0, 0, 8, 8)
+  assert 'dd_linear_plan' in ask(3, 8, 8, 8) and 'dd_linear_plan' in ask(0, 8, 8, 8, type=0) and 'dd_linear_plan' in ask(0, 8, 8, 8, act=9)

@@ -189,3 +189,190 @@ def test_shared_memory_is_refused(hip):
   hip.linear_fwd(buf[:16, :16], w, buf[:16, 16:32], res=buf[:16, 32:48], z=buf[16:32, :16])
   hip.linear_fwd(buf[0:32:2, :16], w, buf[1:32:2, :16])
   hip.gated_scan_fwd(buf[:16, :16], buf[:16, 16:32], buf[:16, 32:48], 4)
+
+
+# ---- product: every kernel and plan ---------------------------------------------------------------
+
+
+class View:
+  """A [rows, cols] view inside a larger buffer of `around` on the GPU; `whole` says that nothing around it changed."""
+
+  def __init__(self, rows, cols, dtype, left=1, right=8, value=None, around=7.0):
+    self.base = torch.full((rows + 1, left + cols + right), around, device='cuda').to(dtype)
+    self.t = self.base[:rows, left:left + cols]
+    if value is not None:
+      self.t.copy_(value)
+
+  def whole(self, what):
+    b, t = self.base, self.t
+    left = t.storage_offset() % b.shape[1]
+    for part in (b[:, :left], b[:, left + t.shape[1]:], b[t.shape[0]:]):
+      assert bool((part.float() == 7.0).all()), f'{what}: written outside the view'
+
+
+def near(out, want, tol, what):
+  """|out - want| <= tol + half a step of out's type, elementwise, on the GPU."""
+  lim = tol + HALF[out.dtype] * (want.abs() + tol) + 1e-37
+  over = ~((out.double() - want).abs() <= lim)
+  if bool(over.any()):
+    i = over.nonzero()[0]
+    raise AssertionError(f'{what}: {int(over.sum())} of {over.numel()} off, first at {i.tolist()}: {float(out[tuple(i)])} '
+                         f'for {float(want[tuple(i)])}, allowed {float(lim[tuple(i)])}')
+
+
+def on_gpu(*shape, seed=0, scale=1.0, dtype=F32):
+  g = torch.Generator(device='cuda').manual_seed(seed)
+  return (torch.randn(*shape, generator=g, device='cuda') * scale).to(dtype)
+
+
+def plan_of(hip, what, M, N, K, type=1, act=0, ldr=0, z=0, ldp=None, ldq=None):
+  import ctypes
+  out = (ctypes.c_int * 8)()
+  k, q = ((K, K), (N, K), (N, K))[what]
+  assert hip.lib.dd_linear_plan(what, type, M, N, K, ldp or k, ldq or q, act, ldr, z, hip.ws_bytes, out) == 0
+  return list(out)
+
+
+ACTS = {None: 0, 'elu': 1, 'silu': 2, 'gelu': 3}
+
+
+def slope_and_value(z, act):
+  t = z.clone().requires_grad_(True)
+  y = {None: lambda: t * 1.0, 'elu': lambda: torch.where(t > 0, t, torch.expm1(t)), 'silu': lambda: t * torch.sigmoid(t),
+       'gelu': lambda: t * torch.special.erfc(-t / 2 ** 0.5) / 2}[act]()
+  return y.detach(), torch.autograd.grad(y.sum(), t)[0]
+
+
+# plan: splits above one are written as 2
+TILED = [
+    (25877, 385, 1041, 'gelu', [1, 256, 256, 1, 0, 0, 0]), (20480, 640, 1040, 'silu', [1, 256, 256, 1, 0, 0, 0]),
+    (19845, 515, 1433, None, [1, 256, 256, 1, 0, 0, 0]),
+    (16693, 135, 769, 'elu', [1, 192, 128, 1, 0, 0, 0]), (5403, 129, 3915, 'silu', [1, 192, 128, 2, 0, 0, 0]),
+    (38727, 397, 1753, 'gelu', [1, 128, 128, 1, 32768, 256, 256]), (27413, 659, 1401, 'silu', [1, 192, 128, 1, 21760, 256, 256]),
+    (33129, 403, 1881, 'elu', [1, 128, 128, 2, 32768, 256, 256]), (33313, 131, 1691, 'gelu', [1, 128, 128, 2, 32768, 128, 128]),
+    (33519, 269, 1865, 'gelu', [1, 192, 128, 1, 21760, 128, 128]), (35073, 133, 4289, 'silu', [1, 128, 128, 2, 24576, 192, 128]),
+]
+
+
+def few_splits(plan):
+  return plan[:3] + [min(plan[3], 2)] + plan[4:7]
+
+
+@pytest.mark.parametrize('yt', [BF16, F32])
+@pytest.mark.parametrize('M,N,K,act,plan', TILED)
+def test_tiles_and_launches(hip, M, N, K, act, plan, yt):
+  """Ragged products that take each tile shape, split and pair of launches, with all of the epilogue, and the residual
+  in place."""
+  assert few_splits(plan_of(hip, 0, M, N, K, act=ACTS[act], ldr=N, z=1)) == plan
+  x, w = View(M, K, BF16, value=on_gpu(M, K, seed=1)), View(N, K, BF16, value=on_gpu(N, K, seed=2, scale=K ** -0.5))
+  b, r = on_gpu(N, seed=3), View(M, N, yt, value=on_gpu(M, N, seed=4))
+  y, z = View(M, N, yt), View(M, N, BF16)
+  hip.linear_fwd(x.t, w.t, y.t, bias=b, act=act, res=r.t, z=z.t)
+  xd, wd = x.t.double(), w.t.double()
+  want = xd @ wd.t() + b.double()
+  # the instruction adds 16 products to its accumulator at a time: K / 16 + 32 additions, 4 within an instruction
+  err = (K / 4 + 48) * U * (xd.abs() @ wd.abs().t()) + 4 * U * want.abs()
+  near(z.t, want, err, 'z')
+  rd = r.t.double()
+  near(y.t, slope_and_value(want, act)[0] + rd, 1.13 * err + 16 * U * (want.abs() + rd.abs()), 'y')
+  y.whole('y'), z.whole('z')
+  hip.linear_fwd(x.t, w.t, r.t, bias=b, act=act, res=r.t)
+  if few_splits(plan_of(hip, 0, M, N, K, act=ACTS[act], ldr=N)) == plan:
+    assert torch.equal(r.t, y.t), 'the residual in place'
+  else:
+    near(r.t, slope_and_value(want, act)[0] + rd, 1.13 * err + 16 * U * (want.abs() + rd.abs()), 'the residual in place')
+  r.whole('res')
+
+
+@pytest.mark.parametrize('M,N,K,act,res,plan', [
+    (25445, 385, 855, 'gelu', False, [1, 256, 256, 1, 0, 0, 0]), (25445, 385, 855, None, True, [1, 256, 256, 1, 0, 0, 0]),
+    (25445, 385, 2047, 'elu', True, [1, 256, 256, 1, 0, 0, 0]),
+    (39339, 389, 1975, 'silu', False, [1, 128, 128, 1, 32768, 256, 256]), (39339, 389, 1975, None, True, [1, 128, 128, 1, 32768, 256, 256]),
+    (16693, 135, 1099, 'elu', False, [1, 192, 128, 1, 0, 0, 0]), (16693, 135, 1099, None, True, [1, 192, 128, 1, 0, 0, 0]),
+    (28039, 655, 1621, 'gelu', False, [1, 192, 128, 1, 21760, 256, 256]), (28039, 655, 1621, None, True, [1, 192, 128, 1, 21760, 256, 256]),
+    (5549, 131, 4873, None, False, [1, 192, 128, 2, 0, 0, 0]), (32803, 429, 2355, None, True, [1, 128, 128, 2, 32768, 256, 256])])
+def test_tiles_and_launches_e4m3(hip, M, N, K, act, res, plan):
+  assert few_splits(plan_of(hip, 0, M, N, K, type=2, act=ACTS[act], ldr=N if res else 0)) == plan
+  x = View(M, K, FP8, value=on_gpu(M, K, seed=1, scale=60.0).clamp(-448, 448).to(FP8))
+  w = View(N, K, FP8, value=on_gpu(N, K, seed=2, scale=60.0).clamp(-448, 448).to(FP8))
+  sx, sw, b = on_gpu(M, seed=3).abs() * 0.01 + 1e-3, on_gpu(N, seed=4).abs() * 1e-3 + 1e-4, on_gpu(N, seed=5)
+  r, y = View(M, N, BF16, value=on_gpu(M, N, seed=6)) if res else None, View(M, N, BF16)
+  hip.linear_fwd(x.t, w.t, y.t, bias=b, act=act, res=r.t if res else None, x_scale=sx, w_scale=sw)
+  xd, wd = x.t.float().double(), w.t.float().double()
+  s = sx.double()[:, None] * sw.double()
+  want = (xd @ wd.t()) * s + b.double()
+  eights = lambda t: torch.nn.functional.pad(t, (0, -K % 8)).reshape(t.shape[0], -1, 8).abs().amax(2)  # noqa: E731
+  # sums as in bf16, and of eight consecutive products what is below 2^-13 of the largest: less than 7 2^-13 of it
+  err = ((K / 4 + 48) * U * (xd.abs() @ wd.abs().t()) + 7 * 2.0 ** -13 * (eights(xd) @ eights(wd).t())) * s + 8 * U * want.abs()
+  rd = r.t.double() if res else torch.zeros_like(want)
+  near(y.t, slope_and_value(want, act)[0] + rd, 1.13 * err + 16 * U * (want.abs() + rd.abs()), 'y')
+  y.whole('y')
+
+
+@pytest.mark.parametrize('M,N,K,what,plan', [
+    (2701, 103, 4433, 1, [1, 256, 256, 1, 0, 0, 0]), (605, 8711, 4383, 1, [1, 256, 256, 2, 0, 0, 0]),
+    (4135, 529, 4397, 1, [1, 128, 128, 1, 3584, 256, 256]), (5641, 461, 3597, 1, [1, 192, 128, 1, 4352, 256, 256]),
+    (2307, 2537, 3569, 1, [1, 128, 128, 2, 2304, 128, 128]),
+    (269, 1723, 4777, 2, [1, 256, 256, 1, 0, 0, 0]), (22203, 131, 2295, 2, [1, 256, 256, 2, 0, 0, 0]),
+    (521, 3861, 4231, 2, [1, 128, 128, 1, 3840, 256, 256]), (2167, 2691, 2953, 2, [1, 128, 128, 2, 2688, 128, 128])])
+def test_tiles_and_launches_of_gradients(hip, M, N, K, what, plan):
+  assert few_splits(plan_of(hip, what, M, N, K)) == plan
+  x, w = View(M, K, BF16, value=on_gpu(M, K, seed=1)), View(N, K, BF16, value=on_gpu(N, K, seed=2, scale=K ** -0.5))
+  dy = View(M, N, BF16, value=on_gpu(M, N, seed=3))
+  d = dy.t.double()
+  if what == 1:
+    dx, wd = View(M, K, BF16), w.t.double()
+    hip.linear_bwd(dy.t, x.t, w.t, dx=dx.t)
+    near(dx.t, d @ wd, (N / 4 + 48) * U * (d.abs() @ wd.abs()), 'dx')
+    dx.whole('dx')
+    return
+  xd = x.t.double()
+  want, err = d.t() @ xd, (M / 4 + 48) * U * (d.abs().t() @ xd.abs())
+  old = on_gpu(N, K, seed=4)
+  for acc in (False, True):
+    dw = View(N, K, F32, value=old)
+    hip.linear_bwd(dy.t, x.t, w.t, dw=dw.t, accumulate=acc)
+    near(dw.t, want + old.double() if acc else want, err + 2 * U * (want.abs() + old.double().abs()), 'dw')
+    dw.whole('dw')
+
+
+def test_long_rows_of_many_outputs(hip):
+  """Sixteen rows at most with long contractions stay with the few-row kernel however many outputs there are."""
+  M, N, K = 8, 17001, 4100
+  assert plan_of(hip, 0, M, N, K)[:2] == [0, 16]
+  x, w = on_gpu(M, K, seed=1, dtype=BF16), on_gpu(N, K, seed=2, scale=K ** -0.5, dtype=BF16)
+  y = View(M, N, BF16)
+  hip.linear_fwd(x, w, y.t)
+  want = x.double() @ w.double().t()
+  near(y.t, want, (K / 4 + 48) * U * (x.double().abs() @ w.double().abs().t()), 'y')
+  y.whole('y')
+
+
+@pytest.mark.parametrize('accumulate', [False, True])
+def test_general_kernel_split(hip, accumulate):
+  """Rows megabytes apart, whose contraction is split over the general kernel's workgroups, in all three products."""
+  M, N, K, ld = 5, 1003, 1000, (1 << 21) + 2
+  assert plan_of(hip, 0, M, 40, K, ldp=ld)[:2] == [2, 4] and plan_of(hip, 1, M, N, 40, ldp=ld)[:2] == [2, 4]
+  far = torch.empty(M, ld, device='cuda', dtype=BF16)
+  x, w, dz = far[:, 3:3 + K], on_gpu(N, K, seed=2, dtype=BF16), far[:, 5001:5001 + N]
+  x.copy_(on_gpu(M, K, seed=1)), dz.copy_(on_gpu(M, N, seed=3))
+  y, b = View(M, 40, F32), on_gpu(40, seed=4)
+  hip.linear_fwd(x, w[:40], y.t, bias=b)
+  xd, wd = x.double(), w.double()
+  near(y.t, xd @ wd[:40].t() + b.double(), (K / 4 + 50) * U * (xd.abs() @ wd[:40].abs().t() + b.double().abs()), 'y')
+  dx = View(M, 40, F32)
+  hip.linear_bwd(dz, x[:, :40], w[:, :40], dx=dx.t)
+  near(dx.t, dz.double() @ wd[:, :40], (N / 4 + 48) * U * (dz.double().abs() @ wd[:, :40].abs()), 'dx')
+  y.whole('y'), dx.whole('dx')
+  M, N, K, ld = 530, 24, 70, (1 << 23) + 2
+  assert plan_of(hip, 2, M, N, K, ldp=ld)[:2] == [2, 2]
+  far = torch.empty(M, ld, device='cuda', dtype=BF16)
+  dz, x = far[:, 7:7 + N], on_gpu(M, K, seed=5, dtype=BF16)
+  dz.copy_(on_gpu(M, N, seed=6))
+  old = on_gpu(N, K, seed=7)
+  dw = View(N, K, F32, value=old)
+  hip.linear_bwd(dz, x, on_gpu(N, K, seed=8, dtype=BF16), dw=dw.t, accumulate=accumulate)
+  d, xd = dz.double(), x.double()
+  want = d.t() @ xd + (old.double() if accumulate else 0.0)
+  near(dw.t, want, (M / 4 + 48) * U * (d.abs().t() @ xd.abs()) + 2 * U * want.abs(), 'dw')
+  dw.whole('dw')
