@@ -376,3 +376,63 @@ def test_general_kernel_split(hip, accumulate):
   want = d.t() @ xd + (old.double() if accumulate else 0.0)
   near(dw.t, want, (M / 4 + 48) * U * (d.abs().t() @ xd.abs()) + 2 * U * want.abs(), 'dw')
   dw.whole('dw')
+
+
+# ---- in place -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('yt', [BF16, F32])
+@pytest.mark.parametrize('M,N,K', [(8, 2048, 1024), (13, 47, 200), (40, 521, 520), (100, 1001, 520), (70, 95, 256), (300, 257, 1030),
+                                   (1300, 301, 1031), (700, 1021, 333), (257, 129, 8200), (1000, 200, 2048)])
+def test_residual_in_place(hip, M, N, K, yt):
+  """y over res, bit for bit what another output gets: few rows, small tiles, tiles, a split contraction; rows whose last
+  columns overlap their neighbour's."""
+  x, w = on_gpu(M, K, seed=1, dtype=BF16), on_gpu(N, K, seed=2, scale=K ** -0.5, dtype=BF16)
+  r, y, b = View(M, N, yt, value=on_gpu(M, N, seed=3)), View(M, N, yt), on_gpu(N, seed=4)
+  for act in (None, 'gelu'):
+    hip.linear_fwd(x, w, y.t, bias=b, act=act, res=r.t)
+    stream = View(M, N, yt, value=r.t)
+    hip.linear_fwd(x, w, stream.t, bias=b, act=act, res=stream.t)
+    assert torch.equal(stream.t, y.t)
+    stream.whole('stream')
+
+
+@pytest.mark.parametrize('act', ['elu', 'silu', 'gelu'])
+@pytest.mark.parametrize('N', [1, 7, 9, 65, 515, 1021])
+@pytest.mark.parametrize('M', [3, 256, 300, 5001])
+def test_activation_gradient_in_place(hip, M, N, act):
+  """dz over dy and over z, with the same dbias, dx and dw as from a tensor of its own."""
+  K = 24
+  x, w = on_gpu(M, K, seed=1, dtype=BF16), on_gpu(N, K, seed=2, dtype=BF16)
+  dy, z = (View(M, N, BF16, value=on_gpu(M, N, seed=k)) for k in (3, 4))
+  got = []
+  for which in ('apart', 'dy', 'z'):
+    d, t = View(M, N, BF16, value=dy.t), View(M, N, BF16, value=z.t)
+    dz = {'apart': View(M, N, BF16), 'dy': d, 'z': t}[which]
+    db, dx, dw = torch.zeros(N, device='cuda'), torch.zeros(M, K, device='cuda'), torch.zeros(N, K, device='cuda')
+    hip.linear_bwd(d.t, x, w, dx=dx, dw=dw, dbias=db, act=act, z=t.t, dz=dz.t)
+    for v in (d, t, dz):
+      v.whole(which)
+    got.append((dz.t, db, dx, dw))
+  for other in got[1:]:
+    assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+  zd = z.t.double()
+  near(got[0][0], dy.t.double() * slope_and_value(zd, act)[1], 32 * U * dy.t.double().abs() * (1 + zd.abs()), 'dz')
+
+
+@pytest.mark.parametrize('C', [1, 7, 9, 33, 100, 1024, 1542, 2051, 4099, 8195, 16389])
+@pytest.mark.parametrize('t', [F32, BF16])
+def test_sum_over_x(hip, C, t):
+  """s over x, with and without a residual."""
+  rows = 37
+  x, res, g = on_gpu(rows, C, seed=1, dtype=t), on_gpu(rows, C, seed=2, dtype=t), 1 + on_gpu(C, seed=3, scale=0.1)
+  for r in (None, res):
+    out = []
+    for over in (False, True):
+      v = View(rows, C, t, value=x)
+      s, y, rstd = View(rows, C, t), View(rows, C, BF16), torch.zeros(rows, device='cuda')
+      hip.rms_norm_fwd(v.t, g, y.t, rstd=rstd, res=r, s=v.t if over else s.t)
+      out.append(((v if over else s).t, y.t, rstd))
+      v.whole('x'), s.whole('s'), y.whole('y')
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    assert torch.equal(out[0][0], x if r is None else (x.float() + r.float()).to(t))
