@@ -436,3 +436,31 @@ def test_sum_over_x(hip, C, t):
       v.whole('x'), s.whole('s'), y.whole('y')
     assert all(torch.equal(a, b) for a, b in zip(*out))
     assert torch.equal(out[0][0], x if r is None else (x.float() + r.float()).to(t))
+
+
+# ---- norm: more rows than workgroups --------------------------------------------------------------
+
+
+@pytest.mark.parametrize('over', [False, True])
+@pytest.mark.parametrize('rows,C,slots', [(120001, 64, 1536 * 32), (50001, 17, 1536 * 32), (13001, 300, 1536 * 4), (7001, 1000, 768 * 4),
+                                          (4001, 1542, 1536), (2001, 2500, 768), (700, 8101, 256), (701, 9001, 256), (600, 20001, 256)])
+def test_norm_gradients_of_many_rows(hip, rows, C, slots, over):
+  """More rows than are in flight at once, no multiple of them: a workgroup goes round its loop two or three times."""
+  assert rows > slots and rows % slots
+  for t in (F32, BF16):
+    s, dy, dres, g = on_gpu(rows, C, seed=1, dtype=t), on_gpu(rows, C, seed=2, dtype=BF16), on_gpu(rows, C, seed=3, dtype=t), 1 + on_gpu(C, seed=4, scale=0.1)
+    rstd = 1 / s.float().square().mean(1).sqrt()
+    dr = View(rows, C, t, value=dres)
+    ds, dgamma = dr if over else View(rows, C, t), torch.zeros(C, device='cuda')
+    hip.rms_norm_bwd(dy, s, rstd, g, ds.t, dgamma, dr.t)
+    inv = rstd.double()[:, None]
+    n, d = s.double() * inv, dy.double()
+    dn = d * g.double()
+    size = dres.double().abs() + inv * (dn.abs() + n.abs() * (dn * n).abs().mean(1, keepdim=True))
+    # the row's mean: 32 elements of a lane, 6 steps over a wave, 16 waves
+    near(ds.t, dres.double() + inv * (dn - n * (dn * n).mean(1, keepdim=True)), 64 * U * size, 'ds')
+    # dgamma: the rows of a lane, up to 32 rows of a workgroup, the workgroups in 32 runs and then those; n and a product
+    per = slots // (1536 if C <= 512 or 1024 < C <= 2048 else 768 if C <= 4096 else 256)
+    chain = rows / slots + 1 + per + slots / per / 32 + 32 + 4
+    near(dgamma, (d * n).sum(0), chain * U * (d * n).abs().sum(0), 'dgamma')
+    ds.whole('ds')
