@@ -464,3 +464,39 @@ def test_norm_gradients_of_many_rows(hip, rows, C, slots, over):
     chain = rows / slots + 1 + per + slots / per / 32 + 32 + 4
     near(dgamma, (d * n).sum(0), chain * U * (d * n).abs().sum(0), 'dgamma')
     ds.whole('ds')
+
+
+# ---- what surrounds a view ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('M,N,K', [(300, 260, 1030), (300, 257, 1031), (1300, 301, 577), (257, 129, 8201), (2500, 515, 1542), (40, 33, 1030),
+                                   (70, 61, 77), (19845, 515, 433)])
+def test_what_surrounds_a_view_is_not_read_as_data(hip, M, N, K):
+  """Rows and columns around every operand hold NaN: the results are those of compact operands, bit for bit."""
+  x, w, r = on_gpu(M, K, seed=1, dtype=BF16), on_gpu(N, K, seed=2, scale=K ** -0.5, dtype=BF16), on_gpu(M, N, seed=3, dtype=BF16)
+  dy, z, b = on_gpu(M, N, seed=4, dtype=BF16), on_gpu(M, N, seed=5, dtype=BF16), on_gpu(N, seed=6)
+  nan = float('nan')
+  results = []
+  for left in (None, 3, 8):
+    put = lambda t: t if left is None else View(*t.shape, t.dtype, left, 5, value=t, around=nan).t  # noqa: E731
+    bias = b if left is None else torch.cat([b.new_full((1,), nan), b, b.new_full((1,), nan)])[1:-1]
+    y, y32, kept = torch.zeros(M, N, device='cuda', dtype=BF16), torch.zeros(M, N, device='cuda'), torch.zeros(M, N, device='cuda', dtype=BF16)
+    hip.linear_fwd(put(x), put(w), y, bias=bias, act='gelu', res=put(r), z=kept)
+    hip.linear_fwd(put(x), put(w), y32, res=put(r.float()))
+    dx, dw, db, dz = (torch.zeros(*s, device='cuda', dtype=t) for s, t in [((M, K), BF16), ((N, K), F32), ((N,), F32), ((M, N), BF16)])
+    hip.linear_bwd(put(dy), put(x), put(w), dx=dx, dw=dw, dbias=db, act='silu', z=put(z), dz=dz if left is None else put(dz))
+    results.append((y, y32, kept, dx, dw, db))
+  for k, t in enumerate(results[0]):
+    assert bool(torch.isfinite(t).all())
+    for other in results[1:]:
+      assert torch.equal(t, other[k]), k
+
+
+@pytest.mark.parametrize('M,N,K', [(300, 260, 1030), (1300, 301, 577), (25445, 385, 855), (40, 33, 1030), (70, 61, 77)])
+def test_what_surrounds_rows_in_8_bits(hip, M, N, K):
+  x, w = (on_gpu(*s, seed=k, scale=60.0).clamp(-448, 448).to(FP8) for k, s in ((1, (M, K)), (2, (N, K))))
+  sx, sw = on_gpu(M, seed=3).abs() * 0.01, on_gpu(N, seed=4).abs() * 1e-3
+  y, y2 = (torch.zeros(M, N, device='cuda', dtype=BF16) for _ in range(2))
+  hip.linear_fwd(x, w, y, x_scale=sx, w_scale=sw)
+  hip.linear_fwd(View(M, K, FP8, 3, 5, value=x, around=float('nan')).t, View(N, K, FP8, 3, 5, value=w, around=float('nan')).t, y2, x_scale=sx, w_scale=sw)
+  assert bool(torch.isfinite(y).all()) and torch.equal(y, y2)
