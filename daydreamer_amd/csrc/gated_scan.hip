@@ -20,7 +20,10 @@
 //
 // A restart is A == 0 EXACTLY and cuts whatever came before, non-finite values too (0 * NaN would
 // not); every other factor is kept at or above FLT_MIN, so that a product that underflows does not look
-// like a restart and a NaN in the state is not lost.  State, pairs and all arithmetic are fp32.
+// like a restart and a NaN in the state is not lost.  The running state, pairs and all arithmetic are fp32; h is stored in
+// the operands' type, half the bytes in bf16, and the backward pass reads the states before each step as stored: with bf16
+// operands that leaves du off by 7e-4 in the 2-norm, by 1.6e-3 (h alone is its factor) with an input gate, beside 1.7e-3
+// for its own rounding; fp32 operands have neither.
 #include "block_core.h"
 #include <float.h>
 

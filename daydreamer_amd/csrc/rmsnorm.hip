@@ -8,12 +8,13 @@
 // derivative of what the forward pass computed; all arithmetic is fp32.
 //
 // Bound: HBM.  A row's elements stay in registers from their load to the last store - each input is
-// read once, each output written once - so a row belongs to a wave or a part of one (C <= 1024), four (<= 4096) or
-// sixteen (<= 32768), 8 or 16 elements per lane (32 past 16384) in vectors of eight: with 32 in a lane of
-// fewer waves too few fit a CU (backward, 20001 x 1542: 101 us).  The last vector of a ragged row
-// ends at the row's end and so overlaps the one before it: both lanes hold and store the same values there,
-// the sums over a row count them once.  (Element by element, its loads came one round trip after the other:
-// 20001 x 1542 bf16, backward, 141 us; now 63, at the 52 of its bytes.)
+// read once, each output written once - so a row belongs to a wave or a part of one, to four or to sixteen, in vectors
+// of eight elements, up to four of them per lane.  Forward a wave takes rows up to 2048, four up to 8192.  The
+// backward pass holds four rows' worth: a wave up to 1024, four up to 4096, with two vectors a lane (with four of them in
+// fewer waves too few fit a CU: 20001 x 1542 101 us).  Sixteen waves take rows up to 32768, four vectors a lane past 16384.
+// The last vector of a ragged row ends at the row's end and so overlaps the one before it: both lanes hold and store the
+// same values there, the sums over a row count them once.  (Element by element, its loads came one round trip after
+// the other: 20001 x 1542 bf16, backward, 141 us; now 60, at the 52 of its bytes.)
 #include "block_core.h"
 
 namespace {

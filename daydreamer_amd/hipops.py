@@ -644,7 +644,7 @@ class HipOps:
   def linear_bwd(self, dy, x, w, dx=None, dw=None, dbias=None, act=None, z=None, dz=None, accumulate=False):
     """Gradients of linear_fwd's bf16 form (the gradient of res is dy): dx bf16 or fp32, dw and dbias fp32
     or bf16 (written, or added to with `accumulate`).  With an activation z is what linear_fwd kept and
-    dz (bf16) receives dy * act'(z); dz may be dy or z."""
+    dz (bf16, the operand of both products) receives dy * act'(z); dz may be dy or z."""
     self._launch('linear_bwd', dy, x, w, dx, dw, dbias, act, z, dz, accumulate, self._ws_ptr, self.ws_bytes)
 
   def gated_scan_fwd(self, u, c, h, T, i=None, first=None, h0=None, hT=None, shift=-1.0, cand='tanh'):
@@ -660,8 +660,9 @@ class HipOps:
 
   def gated_scan_bwd(self, dh, u, c, h, du, dc, T, i=None, di=None, first=None, h0=None, dhT=None, dh0=None,
                      shift=-1.0, cand='tanh'):
-    """Gradients of gated_scan_fwd from dh [B * T, D] and dhT [B, D], with the h it wrote: du, dc, di in the
-    operands' type, dh0 [B, D] fp32 (may be dhT)."""
+    """Gradients of gated_scan_fwd from dh [B * T, D] and dhT [B, D], with the h it wrote (the states before
+    each step as they are stored: rounded, where the operands are bf16): du, dc, di in the operands' type,
+    dh0 [B, D] fp32 (may be dhT)."""
     self._launch('gated_scan_bwd', dh, u, c, h, du, dc, T, i, di, first, h0, dhT, dh0, shift, cand, self._ws_ptr,
                  self.ws_bytes)
 

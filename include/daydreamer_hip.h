@@ -319,7 +319,8 @@ int dd_linear_bwd_weight(const void* dz, long lddz, const void* x, long ldx, voi
 int dd_gated_scan_fwd(const void* u, long ldu, const void* c, long ldc, const void* i, long ldi, int type,
                       const float* first, long fstride, const float* h0, void* h, long ldh, float* hT,
                       int B, int T, int D, float shift, int cand_tanh, float* ws, size_t ws_bytes, void* stream);
-/* Gradients from dh (of every h) and dhT (of the state after the last step, NULL ok), with the stored h:
+/* Gradients from dh (of every h) and dhT (of the state after the last step, NULL ok), with the h that was stored (in the
+ * operands' type: bf16 operands keep bf16 states for du; fp32 operands keep them whole):
  * du, dc, di (with i) in the operands' type, dh0 [B,D] (NULL ok; may be dhT). */
 int dd_gated_scan_bwd(const void* dh, long lddh, const void* u, long ldu, const void* c, long ldc, const void* i,
                       long ldi, const void* h, long ldh, int type, const float* first, long fstride,
