@@ -71,9 +71,11 @@ __device__ __forceinline__ void compose(float& A1, float& B1, float A2, float B2
 
 // z = sigmoid(u + shift) and the decay q = 1 - z from E = e^-v, neither by a difference: a gate that is all but open
 // keeps its decay, and du, to a few ulp of themselves.  E is held between 2^-125 and 2^125: E z is no infinity times
-// zero, q is above FLT_MIN, and a NaN stays one (minimum and maximum keep it).
+// zero, q is above FLT_MIN, and a NaN stays one (minimum and maximum keep it).  FUSED (bf16 operands): u + shift is not
+// formed by itself, one instruction less; E is then off by |shift| 2^-24 for the rounding of shift's product.
+template <bool FUSED>
 __device__ __forceinline__ void gates(float u, float shift, float& z, float& q) {
-  const float t = fma_(u, -1.44269504088896341f, shift * -1.44269504088896341f);
+  const float t = FUSED ? fma_(u, -1.44269504088896341f, shift * -1.44269504088896341f) : (u + shift) * -1.44269504088896341f;
   const float E = __builtin_amdgcn_exp2f(__builtin_elementwise_maximum(__builtin_elementwise_minimum(t, 125.f), -125.f));
   z = fast_rcp(1.0f + E);
   q = E * z;
@@ -137,7 +139,7 @@ __device__ __forceinline__ void run_pairs(const ScanArgs& p, long b, int o0, int
   for (int s = 0; s < STEPS; ++s)
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-      gates(u[s][j], p.shift, z[s][j], q[s][j]);
+      gates<BRIEF>(u[s][j], p.shift, z[s][j], q[s][j]);
       if constexpr (!BWD) bb[s][j] = (GATE ? sigmoid1(i[s][j]) : z[s][j]) * phi_of<BRIEF>(c[s][j], p.tanh_c);
     }
 }
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_scan_bwd(ScanArgs p) {
         const float gz = gr * z[s][j];
         if constexpr (GATE) {
           float w, w1;
-          gates(gi[s][j], 0.f, w, w1);
+          gates<true>(gi[s][j], 0.f, w, w1);
           const float gw = gr * w;
           du[j] = -gz * q[s][j] * before;
           di[j] = gw * phi * w1;

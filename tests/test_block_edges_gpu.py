@@ -55,6 +55,20 @@ def test_a_decay_that_is_all_but_shut(hip, dt):
   close(dc, torch.sigmoid(x), rel, 'dc')
 
 
+@pytest.mark.parametrize('shift', [-96.0, 31.0, 5.3])
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_shifts_that_cancel(hip, dt, shift):
+  """Gates near their middle and far from it whose operand and shift are both large."""
+  v = torch.arange(-24, 25, dtype=F32) / 2
+  u = (v - shift)[None].to(dt)
+  D = v.numel()
+  h, hT = torch.zeros(1, D, device='cuda', dtype=dt), torch.zeros(1, D, device='cuda')
+  hip.gated_scan_fwd(u.cuda(), torch.zeros(1, D, device='cuda', dtype=dt), h, 1, h0=torch.ones(1, D, device='cuda'), hT=hT, shift=shift, cand=None)
+  x = u.double() + float(torch.tensor(shift))
+  # as in test_a_decay_that_is_all_but_shut, the sum's rounding in the exponent; bf16: the rounding of shift's product
+  close(hT, torch.sigmoid(-x), (2.5 * x.abs() + 10 + (abs(shift) if dt == BF16 else 0.0)) * U, 'hT')
+
+
 @pytest.mark.parametrize('gate', [False, True])
 @pytest.mark.parametrize('dt', [F32, BF16])
 def test_small_candidates(hip, dt, gate):
