@@ -153,15 +153,15 @@ def load_library():
         f'{_LIB_PATH} not found: build it with __graft_entry__.build() '
         f'(make -C daydreamer_amd/csrc).  There is no fallback path.')
   lib = ctypes.CDLL(str(_LIB_PATH))
+  lib.dd_version.restype = c_i
+  lib.dd_last_error.restype = ctypes.c_char_p
+  if lib.dd_version() != ABI_VERSION:   # a stale build: the signatures may not match
+    raise RuntimeError(f'{_LIB_PATH} has ABI version {lib.dd_version()}, this binding needs '
+                       f'{ABI_VERSION}: rebuild it (make -C daydreamer_amd/csrc)')
   for name, args in _SIGS.items():
     fn = getattr(lib, name)
     fn.argtypes = args
     fn.restype = c_i
-  lib.dd_version.restype = c_i
-  lib.dd_last_error.restype = ctypes.c_char_p
-  if lib.dd_version() != ABI_VERSION:   # a stale build: signatures below may not match
-    raise RuntimeError(f'{_LIB_PATH} has ABI version {lib.dd_version()}, this binding needs '
-                       f'{ABI_VERSION}: rebuild it (make -C daydreamer_amd/csrc)')
   global _block
   try:   # native binding of the residual recurrent block (csrc/block_bind.cpp); nothing else needs it
     from . import _block

@@ -78,3 +78,13 @@ def test_plans_of_products():
   assert ask(2, 37500, 1024, 2048)[3] > 1 and ask(2, 37500, 1024, 2048, ws=0)[3] == 1   # no room, no split
   assert 'dd_linear_plan' in ask(1, 8, 8, 8, type=2) and 'dd_linear_plan' in ask(0, 0, 8, 8)
   assert 'dd_linear_plan' in ask(3, 8, 8, 8) and 'dd_linear_plan' in ask(0, 8, 8, 8, type=0) and 'dd_linear_plan' in ask(0, 8, 8, 8, act=9)
+
+
+def test_a_library_of_another_version_is_named(tmp_path, monkeypatch):
+  """A build that lacks the newest entry points is refused for its version, before they are looked up."""
+  (tmp_path / 'old.c').write_text('int dd_version(void) { return 7; }\nconst char* dd_last_error(void) { return ""; }\n')
+  subprocess.run(['gcc', '-shared', '-fPIC', str(tmp_path / 'old.c'), '-o', str(tmp_path / 'old.so')], check=True)
+  monkeypatch.setattr(hipops, '_LIB_PATH', tmp_path / 'old.so')
+  monkeypatch.setattr(hipops, '_lib', None)
+  with pytest.raises(RuntimeError, match='ABI version 7'):
+    hipops.load_library()
