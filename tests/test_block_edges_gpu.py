@@ -456,10 +456,13 @@ def test_sum_over_x(hip, C, t):
 
 
 @pytest.mark.parametrize('over', [False, True])
-@pytest.mark.parametrize('rows,C,slots', [(120001, 64, 1536 * 32), (50001, 17, 1536 * 32), (13001, 300, 1536 * 4), (7001, 1000, 768 * 4),
-                                          (4001, 1542, 1536), (2001, 2500, 768), (700, 8101, 256), (701, 9001, 256), (600, 20001, 256)])
-def test_norm_gradients_of_many_rows(hip, rows, C, slots, over):
-  """More rows than are in flight at once, no multiple of them: a workgroup goes round its loop two or three times."""
+@pytest.mark.parametrize('rows,C,workgroups,per', [
+    (120001, 64, 1536, 32), (50001, 17, 1536, 32), (13001, 300, 1536, 4), (7001, 1000, 768, 4), (4001, 1542, 1536, 1),
+    (2001, 2500, 768, 1), (700, 8101, 256, 1), (701, 9001, 256, 1), (600, 20001, 256, 1)])
+def test_norm_gradients_of_many_rows(hip, rows, C, workgroups, per, over):
+  """More rows than are in flight at once (`per` of a workgroup), no multiple of them: a workgroup goes round its loop two
+  or three times."""
+  slots = workgroups * per
   assert rows > slots and rows % slots
   for t in (F32, BF16):
     s, dy, dres, g = on_gpu(rows, C, seed=1, dtype=t), on_gpu(rows, C, seed=2, dtype=BF16), on_gpu(rows, C, seed=3, dtype=t), 1 + on_gpu(C, seed=4, scale=0.1)
@@ -474,8 +477,7 @@ def test_norm_gradients_of_many_rows(hip, rows, C, slots, over):
     # the row's mean: 32 elements of a lane, 6 steps over a wave, 16 waves
     near(ds.t, dres.double() + inv * (dn - n * (dn * n).mean(1, keepdim=True)), 64 * U * size, 'ds')
     # dgamma: the rows of a lane, up to 32 rows of a workgroup, the workgroups in 32 runs and then those; n and a product
-    per = slots // (1536 if C <= 512 or 1024 < C <= 2048 else 768 if C <= 4096 else 256)
-    chain = rows / slots + 1 + per + slots / per / 32 + 32 + 4
+    chain = rows / slots + 1 + per + workgroups / 32 + 32 + 4
     near(dgamma, (d * n).sum(0), chain * U * (d * n).abs().sum(0), 'dgamma')
     ds.whole('ds')
 
